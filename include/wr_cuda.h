@@ -234,6 +234,73 @@ int wr_cuda_attn_prefill(wr_cuda_ctx *ctx, wr_cuda_kv *kv, uint32_t layer,
                          float *out, uint32_t n_q_heads, float scale_override,
                          uint32_t window, int mem);
 
+/* ---- sessions that go on from one another (no reference counterpart: a session of
+ * the reference owns its slab, session.c:640-733, and nothing forks) --------- */
+
+/* A new session that stands where `kv` stood after its first n_rows rows.  The two
+ * hold the pages of 64 tokens that those rows fill together; the rows behind them
+ * are copied (enqueued), and so is the recurrent state, which has to stand at
+ * n_rows (WR_CUDA_ERR_STATE).  A fork can be forked again.  While more than one
+ * session holds a page nobody may write it: an append, a write_rows or a
+ * forward pass that would is WR_CUDA_ERR_STATE before anything runs.  Destroying a
+ * session gives back what no other holds.  Takes memory for the fork's own
+ * pages; not while the context's stream is being captured (WR_CUDA_ERR_STATE). */
+int wr_cuda_kv_fork(wr_cuda_ctx *ctx, wr_cuda_kv *kv, uint32_t n_rows, wr_cuda_kv **out);
+/* Leading rows whose pages both hold, a multiple of WR_CUDA_PAGE_TOKENS. */
+uint32_t wr_cuda_kv_shared_rows(const wr_cuda_kv *a, const wr_cuda_kv *b);
+
+/* The caches of n <= WR_CUDA_BATCH_MAX sessions follow a search's choice: afterwards
+ * kv[i] holds what kv[parents[i]] held, rows[parents[i]] rows (rows[i]: what kv[i] holds
+ * before; a recurrent state has to stand there).  All at once, so parents may name each other.
+ * A parent's first child takes its memory over, the others copy the rows that
+ * are not shared into what sessions without children held: n sessions of one
+ * family (forks, equal max_ctx and layers; WR_CUDA_ERR_INVAL), whose own rows
+ * nobody outside the call holds (WR_CUDA_ERR_STATE).  Enqueues on the context's
+ * stream and allocates nothing.  A refused call changes nothing.  Launches that a
+ * graph has captured name the memory, not the session: they are captured again after
+ * this call, and while the context's stream is being captured it is WR_CUDA_ERR_STATE. */
+int wr_cuda_kv_reorder(wr_cuda_ctx *ctx, uint32_t n, wr_cuda_kv *const *kv, const uint32_t *parents,
+                       const uint32_t *rows);
+
+/* wr_cuda_attn_decode for sessions that share their first rows: each group's shared
+ * keys are fetched once for all of its sessions.  kv lists group after group:
+ * group g is the next group_sess[g] sessions, which hold the pages of the first
+ * group_rows[g] rows together (a multiple of WR_CUDA_PAGE_TOKENS, at most the shortest
+ * seq_len; 0, or a group of one session, shares nothing).  Same checks and the same
+ * values as wr_cuda_attn_decode, to rounding: F32 queries and F32 sums, and the order of
+ * the sums hangs on all lengths of the call.  head_dim 128 only
+ * (WR_CUDA_ERR_UNSUPPORTED), no window.  Scratch is kept by the context and grows with the
+ * call: make the largest call once before capturing one.  Calls of one context share it, so
+ * graphs that hold such calls are launched one after another. */
+int wr_cuda_attn_decode_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer,
+                               const uint32_t *seq_lens, uint32_t n_groups, const uint32_t *group_sess,
+                               const uint32_t *group_rows, const float *q, float *out,
+                               uint32_t n_q_heads, float scale_override, int mem);
+
+/* wr_cuda_decode_step for such sessions: wr_cuda_kv_append with n_tokens = 1, then
+ * wr_cuda_attn_decode_shared over positions[s] + 1 rows; group_rows[g] is at most the
+ * smallest position.  Host q rows are left as given. */
+int wr_cuda_decode_step_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer,
+                               const uint32_t *positions, uint32_t n_groups, const uint32_t *group_sess,
+                               const uint32_t *group_rows, float *q, const float *k_rows,
+                               const float *v_rows, float *out, uint32_t n_q_heads, float theta_base,
+                               uint32_t n_rot_pairs, uint32_t flags, float scale_override, int mem);
+
+/* A beam search's choice (no reference counterpart; the reference samples one row,
+ * src/core/sample.c:239).  Per group (request) the n_out best of its beams'
+ * continuations by score + log softmax(logits), in descending order; equal ones go to
+ * the lower beam, then the lower token.  logits: F32 [n_groups][beams][vocab], scores:
+ * F32 [n_groups][beams] (a beam at -inf or NaN has ended and its row is not read);
+ * out_*: [n_groups][n_out].  Tokens with a logit of -inf are no continuations, nor is any of a row
+ * with a NaN or +inf; places for which there is none hold score -inf, beam and token
+ * 0xffffffff.  Totals are compared in 64 bits and returned in F32.  beams <=
+ * WR_CUDA_BATCH_MAX, n_out <= WR_CUDA_BEAM_MAX_OUT, n_groups * beams <= 65535
+ * (WR_CUDA_ERR_LIMIT).  Scratch as wr_cuda_attn_decode_shared. */
+#define WR_CUDA_BEAM_MAX_OUT 32
+int wr_cuda_beam_select(wr_cuda_ctx *ctx, uint32_t n_groups, uint32_t beams, uint32_t vocab,
+                        const float *logits, const float *scores, uint32_t n_out,
+                        float *out_scores, uint32_t *out_beams, uint32_t *out_tokens, int mem);
+
 /* ---- split-KV across devices --------------------------------------------- */
 
 /* Like wr_cuda_attn_decode over this device's shard of each session's keys,
@@ -381,6 +448,16 @@ int wr_cuda_model_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t
                           const uint32_t *tokens, uint32_t out_from, float *hidden_out,
                           float *normed_out, float *const *logits_out, uint32_t *argmax_out,
                           float *attn_tap_out);
+
+/* One step of beam searches: a decode pass (as wr_cuda_model_forward, WR_CUDA_FWD_DECODE) of
+ * n_groups * beams <= WR_CUDA_BATCH_MAX rows, then wr_cuda_beam_select on its logits, which
+ * stay on the device.  Either kind of model.  scores and out_* are host memory; kv,
+ * positions and tokens are as for the pass.  Sessions of the dense stack that hold pages together
+ * attend to them together where those are long enough to pay. */
+int wr_cuda_model_beam_step(wr_cuda_ctx *ctx, wr_cuda_model *m, uint32_t n_groups, uint32_t beams,
+                            wr_cuda_kv *const *kv, const uint32_t *positions, const uint32_t *tokens,
+                            const float *scores, uint32_t n_out, float *out_scores,
+                            uint32_t *out_beams, uint32_t *out_tokens);
 
 /* ---- models whose layers differ ------------------------------------------- */
 

@@ -1,0 +1,168 @@
+"""GPU: wr_cuda_beam_select against a 64-bit restatement."""
+import numpy as np
+import pytest
+
+from _plain_beams import NONE, choose, choose_error
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    import wayruntime_b200 as wr
+    c = wr.Context(0)
+    yield c
+    c.close()
+
+
+def run(ctx, logits, scores, n_out, device=True, offset=0):
+    import torch
+    groups = logits.shape[0]
+    if not device:
+        out = np.full((groups, n_out), np.nan, np.float32), np.zeros((groups, n_out), np.uint32), np.zeros((groups, n_out), np.uint32)
+        ctx.beam_select(np.ascontiguousarray(logits), np.ascontiguousarray(scores), *out)
+        return out
+    room = torch.empty(logits.size + offset, dtype=torch.float32, device="cuda")
+    lg = room[offset:].view(logits.shape)
+    lg.copy_(torch.from_numpy(logits))
+    out = (torch.full((groups, n_out), float("nan"), device="cuda"), torch.zeros((groups, n_out), dtype=torch.int32, device="cuda"),
+           torch.zeros((groups, n_out), dtype=torch.int32, device="cuda"))
+    sc = torch.from_numpy(scores).cuda()
+    torch.cuda.synchronize()
+    ctx.beam_select(lg, sc, *out)
+    ctx.sync()
+    s, b, t = (x.cpu().numpy() for x in out)
+    return s, b.view(np.uint32), t.view(np.uint32)
+
+
+def check(got, logits, scores, n_out):
+    want = choose(logits, scores, n_out)
+    assert np.array_equal(got[1], want[1]) and np.array_equal(got[2], want[2])
+    there = want[1] != NONE
+    assert np.array_equal(np.isneginf(got[0]), ~there)
+    assert (np.abs(got[0][there] - want[0][there]) <= choose_error(want[0], logits.shape[2])[there]).all()
+
+
+def rows(seed, groups, beams, vocab, spread=2.5):
+    rng = np.random.default_rng(seed)
+    return ((rng.standard_normal((groups, beams, vocab)) * spread).astype(np.float32),
+            (-20 - np.abs(rng.standard_normal((groups, beams)))).astype(np.float32))
+
+
+@pytest.mark.parametrize("groups, beams, vocab, n_out", [
+    (1, 1, 1, 1), (1, 1, 1, 32), (1, 2, 3, 4), (2, 3, 31, 7), (1, 1, 4093, 2), (1, 1, 4096, 8), (3, 2, 4097, 4), (2, 5, 8191, 10),
+    (1, 4, 32003, 8), (1, 16, 12289, 32), (4, 4, 50257, 8), (1, 1, 151936, 16), (1, 3, 151936, 17), (40, 8, 1000, 16),
+    (130, 16, 515, 32), (1, 16, 65536, 32)])
+def test_choice(ctx, groups, beams, vocab, n_out):
+    logits, scores = rows(groups * 1000 + vocab, groups, beams, vocab)
+    check(run(ctx, logits, scores, n_out), logits, scores, n_out)
+
+
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_rows_at_any_alignment(ctx, offset):
+    logits, scores = rows(offset, 2, 3, 10001)
+    check(run(ctx, logits, scores, 6, offset=offset), logits, scores, 6)
+
+
+def test_host_buffers(ctx):
+    logits, scores = rows(5, 2, 4, 9999)
+    check(run(ctx, logits, scores, 8, device=False), logits, scores, 8)
+
+
+@pytest.mark.parametrize("vocab, n_out", [(5, 8), (6000, 8), (6000, 32), (40000, 3)])
+def test_ties_go_to_the_lower_beam_then_the_lower_token(ctx, vocab, n_out):
+    logits = np.zeros((2, 3, vocab), np.float32)                   # every candidate of a group is equal
+    scores = np.full((2, 3), -1.0, np.float32)
+    check(run(ctx, logits, scores, n_out), logits, scores, n_out)
+    rng = np.random.default_rng(vocab)                              # few different values, both zeros among them
+    logits = rng.choice(np.array([-1.0, -0.0, 0.0, 0.5], np.float32), (2, 3, vocab))
+    check(run(ctx, logits, scores, n_out), logits, scores, n_out)
+
+
+def test_rows_in_ascending_and_descending_order(ctx):
+    logits = np.stack([np.linspace(-9, 9, 20000), np.linspace(9, -9, 20000)]).astype(np.float32)[None]
+    scores = np.array([[-3.0, -3.0]], np.float32)
+    got = run(ctx, logits, scores, 16)
+    want = choose(logits, scores, 16)
+    assert np.array_equal(got[2], want[2]) and np.array_equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("n_out", [4, 20, 32])
+def test_the_best_lie_together(ctx, n_out):
+    logits, scores = rows(77, 1, 2, 30000)
+    logits[0, 1, 12000:12700] += 30                                 # (700 large ones, all in one part of the row)
+    check(run(ctx, logits, scores, n_out), logits, scores, n_out)
+
+
+def test_what_is_masked_ended_or_not_a_number_has_no_continuation(ctx):
+    logits, scores = rows(9, 6, 3, 5000)
+    logits[0, :, 7:] = -np.inf                                      # seven tokens a beam
+    logits[1] = -np.inf                                             # a row that a mask leaves nothing of
+    scores[2, 1] = -np.inf                                          # an ended beam
+    scores[3] = np.nan
+    logits[4, 0, 4999] = np.nan
+    logits[4, 1, 0] = np.inf
+    scores[5, 0] = np.inf
+    logits[2, 0, ::2] = np.finfo(np.float32).min                    # a mask of the type's lowest value
+    got = run(ctx, logits, scores, 24)
+    check(got, logits, scores, 24)
+    assert (got[1][1] == NONE).all() and (got[1][3] == NONE).all() and (got[1][2] != 1).all()
+    assert (got[1][0] != NONE).sum() == 21 and set(got[1][4]) == {2}
+
+
+def test_an_ended_beams_row_is_not_read(ctx):
+    """Its address may be anything the buffer covers; here NaN, which would take every candidate out if it were read."""
+    logits, scores = rows(10, 1, 2, 3000)
+    logits[0, 0] = np.nan
+    scores[0, 0] = -np.inf
+    check(run(ctx, logits, scores, 4), logits, scores, 4)
+
+
+def test_same_bits_every_time(ctx):
+    logits, scores = rows(11, 3, 5, 40000)
+    first = run(ctx, logits, scores, 10)
+    for _ in range(20):
+        assert all(np.array_equal(a, b) for a, b in zip(first, run(ctx, logits, scores, 10)))
+
+
+def test_captured_in_a_graph(ctx):
+    import torch
+    logits, scores = rows(12, 1, 4, 20011)
+    lg, sc = torch.from_numpy(logits).cuda(), torch.from_numpy(scores).cuda()
+    out = (torch.zeros((1, 8), device="cuda"), torch.zeros((1, 8), dtype=torch.int32, device="cuda"),
+           torch.zeros((1, 8), dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+    ctx.beam_select(lg, sc, *out)
+    ctx.sync()
+    stream, graph = torch.cuda.ExternalStream(ctx.stream), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        ctx.beam_select(lg, sc, *out)
+    big, small = rows(13, 16, 16, 60000)                            # the scratch grows between capture and launch
+    run(ctx, big, small, 32)
+    other, _ = rows(14, 1, 4, 20011)
+    lg.copy_(torch.from_numpy(other))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        graph.replay()
+    ctx.sync()
+    check((out[0].cpu().numpy(), out[1].cpu().numpy().view(np.uint32), out[2].cpu().numpy().view(np.uint32)), other, scores, 8)
+
+
+def test_refusals(ctx):
+    import wayruntime_b200 as wr
+    logits, scores = rows(1, 1, 2, 10)
+    out = lambda n: (np.zeros((1, n), np.float32), np.zeros((1, n), np.uint32), np.zeros((1, n), np.uint32))  # noqa: E731
+    for bad_logits, bad_scores, n, status in ((logits, scores, 33, -8), (np.zeros((1, 17, 10), np.float32), np.zeros((1, 17), np.float32), 4, -8),
+                                              (np.zeros((1, 2, 0), np.float32), scores, 4, -4)):
+        with pytest.raises(wr.WrCudaError) as e:
+            ctx.beam_select(bad_logits, bad_scores, *out(n))
+        assert e.value.status == status
+    with pytest.raises(ValueError):
+        ctx.beam_select(logits, scores[:, :1], *out(4))
+    with pytest.raises(ValueError):
+        ctx.beam_select(logits.astype(np.float64), scores, *out(4))
+    lib = ctx._lib
+    p = logits.ctypes.data
+    assert lib.wr_cuda_beam_select(ctx._h, 70000, 1, 1, p, p, 1, p, p, p, 0) == -8
+    assert lib.wr_cuda_beam_select(ctx._h, 1, 1, 1, None, p, 1, p, p, p, 0) == -4
+    assert lib.wr_cuda_beam_select(ctx._h, 1, 1, 1, p, p, 1, p, p, p, 2) == -4

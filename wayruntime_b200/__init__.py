@@ -9,6 +9,7 @@ from .binding import (  # noqa: F401
     Batch,
     Exchange,
     Context,
+    Groups,
     DeviceModel,
     MixedModel,
     KVCache,
@@ -26,6 +27,6 @@ from .binding import (  # noqa: F401
 )
 
 __all__ = [
-    "Batch", "Context", "DeviceModel", "Exchange", "KVCache", "MixedModel", "WrCudaError", "MEM_DEVICE", "MEM_HOST", "F16", "F32", "BF16",
+    "Batch", "Context", "DeviceModel", "Exchange", "Groups", "KVCache", "MixedModel", "WrCudaError", "MEM_DEVICE", "MEM_HOST", "F16", "F32", "BF16",
     "APPEND_ROPE", "TRIPLE_PAD", "device_check", "load_library", "status_name",
 ]

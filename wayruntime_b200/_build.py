@@ -18,7 +18,8 @@ INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 
 SOURCES = ["kv_cache.cu", "attn_decode.cu", "attn_decode_static.cu", "attn_prefill.cu", "attn_exchange.cu",
            "model_glue.cu", "attn_step_small.cu", "gemv.cu", "gemm_f32.cu", "gemm_bf16.cu", "gemm_skinny.cu", "mixers.cu", "latent.cu", "attn_latent.cu",
-           "moe.cu", "model_mixed.cu"]
+           "moe.cu", "model_mixed.cu",
+           "attn_shared.cu", "kv_share.cu", "beam.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",

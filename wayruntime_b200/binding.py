@@ -24,6 +24,9 @@ F32, F16, BF16 = 0, 1, 2
 APPEND_ROPE = 1
 TRIPLE_PAD = 4
 BATCH_MAX = 16
+PAGE_TOKENS = 64
+BEAM_MAX_OUT = 32
+NO_BEAM = 0xFFFFFFFF            # beam and token where there is no continuation
 
 _STATUS = {
     0: "WR_OK", -3: "WR_ERR_UNSUPPORTED", -4: "WR_ERR_INVAL", -5: "WR_ERR_NOMEM",
@@ -45,6 +48,8 @@ EXPORTS = [
     "wr_cuda_model_create", "wr_cuda_model_destroy", "wr_cuda_model_bytes", "wr_cuda_model_launches", "wr_cuda_model_last_enqueue_ns",
     "wr_cuda_model_forward", "wr_cuda_kv_create_layout", "wr_cuda_model_create_mixed", "wr_cuda_model_kv_create",
     "wr_cuda_model_set_hidden_tap",
+    "wr_cuda_kv_fork", "wr_cuda_kv_shared_rows", "wr_cuda_kv_reorder", "wr_cuda_attn_decode_shared", "wr_cuda_decode_step_shared",
+    "wr_cuda_beam_select", "wr_cuda_model_beam_step",
 ]
 
 
@@ -178,6 +183,15 @@ def load_library():
         "wr_cuda_model_create_mixed": (i32, [vp, C.POINTER(MixedDesc), C.POINTER(vp)]),
         "wr_cuda_model_kv_create": (i32, [vp, vp, u32, C.POINTER(vp)]),
         "wr_cuda_model_set_hidden_tap": (i32, [vp, vp]),
+        "wr_cuda_kv_fork": (i32, [vp, vp, u32, C.POINTER(vp)]),
+        "wr_cuda_kv_shared_rows": (u32, [vp, vp]),
+        "wr_cuda_kv_reorder": (i32, [vp, u32, C.POINTER(vp), C.POINTER(u32), C.POINTER(u32)]),
+        "wr_cuda_attn_decode_shared": (i32, [vp, u32, C.POINTER(vp), u32, C.POINTER(u32), u32, C.POINTER(u32), C.POINTER(u32),
+                                             vp, vp, u32, f32, i32]),
+        "wr_cuda_decode_step_shared": (i32, [vp, u32, C.POINTER(vp), u32, C.POINTER(u32), u32, C.POINTER(u32), C.POINTER(u32),
+                                             vp, vp, vp, vp, u32, f32, u32, u32, f32, i32]),
+        "wr_cuda_beam_select": (i32, [vp, u32, u32, u32, vp, vp, u32, vp, vp, vp, i32]),
+        "wr_cuda_model_beam_step": (i32, [vp, vp, u32, u32, C.POINTER(vp), C.POINTER(u32), C.POINTER(u32), vp, u32, vp, vp, vp]),
         "wr_cuda_model_forward": (i32, [vp, vp, i32, u32, C.POINTER(vp), C.POINTER(u32), C.POINTER(u32), u32,
                                         vp, vp, C.POINTER(vp), C.POINTER(u32), vp]),
     }
@@ -461,6 +475,53 @@ class Context:
         rc = self._lib.wr_cuda_attn_combine(self._h, n_shards, n_rows, head_dim, tp, op, mem)
         _check(rc, "wr_cuda_attn_combine")
 
+    def attn_decode_shared(self, kvs, layer, seq_lens, groups, q, out, n_q_heads, scale=0.0):
+        """wr_cuda_attn_decode_shared: attn_decode for sessions that share their first rows.  groups: for each group, in the
+        order of kvs, (sessions, rows that they share) — a list, or a Groups built once."""
+        qp, qm, _q = _buf(q)
+        op, om, _o = _buf(out)
+        g = Groups.of(groups, len(kvs))
+        _check(self._lib.wr_cuda_attn_decode_shared(self._h, len(kvs), self._handles(kvs), layer, self._u32s(seq_lens), len(g),
+                                                    g.sessions, g.rows, qp, op, n_q_heads, scale, _same_mem(qm, om)),
+               "wr_cuda_attn_decode_shared")
+
+    def decode_step_shared(self, kvs, layer, positions, groups, q, k_rows, v_rows, out, n_q_heads, theta=10000.0,
+                           n_rot_pairs=0, rope=True, scale=0.0):
+        """wr_cuda_decode_step_shared: decode_step for sessions that share their first rows (groups as in attn_decode_shared)."""
+        qp, qm, _q = _buf(q)
+        kp, km, _k = _buf(k_rows)
+        vp, vm, _v = _buf(v_rows)
+        op, om, _o = _buf(out)
+        g = Groups.of(groups, len(kvs))
+        _check(self._lib.wr_cuda_decode_step_shared(self._h, len(kvs), self._handles(kvs), layer, self._u32s(positions), len(g),
+                                                    g.sessions, g.rows, qp, kp, vp, op, n_q_heads, theta, n_rot_pairs,
+                                                    APPEND_ROPE if rope else 0, scale, _same_mem(qm, km, vm, om)),
+               "wr_cuda_decode_step_shared")
+
+    def kv_reorder(self, kvs, parents, rows):
+        """wr_cuda_kv_reorder: kvs[i] goes on from what kvs[parents[i]] holds; rows[i]: rows that kvs[i] holds before."""
+        if len(parents) != len(kvs) or len(rows) != len(kvs):
+            raise ValueError("one parent and one number of rows per session")
+        _check(self._lib.wr_cuda_kv_reorder(self._h, len(kvs), self._handles(kvs), self._u32s(parents), self._u32s(rows)),
+               "wr_cuda_kv_reorder")
+
+    def beam_select(self, logits, scores, out_scores, out_beams, out_tokens):
+        """wr_cuda_beam_select: the best continuations of every group.  logits: float32 [groups, beams, vocab], scores: float32
+        [groups, beams]; out_scores float32, out_beams and out_tokens 32-bit integers, [groups, n_out] each (0xffffffff, or -1,
+        where there is no continuation)."""
+        groups, beams, vocab = logits.shape
+        if tuple(scores.shape) != (groups, beams):
+            raise ValueError("scores: one per row of logits")
+        if any(tuple(x.shape) != tuple(out_scores.shape) for x in (out_beams, out_tokens)) or out_scores.shape[0] != groups:
+            raise ValueError("results: [groups, n_out] each")
+        for x, kind in ((logits, "float32"), (scores, "float32"), (out_scores, "float32"), (out_beams, "int32"), (out_tokens, "int32")):
+            if not str(x.dtype).endswith(kind):                  # (uint32 too)
+                raise ValueError(f"{kind} expected, got {x.dtype}")
+        bufs = [_buf(x) for x in (logits, scores, out_scores, out_beams, out_tokens)]
+        (lp, sp, a, b, t), mem = (x[0] for x in bufs), _same_mem(*(x[1] for x in bufs))
+        _check(self._lib.wr_cuda_beam_select(self._h, groups, beams, vocab, lp, sp, out_scores.shape[1], a, b, t, mem),
+               "wr_cuda_beam_select")
+
     def attn_prefill(self, kv, layer, p0, n, q, out, n_q_heads, scale=0.0, window=0):
         qp, qm, qa = _buf(q)
         op, om, _o = _buf(out)
@@ -642,6 +703,20 @@ class DeviceModel:
         return res
 
 
+    def beam_step(self, kvs, positions, tokens, scores, n_out):
+        """wr_cuda_model_beam_step: one token for every beam, then the n_out best continuations of every group.  scores: float32
+        [groups, beams], the rows of kvs, positions and tokens in that order.  Returns (scores, beams, tokens), [groups, n_out] each."""
+        scores = np.ascontiguousarray(scores, np.float32)
+        groups, beams = scores.shape
+        if not len(kvs) == len(positions) == len(tokens) == scores.size:
+            raise ValueError("one session, position and token per score")
+        out = np.empty((groups, n_out), np.float32), np.empty((groups, n_out), np.uint32), np.empty((groups, n_out), np.uint32)
+        _check(self._lib.wr_cuda_model_beam_step(
+            self._ctx._h, self._h, groups, beams, Context._handles(kvs), Context._u32s(positions), Context._u32s(tokens),
+            scores.ctypes.data, n_out, *(x.ctypes.data for x in out)), "wr_cuda_model_beam_step")
+        return out
+
+
 class MixedModel(DeviceModel):
     """wr_cuda_model of the mixed kind (wr_cuda_model_create_mixed).  `layers` is a list of dicts with the
     scalar fields of wr_cuda_mixed_layer; `tensor(i, field)` returns layer i's array for a tensor field (or None;
@@ -706,6 +781,25 @@ class Batch:
         return (C.c_uint32 * len(vals))(*[int(v) for v in vals])
 
 
+class Groups:
+    """How a fixed list of sessions shares its first rows, built once (see Context.attn_decode_shared)."""
+
+    def __init__(self, groups):
+        self.sessions = Batch.u32([n for n, _ in groups])
+        self.rows = Batch.u32([rows for _, rows in groups])
+        self.total = sum(self.sessions)
+
+    def __len__(self):
+        return len(self.sessions)
+
+    @classmethod
+    def of(cls, groups, n_sessions):
+        g = groups if isinstance(groups, cls) else cls(groups)
+        if g.total != n_sessions:
+            raise ValueError("the groups' sessions are those of the call")
+        return g
+
+
 class KVCache:
     """One session's paged F16 K/V cache (wr_cuda_kv)."""
 
@@ -736,6 +830,19 @@ class KVCache:
             self.close()
         except Exception:
             pass
+
+    def fork(self, n_rows) -> "KVCache":
+        """A session that goes on from this one's first n_rows rows (wr_cuda_kv_fork): full pages are held together, the
+        rows behind them copied."""
+        h = C.c_void_p()
+        _check(self._lib.wr_cuda_kv_fork(self._ctx._h, self._h, n_rows, C.byref(h)), "wr_cuda_kv_fork")
+        kv = KVCache._of_handle(self._ctx, h, self.max_ctx)
+        kv.n_layers, kv.n_kv_heads, kv.head_dim = self.n_layers, self.n_kv_heads, self.head_dim
+        return kv
+
+    def shared_rows(self, other) -> int:
+        """Leading rows whose pages both sessions hold."""
+        return int(self._lib.wr_cuda_kv_shared_rows(self._h, other._h))
 
     def write_rows(self, layer, which, row0, rows):
         """rows: uint16/float16 [n, n_kv_heads, head_dim] in the reference's row layout."""

@@ -1,0 +1,734 @@
+// attn_shared.cu — decode attention for sessions whose first rows are the same pages (a batch behind one prompt, the beams
+// of a search), on the tensor cores.
+//
+// A row of the result is softmax(scale q K^T) V over the session's keys, and the keys fall into two parts: those that the
+// sessions of a group share, and the session's own behind them.  For any split of the keys
+//     m = max of the parts' m_i,   l = sum of 2^(m_i - m) l_i,   o = sum of 2^(m_i - m) o_i / l
+// (m_i the largest score of a part, in powers of two, l_i and o_i its sums against it), so the shared part is worked out once
+// for all queries of the group: a page is fetched from HBM once for up to 64 of them.
+//
+// A SEGMENT is a run of keys with the queries that attend it: per kv head the queries of all sessions of a group (shared
+// rows), or of one session (its own rows).  A segment is cut into chunks; a WORK ITEM is (segment, chunk, kv head, 64 of its
+// queries).  Persistent CTAs, one per SM, draw items from a counter, longest first; shared_merge_kernel adds the chunks
+// of a row up in order, so results do not hang on who worked what out.  Operands are swapped, as in attn_latent.cu: keys
+// (128, two pages) are the tensor core's M, queries its N, so a tile costs what its queries cost.  Per tile
+//   * two loading warps bring K and V in with linear bulk copies (a page's blocks are the operand's layout);
+//   * one warp issues S^T[key][query] = K . Q^T and O^T[dim][query] = V^T . P^T; the scores of the next tile are issued
+//     before this tile's values, so both buffers of S are in use;
+//   * four warps, a thread per key: exponentials against a running reference, P^T to shared memory (queries contiguous:
+//     the MN-major operand, a thread writes 16 bytes at a time); then, a thread per value dimension, the tile's O^T is added
+//     to sums in registers.  The reference moves when a score is more than 2^8 above it: the threads vote, and only then
+//     is the maximum over keys worked out (a segment's first tile always does).
+// Queries and probabilities are split in two F16 numbers (22 bits; queries against a power of two of their row), two
+// products each, the small one first: F32 rows come in and go out, and one F16 rounding of either would leave 2^-12.  Sums of
+// one tile stay in the tensor core's accumulator (8 steps of 16 keys behind the small ones), longer ones are F32 additions in
+// registers: the accumulator rounds towards zero, which over a long chunk would show.
+// Every wait is bounded by the context's wait limit.
+#include <algorithm>
+
+#include "kv_share.cuh"
+#include "tcgen05_dev.cuh"
+#include "warp_reduce.cuh"
+
+namespace {
+
+constexpr uint32_t kHd = 128, kTile = 128, kMaxQ = 64, kThreads = 224;
+constexpr uint32_t kPageBlock = kPageTokens * kHd * 2, kSlot = 2 * kPageBlock;   // K or V of a page, of a tile
+constexpr uint32_t kBox = kTile * 128, kQBox = kMaxQ * 128;                      // 64 dims of a tile's keys, of the queries
+constexpr uint32_t kQBytes = 4 * kQBox, kPBytes = 2 * kTile * 128;               // high and low parts
+constexpr uint32_t kKSlots = 2, kVSlots = 3, kItemSlots = 8;
+constexpr uint32_t kTmemCols = 256, kTmemO = 128;                                // two buffers of 64 columns each
+constexpr uint32_t kMaxSegs = 2 * WR_CUDA_BATCH_MAX, kMaxParts = 1024;
+constexpr float kGrow = 8.0f, kLog2e = 1.4426950408889634f;
+
+struct Segment {
+    const uint64_t *pages;               // page table from the segment's first page on
+    uint32_t rows;                       // keys
+    uint32_t row0, queries;              // first session; queries per kv head
+    uint32_t chunks, qtiles, item0, part0;
+};
+struct SharedParams {
+    Segment seg[kMaxSegs];
+    uint8_t group_seg[WR_CUDA_BATCH_MAX], own_seg[WR_CUDA_BATCH_MAX];            // of a session; kMaxSegs: none
+    uint32_t n_segs, items, n_q, n_kv, per;                                      // per: query heads to a kv head
+    const float *q;
+    float *out;
+    float2 *ml;                          // [part]: reference (log2), sum
+    float *o;                            // [part][128]
+    int *sched;                          // next item, CTAs that have left
+    float scale_log2;
+    long long wait_limit;
+    int *err;
+};
+struct Item {
+    const uint64_t *pages;
+    uint32_t tiles, tile0, rows;         // tiles 0: no more work
+    uint32_t row0, kvh, q0, nq;
+    uint32_t part;
+};
+struct Bars {
+    uint64_t k_full[kKSlots], k_free[kKSlots], v_full[kVSlots], v_free[kVSlots];
+    uint64_t q_full, s_full[2], p_full, o_full, drained;
+    uint64_t item_ready[kItemSlots];
+    Item item[kItemSlots];
+    uint32_t tmem;
+    alignas(16) float c[2][kMaxQ];       // per query: score to log2
+    alignas(16) float m[kMaxQ], a[kMaxQ];
+    alignas(16) float red[kMaxQ][4];
+};
+constexpr uint32_t kSmem = kKSlots * kSlot + kVSlots * kSlot + kQBytes + kPBytes + (uint32_t)sizeof(Bars);
+static_assert(kSmem <= 232448, "the CTA's shared memory is 227 KB at most");
+
+__device__ __forceinline__ Item item_of(const SharedParams &p, uint32_t i)
+{
+    Item it{};
+    if (i >= p.items) return it;
+    uint32_t s = 0;
+    while (s + 1 < p.n_segs && i >= p.seg[s + 1].item0) ++s;
+    const Segment &g = p.seg[s];
+    i -= g.item0;
+    it.kvh = i % p.n_kv;
+    i /= p.n_kv;
+    it.q0 = i % g.qtiles * kMaxQ;
+    const uint32_t chunk = i / g.qtiles, tiles = (g.rows + kTile - 1) / kTile;
+    it.tile0 = tiles * chunk / g.chunks;
+    it.tiles = tiles * (chunk + 1) / g.chunks - it.tile0;
+    it.pages = g.pages;
+    it.rows = g.rows;
+    it.row0 = g.row0;
+    it.nq = min(g.queries - it.q0, kMaxQ);
+    it.part = g.part0 + (chunk * p.n_kv + it.kvh) * g.queries + it.q0;
+    return it;
+}
+__device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool group_or(bool x)
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"((uint32_t)x) : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Largest of the warp's 32 lanes for each of 32 values: v[0] holds that of the value whose index is returned.
+__device__ __forceinline__ uint32_t warp_max_32(float (&v)[32], uint32_t lane)
+{
+    uint32_t idx = 0;
+#pragma unroll
+    for (uint32_t o = 16, half = 16; o >= 1; o >>= 1, half >>= 1) {
+        const bool upper = (lane & o) != 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i)
+            if (i < half) {
+                const float send = upper ? v[i] : v[i + half], keep = upper ? v[i + half] : v[i];
+                v[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, o));
+            }
+        if (upper) idx += half;
+    }
+    return idx;
+}
+// kind::f16, F16 x F16 -> F32: V^T (its dims contiguous) times P^T (its queries contiguous)
+__device__ __forceinline__ uint32_t idesc_values(uint32_t n) { return tc5::idesc_f16(128, n) | tc5::kIdescAMnMajor | (1u << 16); }
+
+__global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_constant__ SharedParams p)
+{
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *const ks = smem_raw, *const vs = ks + kKSlots * kSlot, *const qs = vs + kVSlots * kSlot, *const ps = qs + kQBytes;
+    Bars &sm = *reinterpret_cast<Bars *>(ps + kPBytes);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < kKSlots; ++i) {
+            mbar_init(&sm.k_full[i], 1);
+            mbar_init(&sm.k_free[i], 1);
+        }
+        for (uint32_t i = 0; i < kVSlots; ++i) {
+            mbar_init(&sm.v_full[i], 1);
+            mbar_init(&sm.v_free[i], 1);
+        }
+        for (uint32_t i = 0; i < kItemSlots; ++i) mbar_init(&sm.item_ready[i], 1);
+        mbar_init(&sm.q_full, 4);
+        mbar_init(&sm.s_full[0], 1);
+        mbar_init(&sm.s_full[1], 1);
+        mbar_init(&sm.p_full, 4);
+        mbar_init(&sm.o_full, 1);
+        mbar_init(&sm.drained, 1);
+        fence_barrier_init();
+    }
+    if (warp == 1) tc5::alloc(&sm.tmem, kTmemCols);
+    tc5::fence_before();
+    __syncthreads();
+    tc5::fence_after();
+    pdl_wait();
+    pdl_trigger();                       // (only now: what starts early behind this may rely on everything before it)
+    const uint32_t tmem = sm.tmem;
+    const long long limit = p.wait_limit;
+    // Item number `it` of this CTA; the loading warp is at most four items ahead of the slowest reader.
+    auto item_at = [&](uint32_t it, bool &ok, bool whole_warp) -> Item {
+        uint64_t *bar = &sm.item_ready[it % kItemSlots];
+        const uint32_t parity = (it / kItemSlots) & 1;
+        ok = whole_warp ? mbar_wait_warp(bar, parity, limit) : mbar_wait(bar, parity, limit);
+        return ok ? sm.item[it % kItemSlots] : Item{};
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {                                         // work items and K
+            uint32_t n = 0;
+            bool ok = true;
+            uint32_t next = blockIdx.x;
+            for (uint32_t it = 0; ok; ++it) {
+                const Item im = item_of(p, next);
+                sm.item[it % kItemSlots] = im;
+                mbar_arrive(&sm.item_ready[it % kItemSlots]);
+                if (!im.tiles) break;
+                for (uint32_t t = 0; t < im.tiles; ++t, ++n) {
+                    const uint32_t st = n % kKSlots, pg = 2 * (im.tile0 + t);
+                    const uint32_t pages = im.rows > (pg + 1) * kPageTokens ? 2u : 1u;
+                    const char *src[2] = {reinterpret_cast<const char *>(im.pages[pg]), nullptr};
+                    if (pages > 1) src[1] = reinterpret_cast<const char *>(im.pages[pg + 1]);
+                    if (n >= kKSlots && !mbar_wait(&sm.k_free[st], (n / kKSlots - 1) & 1, limit)) {
+                        ok = false;
+                        break;
+                    }
+                    mbar_expect_tx(&sm.k_full[st], pages * kPageBlock);
+                    for (uint32_t g = 0; g < pages; ++g)
+                        for (uint32_t h = 0; h < 2; ++h)
+                            bulk_g2s(ks + st * kSlot + h * kBox + g * 8192, src[g] + wr_block_off(im.kvh, 0, kHd) + h * 8192, 8192,
+                                     &sm.k_full[st]);
+                }
+                if (ok) next = gridDim.x + (uint32_t)atomicAdd(p.sched, 1);
+            }
+            if (!ok) atomicCAS(p.err, 0, 81);
+            // the last CTA to leave makes the counters ready for the next launch
+            __threadfence();
+            if (atomicAdd(p.sched + 1, 1) == (int)gridDim.x - 1) {
+                p.sched[0] = 0;
+                p.sched[1] = 0;
+            }
+            for (uint32_t i = n - min(n, kKSlots); i < n; ++i) (void)mbar_wait(&sm.k_full[i % kKSlots], (i / kKSlots) & 1, limit);
+        }
+        __syncwarp();
+    } else if (warp == 6) {
+        if (lane == 0) {                                         // V
+            uint32_t n = 0;
+            bool ok = true;
+            for (uint32_t it = 0; ok; ++it) {
+                const Item im = item_at(it, ok, false);
+                if (!im.tiles) break;
+                for (uint32_t t = 0; t < im.tiles; ++t, ++n) {
+                    const uint32_t st = n % kVSlots, pg = 2 * (im.tile0 + t);
+                    const uint32_t pages = im.rows > (pg + 1) * kPageTokens ? 2u : 1u;
+                    const char *src[2] = {reinterpret_cast<const char *>(im.pages[pg]), nullptr};
+                    if (pages > 1) src[1] = reinterpret_cast<const char *>(im.pages[pg + 1]);
+                    if (n >= kVSlots && !mbar_wait(&sm.v_free[st], (n / kVSlots - 1) & 1, limit)) {
+                        ok = false;
+                        break;
+                    }
+                    mbar_expect_tx(&sm.v_full[st], pages * kPageBlock);
+                    for (uint32_t g = 0; g < pages; ++g)
+                        bulk_g2s(vs + st * kSlot + g * kPageBlock, src[g] + wr_block_off(im.kvh, 1, kHd), kPageBlock, &sm.v_full[st]);
+                }
+            }
+            if (!ok) atomicCAS(p.err, 0, 82);
+            for (uint32_t i = n - min(n, kVSlots); i < n; ++i) (void)mbar_wait(&sm.v_full[i % kVSlots], (i / kVSlots) & 1, limit);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        const bool lead = tc5::elect_one();
+        const uint32_t q_addr = smem_u32(qs), p_addr = smem_u32(ps), k_addr = smem_u32(ks), v_addr = smem_u32(vs);
+        uint32_t n_s = 0, n_o = 0;                               // tiles scored, multiplied
+        bool ok = true;
+        auto score = [&](uint32_t n) {
+            const uint32_t st = n_s % kKSlots;
+            if (!mbar_wait_warp(&sm.k_full[st], (n_s / kKSlots) & 1, limit)) return false;
+            tc5::fence_after();
+            const uint32_t d = tmem + (n_s & 1) * kMaxQ, idesc = tc5::idesc_f16(128, n);
+            const uint64_t a = tc5::desc_kmajor(k_addr + st * kSlot), b = tc5::desc_kmajor(q_addr);
+#pragma unroll
+            for (uint32_t kk = 0; kk < 16; ++kk) {               // the queries' low parts, then the high ones
+                const uint32_t half = (kk >> 2) & 1, step = 2 * (kk & 3);
+                if (lead) tc5::mma_ss(d, a + half * (kBox >> 4) + step, b + ((kk >> 2) ^ 2) * (kQBox >> 4) + step, idesc, kk != 0);
+            }
+            if (lead) {
+                tc5::commit(&sm.k_free[st]);
+                tc5::commit(&sm.s_full[n_s & 1]);
+            }
+            ++n_s;
+            return true;
+        };
+        for (uint32_t it = 0; ok; ++it) {
+            const Item im = item_at(it, ok, true);
+            if (!im.tiles) break;
+            const uint32_t n = (im.nq + 15) & ~15u;
+            ok = mbar_wait_warp(&sm.q_full, it & 1, limit) && score(n);
+            for (uint32_t t = 0; t < im.tiles && ok; ++t) {
+                // (the scores two tiles ago have been read: their P has been waited for)
+                if (t + 1 < im.tiles) ok = score(n);
+                ok = ok && mbar_wait_warp(&sm.p_full, n_o & 1, limit);
+                const uint32_t st = n_o % kVSlots;
+                ok = ok && mbar_wait_warp(&sm.v_full[st], (n_o / kVSlots) & 1, limit);
+                if (!ok) break;
+                tc5::fence_after();
+                const uint32_t d = tmem + kTmemO + (n_o & 1) * kMaxQ, idesc = idesc_values(n);
+                const uint64_t a = tc5::desc_mnmajor(v_addr + st * kSlot, 8192), b = tc5::desc_mnmajor(p_addr, 8192);
+#pragma unroll
+                for (uint32_t kk = 0; kk < 16; ++kk) {           // 16 keys a step; P's low parts, then the high ones
+                    const uint32_t step = kk & 7;
+                    if (lead)
+                        tc5::mma_ss(d, a + (step >> 2) * (kPageBlock >> 4) + (step & 3) * (2048 >> 4),
+                                    b + ((kk >> 3) ^ 1) * (kTile * 128 >> 4) + step * (2048 >> 4), idesc, kk != 0);
+                }
+                if (lead) {
+                    tc5::commit(&sm.v_free[st]);
+                    tc5::commit(&sm.o_full);
+                }
+                ++n_o;
+            }
+        }
+        if (!ok && lane == 0) atomicCAS(p.err, 0, 83);
+        __syncwarp();
+        if (lead) tc5::commit(&sm.drained);                      // no product is running when the TMEM is given back
+        (void)mbar_wait_warp(&sm.drained, 0, limit);
+    } else {
+        // a thread per key (scores) and per value dimension (output): its TMEM lane either way
+        const uint32_t quarter = warp & 3, key = quarter * 32 + lane, tid = threadIdx.x - 64, lanes = (quarter * 32) << 16;
+        uint32_t n = 0;                                          // tiles so far
+        bool ok = true;
+        // The item's queries as operands: against the power of two of their row, high and low F16 parts.
+        auto queries = [&](const Item &im, uint32_t it) {
+            const uint32_t rows = (im.nq + 15) & ~15u;
+#pragma unroll 1
+            for (uint32_t r0 = tid >> 5; r0 < rows; r0 += 16) {
+                float4 x[4];
+#pragma unroll
+                for (uint32_t u = 0; u < 4; ++u) {
+                    const uint32_t r = r0 + 4 * u, qi = im.q0 + r;
+                    x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (r < im.nq)
+                        x[u] = __ldg(reinterpret_cast<const float4 *>(
+                                         p.q + ((size_t)(im.row0 + qi / p.per) * p.n_q + im.kvh * p.per + qi % p.per) * kHd) + lane);
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < 4; ++u) {
+                    const uint32_t r = r0 + 4 * u;
+                    float top = fmaxf(fmaxf(fabsf(x[u].x), fabsf(x[u].y)), fmaxf(fabsf(x[u].z), fabsf(x[u].w)));
+#pragma unroll
+                    for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 126);
+                    const float down = __int_as_float((127 - e) << 23);
+                    const float y[4] = {x[u].x * down, x[u].y * down, x[u].z * down, x[u].w * down};
+                    uint32_t hi[2], lo[2];
+                    split_half2(y[0], y[1], hi[0], lo[0]);
+                    split_half2(y[2], y[3], hi[1], lo[1]);
+                    if (r < rows) {
+                        uint8_t *at = qs + (lane >> 4) * kQBox + r * 128 + ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
+                        *reinterpret_cast<uint2 *>(at) = make_uint2(hi[0], hi[1]);
+                        *reinterpret_cast<uint2 *>(at + 2 * kQBox) = make_uint2(lo[0], lo[1]);
+                        if (lane == 0) sm.c[it & 1][r] = p.scale_log2 * __int_as_float((127 + e) << 23);
+                    }
+                }
+            }
+            fence_proxy_async();
+            group_sync();
+            if (lane == 0) mbar_arrive(&sm.q_full);
+        };
+        Item im = item_at(0, ok, true);
+        // (a warp whose wait ran out stays with the others: they leave together, and the group's barriers count on all four)
+        ok = !group_or(!ok);
+        if (ok && im.tiles) queries(im, 0);
+        for (uint32_t it = 0; ok && im.tiles; ++it) {
+            const uint32_t nb = (im.nq + 15) >> 4;               // blocks of 16 queries
+            const float4 *const c4 = reinterpret_cast<const float4 *>(sm.c[it & 1]), *const m4 = reinterpret_cast<const float4 *>(sm.m);
+            const float4 *const a4 = reinterpret_cast<const float4 *>(sm.a);
+            float o[kMaxQ], l[kMaxQ];
+#pragma unroll
+            for (uint32_t j = 0; j < kMaxQ; ++j) o[j] = l[j] = 0.f;
+            auto add_values = [&](uint32_t tile, bool scaled) {  // O^T of a finished tile; then the change of reference
+                const uint32_t at = tmem + kTmemO + (tile & 1) * kMaxQ + lanes;
+#pragma unroll
+                for (uint32_t b = 0; b < 4; ++b)
+                    if (b < nb) {
+                        float v[16];
+                        tc5::ld16(at + 16 * b, v);
+                        tc5::wait_ld();
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; ++j) o[16 * b + j] += v[j];
+                    }
+                if (scaled) {
+#pragma unroll
+                    for (uint32_t j = 0; j < kMaxQ; j += 4)
+                        if (j < 16 * nb) {
+                            const float4 a = a4[j / 4];
+                            o[j] *= a.x; o[j + 1] *= a.y; o[j + 2] *= a.z; o[j + 3] *= a.w;
+                        }
+                }
+            };
+            for (uint32_t t = 0; t < im.tiles; ++t, ++n) {
+                if (ok) ok = mbar_wait_warp(&sm.s_full[n & 1], (n >> 1) & 1, limit);
+                tc5::fence_after();
+                const uint32_t at = tmem + (n & 1) * kMaxQ + lanes, here = im.rows - (im.tile0 + t) * kTile;
+                const bool seen = key < here;
+                float s[kMaxQ];
+                auto scores = [&]() {
+#pragma unroll
+                    for (uint32_t b = 0; b < 4; ++b)
+                        if (b < nb) tc5::ld16(at + 16 * b, s + 16 * b);
+                    tc5::wait_ld();
+                };
+                scores();
+                bool moved = t == 0;
+                if (!moved) {
+                    bool above = false;
+#pragma unroll
+                    for (uint32_t j = 0; j < kMaxQ; j += 4)
+                        if (j < 16 * nb) {
+                            const float4 c = c4[j / 4], m = m4[j / 4];
+                            s[j] = fmaf(s[j], c.x, -m.x);
+                            s[j + 1] = fmaf(s[j + 1], c.y, -m.y);
+                            s[j + 2] = fmaf(s[j + 2], c.z, -m.z);
+                            s[j + 3] = fmaf(s[j + 3], c.w, -m.w);
+                            above |= fmaxf(fmaxf(s[j], s[j + 1]), fmaxf(s[j + 2], s[j + 3])) > kGrow;
+                        }
+                    moved = group_or(above && seen);
+                    if (moved) scores();
+                }
+                if (moved) {                                     // (the same in all threads)
+#pragma unroll
+                    for (uint32_t j = 0; j < kMaxQ; j += 4)
+                        if (j < 16 * nb) {
+                            const float4 c = c4[j / 4];
+                            s[j] = seen ? s[j] * c.x : WR_NEG_SENTINEL;
+                            s[j + 1] = seen ? s[j + 1] * c.y : WR_NEG_SENTINEL;
+                            s[j + 2] = seen ? s[j + 2] * c.z : WR_NEG_SENTINEL;
+                            s[j + 3] = seen ? s[j + 3] * c.w : WR_NEG_SENTINEL;
+                        }
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h)
+                        if (2 * h < nb) {
+                            float v[32];
+#pragma unroll
+                            for (uint32_t j = 0; j < 32; ++j) v[j] = j < 16 || 2 * h + 1 < nb ? s[32 * h + j] : WR_NEG_SENTINEL;
+                            const uint32_t idx = warp_max_32(v, lane);
+                            sm.red[32 * h + idx][quarter] = v[0];
+                        }
+                    group_sync();
+                    if (tid < kMaxQ) {
+                        const float4 w = *reinterpret_cast<const float4 *>(sm.red[tid]);
+                        const float top = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), WR_NEG_SENTINEL), old = sm.m[tid];
+                        const bool up = t == 0 || top > old + kGrow;
+                        sm.a[tid] = t == 0 ? 0.f : up ? ex2(old - top) : 1.f;
+                        if (up) sm.m[tid] = top;
+                    }
+                    group_sync();
+#pragma unroll
+                    for (uint32_t j = 0; j < kMaxQ; j += 4)
+                        if (j < 16 * nb) {
+                            const float4 m = m4[j / 4], a = a4[j / 4];
+                            s[j] -= m.x; s[j + 1] -= m.y; s[j + 2] -= m.z; s[j + 3] -= m.w;
+                            l[j] *= a.x; l[j + 1] *= a.y; l[j + 2] *= a.z; l[j + 3] *= a.w;
+                        }
+                }
+                // the tile before has been multiplied: P is free, its O^T is there
+                if (ok && n > 0) ok = mbar_wait_warp(&sm.o_full, (n - 1) & 1, limit);
+                tc5::fence_after();
+#pragma unroll
+                for (uint32_t j = 0; j < kMaxQ; j += 8)
+                    if (j < 16 * nb) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) {
+                            const float w0 = seen ? ex2(s[j + 2 * e]) : 0.f, w1 = seen ? ex2(s[j + 2 * e + 1]) : 0.f;
+                            l[j + 2 * e] += w0;
+                            l[j + 2 * e + 1] += w1;
+                            split_half2(w0, w1, hi[e], lo[e]);
+                        }
+                        uint8_t *to = ps + key * 128 + (((j >> 3) ^ (key & 7)) << 4);
+                        *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4 *>(to + kTile * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                if (here < kTile) {
+                    // rows behind the last one may hold anything, and a weight of zero does not take a NaN out
+                    const uint32_t st = n % kVSlots;
+                    if (ok) ok = mbar_wait_warp(&sm.v_full[st], (n / kVSlots) & 1, limit);
+                    if (!seen) {
+                        uint8_t *row = vs + st * kSlot + (key >> 6) * kPageBlock + (key & 63) * 128;
+#pragma unroll
+                        for (uint32_t e = 0; e < 16; ++e)
+                            *reinterpret_cast<uint4 *>(row + (e >> 3) * 8192 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                }
+                fence_proxy_async();
+                tc5::fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.p_full);
+                if (t > 0) add_values(n - 1, moved);
+            }
+            // the next item's queries (the last scores have been read), then this one's results
+            bool more = true;
+            const Item following = item_at(it + 1, more, true);
+            ok = !group_or(!(ok && more));
+            if (ok && following.tiles) queries(following, it + 1);
+            if (ok) ok = mbar_wait_warp(&sm.o_full, (n - 1) & 1, limit);
+            tc5::fence_after();
+            add_values(n - 1, false);
+            float *to = p.o + (size_t)im.part * kHd + key;
+#pragma unroll
+            for (uint32_t j = 0; j < kMaxQ; ++j)
+                if (j < im.nq) to[(size_t)j * kHd] = o[j];
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h)
+                if (2 * h < nb) {
+                    float v[32];
+#pragma unroll
+                    for (uint32_t j = 0; j < 32; ++j) v[j] = l[32 * h + j];
+                    const int idx = warp_reduce_many<32>(v, (int)lane);
+                    sm.red[32 * h + idx][quarter] = v[0];
+                }
+            group_sync();
+            if (tid < im.nq) {
+                const float4 w = *reinterpret_cast<const float4 *>(sm.red[tid]);
+                p.ml[im.part + tid] = make_float2(sm.m[tid], (w.x + w.y) + (w.z + w.w));
+            }
+            ok = !group_or(!ok);
+            im = following;
+        }
+        if (!ok && lane == 0) atomicCAS(p.err, 0, 84);
+    }
+    tc5::fence_before();
+    __syncthreads();
+    tc5::fence_after();
+    if (warp == 1) tc5::dealloc(tmem, kTmemCols);
+}
+
+// The chunks of a row added up: those of its group's shared rows, then those of its own.
+__global__ void __launch_bounds__(kHd) shared_merge_kernel(const __grid_constant__ SharedParams p)
+{
+    __shared__ float w[kMaxParts];
+    __shared__ float sum;
+    pdl_wait();
+    pdl_trigger();
+    const uint32_t head = blockIdx.x, s = blockIdx.y, kvh = head / p.per, lane = threadIdx.x & 31;
+    uint32_t first[2], step[2], count[2];
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+        const uint32_t at = i ? p.own_seg[s] : p.group_seg[s];
+        count[i] = 0;
+        if (at >= kMaxSegs) continue;
+        const Segment &g = p.seg[at];
+        count[i] = g.chunks;
+        step[i] = p.n_kv * g.queries;
+        first[i] = g.part0 + kvh * g.queries + (s - g.row0) * p.per + head % p.per;
+    }
+    const uint32_t n = count[0] + count[1];
+    auto part = [&](uint32_t i) { return i < count[0] ? first[0] + i * step[0] : first[1] + (i - count[0]) * step[1]; };
+    if (threadIdx.x < 32) {
+        float top = WR_NEG_SENTINEL;
+        for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, p.ml[part(i)].x);
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float l = 0.f;
+        for (uint32_t i = lane; i < n; i += 32) {
+            const float2 ml = p.ml[part(i)];
+            const float f = ex2(ml.x - top);
+            w[i] = f;
+            l += f * ml.y;
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (lane == 0) sum = l;
+    }
+    __syncthreads();
+    float acc = 0.f;
+#pragma unroll 8
+    for (uint32_t i = 0; i < n; ++i) acc = fmaf(w[i], p.o[(size_t)part(i) * kHd + threadIdx.x], acc);
+    // (a row of which no key counts, all scores -inf, is zeros)
+    p.out[((size_t)s * p.n_q + head) * kHd + threadIdx.x] = sum == 0.f ? 0.f : acc / sum;
+}
+
+}  // namespace
+
+// Groups: their sizes add up to the sessions, their rows are whole pages that all their sessions have, no more than the
+// shortest of them attends.  Caller holds ctx->lock.
+int wr_shared_validate(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *seq_lens,
+                       uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, const void *q, const void *out,
+                       uint32_t n_q, int mem)
+{
+    int rc = wr_decode_validate(ctx, n_sess, kv, layer, seq_lens, q, out, n_q, mem, 0);
+    if (rc != WR_CUDA_OK) return rc;
+    if (kv[0]->hd_at(layer) != kHd) return WR_CUDA_ERR_UNSUPPORTED;
+    if (!group_sess || !group_rows || n_groups == 0 || n_groups > n_sess) return WR_CUDA_ERR_INVAL;
+    uint32_t s = 0;
+    for (uint32_t g = 0; g < n_groups; ++g) {
+        if (group_sess[g] == 0 || group_sess[g] > n_sess - s || group_rows[g] % kPageTokens) return WR_CUDA_ERR_INVAL;
+        for (uint32_t i = 0; i < group_sess[g]; ++i) {
+            if (group_rows[g] > seq_lens[s + i]) return WR_CUDA_ERR_INVAL;
+            if (i && wr_kv_common_pages(kv[s], kv[s + i]) < group_rows[g] / kPageTokens) return WR_CUDA_ERR_INVAL;
+        }
+        s += group_sess[g];
+    }
+    return s == n_sess ? WR_CUDA_OK : WR_CUDA_ERR_INVAL;
+}
+
+// Enqueue both kernels on device-resident q / out.  Caller holds ctx->lock and has validated the arguments.
+int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *seq_lens,
+                     uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, const float *dq, float *dout,
+                     uint32_t n_q, float scale_override)
+{
+    SharedParams p{};
+    p.n_q = n_q;
+    p.n_kv = kv[0]->n_kv_at(layer);
+    p.per = n_q / p.n_kv;
+    uint64_t tiles = 0;
+    auto add = [&](const wr_cuda_kv *of, uint32_t first_page, uint32_t rows, uint32_t row0, uint32_t sessions) {
+        Segment &g = p.seg[p.n_segs++];
+        g.pages = of->d_pages + (size_t)layer * of->n_pages + first_page;
+        g.rows = rows;
+        g.row0 = row0;
+        g.queries = sessions * p.per;
+        g.qtiles = (g.queries + kMaxQ - 1) / kMaxQ;
+        tiles += (uint64_t)((rows + kTile - 1) / kTile) * p.n_kv * g.qtiles;
+    };
+    for (uint32_t g = 0, s = 0; g < n_groups; s += group_sess[g++]) {
+        if (group_rows[g]) add(kv[s], 0, group_rows[g], s, group_sess[g]);
+        for (uint32_t i = s; i < s + group_sess[g]; ++i)
+            if (seq_lens[i] > group_rows[g]) add(kv[i], group_rows[g] / kPageTokens, seq_lens[i] - group_rows[g], i, 1);
+    }
+    // Chunks as long as the SMs' even share of all tiles: then there is about one item per SM, and what is left over is
+    // short and comes last.
+    const uint32_t per = (uint32_t)((tiles + ctx->sm_count - 1) / ctx->sm_count);
+    for (uint32_t i = 0; i < p.n_segs; ++i) p.seg[i].chunks = ((p.seg[i].rows + kTile - 1) / kTile + per - 1) / per;
+    std::stable_sort(p.seg, p.seg + p.n_segs, [](const Segment &a, const Segment &b) {
+        return (uint64_t)a.rows * b.chunks > (uint64_t)b.rows * a.chunks;
+    });
+    std::fill(p.group_seg, p.group_seg + WR_CUDA_BATCH_MAX, (uint8_t)kMaxSegs);
+    std::fill(p.own_seg, p.own_seg + WR_CUDA_BATCH_MAX, (uint8_t)kMaxSegs);
+    uint64_t parts = 0;
+    for (uint32_t i = 0; i < p.n_segs; ++i) {
+        Segment &g = p.seg[i];
+        g.item0 = p.items;
+        g.part0 = (uint32_t)parts;
+        p.items += g.chunks * g.qtiles * p.n_kv;
+        parts += (uint64_t)g.chunks * p.n_kv * g.queries;
+    }
+    if (parts > 0x7fffffffu) return WR_CUDA_ERR_LIMIT;
+    for (uint32_t g = 0, s = 0; g < n_groups; s += group_sess[g++])
+        for (uint32_t i = 0; i < p.n_segs; ++i) {
+            const Segment &x = p.seg[i];
+            const bool of_group = group_rows[g] && x.row0 == s && x.queries == group_sess[g] * p.per && x.rows == group_rows[g] &&
+                                  x.pages == kv[s]->d_pages + (size_t)layer * kv[s]->n_pages;
+            for (uint32_t r = s; r < s + group_sess[g]; ++r) {
+                if (of_group) p.group_seg[r] = (uint8_t)i;
+                else if (x.row0 == r && x.queries == p.per) p.own_seg[r] = (uint8_t)i;
+            }
+        }
+    const size_t head = 256, ml = ((size_t)parts * sizeof(float2) + 255) & ~(size_t)255;
+    char *ws = nullptr;
+    int rc = wr_ctx_keep(ctx, head + ml + (size_t)parts * kHd * sizeof(float), &ws);
+    if (rc != WR_CUDA_OK) return rc;
+    p.sched = reinterpret_cast<int *>(ws);
+    p.ml = reinterpret_cast<float2 *>(ws + head);
+    p.o = reinterpret_cast<float *>(ws + head + ml);
+    p.q = dq;
+    p.out = dout;
+    p.scale_log2 = (scale_override > 0.0f ? scale_override : 1.0f / sqrtf((float)kHd)) * kLog2e;
+    p.wait_limit = ctx->wait_limit;
+    p.err = ctx->dev_err;
+    if (!(ctx->attr_flags & 0x100u)) {
+        WR_CUDA_TRY(cudaFuncSetAttribute(attn_shared_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
+        ctx->attr_flags |= 0x100u;
+    }
+    WR_CUDA_TRY(wr_launch_pdl(attn_shared_kernel, dim3(std::min<uint32_t>(p.items, (uint32_t)ctx->sm_count)), dim3(kThreads),
+                              (size_t)kSmem, ctx->stream, p));
+    WR_CUDA_TRY(wr_launch_pdl(shared_merge_kernel, dim3(n_q, n_sess), dim3(kHd), (size_t)0, ctx->stream, p));
+    ctx->launches += 2;
+    WR_CUDA_TRY(cudaGetLastError());
+    return WR_CUDA_OK;
+}
+
+// decode_step's body (append, then attention) and attention alone share the handling of host buffers.
+static int shared_call(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *positions,
+                       const uint32_t *seq_lens, uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, float *q,
+                       const float *k_rows, const float *v_rows, float *out, uint32_t n_q, float theta_base, uint32_t n_rot_pairs,
+                       uint32_t flags, float scale_override, int mem)
+{
+    const bool append = positions != nullptr;
+    const uint32_t n_kv = kv[0]->n_kv_at(layer);
+    const size_t kv_bytes = append ? (size_t)n_sess * n_kv * kHd * sizeof(float) : 0, q_bytes = (size_t)n_sess * n_q * kHd * sizeof(float);
+    const float *dk = k_rows, *dv = v_rows;
+    float *dq = q, *dout = out;
+    int rc;
+    if (mem == WR_CUDA_MEM_HOST) {
+        rc = wr_ctx_reserve_stage(ctx, 2 * kv_bytes + 2 * q_bytes, 0);
+        if (rc != WR_CUDA_OK) return rc;
+        char *d = (char *)ctx->stage_dev;
+        dk = (const float *)d;
+        dv = (const float *)(d + kv_bytes);
+        dq = (float *)(d + 2 * kv_bytes);
+        dout = (float *)(d + 2 * kv_bytes + q_bytes);
+        if (append) {
+            WR_CUDA_TRY(cudaMemcpyAsync((void *)dk, k_rows, kv_bytes, cudaMemcpyHostToDevice, ctx->stream));
+            WR_CUDA_TRY(cudaMemcpyAsync((void *)dv, v_rows, kv_bytes, cudaMemcpyHostToDevice, ctx->stream));
+        }
+        WR_CUDA_TRY(cudaMemcpyAsync(dq, q, q_bytes, cudaMemcpyHostToDevice, ctx->stream));
+    }
+    if (append) {
+        rc = wr_append_launch(ctx, n_sess, kv, layer, positions, 1, dk, dv, dq, n_q, theta_base, n_rot_pairs, flags, nullptr);
+        if (rc != WR_CUDA_OK) return rc;
+    }
+    rc = wr_shared_launch(ctx, n_sess, kv, layer, seq_lens, n_groups, group_sess, group_rows, dq, dout, n_q, scale_override);
+    if (rc != WR_CUDA_OK) return rc;
+    if (mem == WR_CUDA_MEM_HOST) {
+        WR_CUDA_TRY(cudaMemcpyAsync(out, dout, q_bytes, cudaMemcpyDeviceToHost, ctx->stream));
+        return wr_ctx_sync_checked(ctx);
+    }
+    return WR_CUDA_OK;
+}
+
+extern "C" int wr_cuda_attn_decode_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer,
+                                          const uint32_t *seq_lens, uint32_t n_groups, const uint32_t *group_sess,
+                                          const uint32_t *group_rows, const float *q, float *out, uint32_t n_q_heads,
+                                          float scale_override, int mem)
+{
+    if (!ctx) return WR_CUDA_ERR_INVAL;
+    std::lock_guard<std::mutex> g(ctx->lock);
+    int rc = wr_shared_validate(ctx, n_sess, kv, layer, seq_lens, n_groups, group_sess, group_rows, q, out, n_q_heads, mem);
+    if (rc != WR_CUDA_OK) return rc;
+    WR_CUDA_TRY(cudaSetDevice(ctx->device));
+    return shared_call(ctx, n_sess, kv, layer, nullptr, seq_lens, n_groups, group_sess, group_rows, const_cast<float *>(q), nullptr,
+                       nullptr, out, n_q_heads, 0.f, 0, 0, scale_override, mem);
+}
+
+int wr_decode_step_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *positions,
+                          uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, float *q, const float *k_rows,
+                          const float *v_rows, float *out, uint32_t n_q_heads, float theta_base, uint32_t n_rot_pairs, uint32_t flags,
+                          float scale_override, int mem)
+{
+    int rc = wr_append_validate(ctx, n_sess, kv, layer, positions, 1, k_rows, v_rows, q, n_q_heads, mem);
+    if (rc != WR_CUDA_OK) return rc;
+    uint32_t seq_lens[WR_CUDA_BATCH_MAX];
+    for (uint32_t s = 0; s < n_sess; ++s) seq_lens[s] = positions[s] + 1;
+    rc = wr_shared_validate(ctx, n_sess, kv, layer, seq_lens, n_groups, group_sess, group_rows, q, out, n_q_heads, mem);
+    if (rc != WR_CUDA_OK) return rc;
+    // (a group's rows end before the row that is appended: what it shares is read only)
+    for (uint32_t g = 0, s = 0; g < n_groups; s += group_sess[g++])
+        for (uint32_t i = s; i < s + group_sess[g]; ++i)
+            if (group_rows[g] > positions[i]) return WR_CUDA_ERR_INVAL;
+    WR_CUDA_TRY(cudaSetDevice(ctx->device));
+    return shared_call(ctx, n_sess, kv, layer, positions, seq_lens, n_groups, group_sess, group_rows, q, k_rows, v_rows, out, n_q_heads,
+                       theta_base, n_rot_pairs, flags, scale_override, mem);
+}
+
+extern "C" int wr_cuda_decode_step_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer,
+                                          const uint32_t *positions, uint32_t n_groups, const uint32_t *group_sess,
+                                          const uint32_t *group_rows, float *q, const float *k_rows, const float *v_rows, float *out,
+                                          uint32_t n_q_heads, float theta_base, uint32_t n_rot_pairs, uint32_t flags,
+                                          float scale_override, int mem)
+{
+    if (!ctx) return WR_CUDA_ERR_INVAL;
+    std::lock_guard<std::mutex> g(ctx->lock);
+    return wr_decode_step_shared(ctx, n_sess, kv, layer, positions, n_groups, group_sess, group_rows, q, k_rows, v_rows, out, n_q_heads,
+                                 theta_base, n_rot_pairs, flags, scale_override, mem);
+}

@@ -10,6 +10,7 @@
 #include <new>
 
 #include "mathx_dev.cuh"
+#include "kv_share.cuh"
 #include "wr_internal.cuh"
 
 // ------------------------------------------------------------------ device
@@ -85,6 +86,8 @@ extern "C" void wr_cuda_ctx_destroy(wr_cuda_ctx *ctx)
     if (ctx->prefill_sched) (void)cudaFree(ctx->prefill_sched);
     if (ctx->prefill_parts) (void)cudaFree(ctx->prefill_parts);
     if (ctx->debug_buf) (void)cudaFree(ctx->debug_buf);
+    if (ctx->kept) (void)cudaFree(ctx->kept);
+    for (void *p : ctx->outgrown) (void)cudaFree(p);
     if (ctx->host_err) (void)cudaFreeHost(ctx->host_err);       // (dev_err is its device-side alias)
     if (ctx->stage_dev) (void)cudaFree(ctx->stage_dev);
     if (ctx->stage_host) (void)cudaFreeHost(ctx->stage_host);
@@ -255,10 +258,31 @@ int wr_ctx_try_ws(wr_cuda_ctx *ctx, size_t ws_bytes)
     return WR_CUDA_OK;
 }
 
+int wr_ctx_keep(wr_cuda_ctx *ctx, size_t bytes, char **out)
+{
+    if (bytes > ctx->kept_bytes) {
+        // (twice as much as before at least: all that is outgrown together is no more than what is in use)
+        const size_t want = std::max({bytes, 2 * ctx->kept_bytes, (size_t)8 << 20});
+        void *p = nullptr;
+        WR_CUDA_TRY(cudaMalloc(&p, want));
+        const cudaError_t e = cudaMemsetAsync(p, 0, want, ctx->stream);
+        if (e != cudaSuccess) {
+            (void)cudaGetLastError();
+            (void)cudaFree(p);
+            return WR_CUDA_ERR_INTERNAL;
+        }
+        if (ctx->kept) ctx->outgrown.push_back(ctx->kept);
+        ctx->kept = (char *)p;
+        ctx->kept_bytes = want;
+    }
+    *out = ctx->kept;
+    return WR_CUDA_OK;
+}
+
 // -------------------------------------------------------------- page pool
 
-static int pool_take(wr_cuda_ctx *ctx, uint64_t page_bytes, size_t n, size_t *pool_index,
-                     std::vector<void *> &out)
+int wr_pool_take(wr_cuda_ctx *ctx, uint64_t page_bytes, size_t n, size_t *pool_index,
+                 std::vector<void *> &out)
 {
     size_t pi = 0;
     for (; pi < ctx->pools.size(); ++pi)
@@ -293,21 +317,28 @@ static int pool_take(wr_cuda_ctx *ctx, uint64_t page_bytes, size_t n, size_t *po
 
 // Everything a session holds goes back to the pools it came from, cleared so that the next owner
 // starts from zeros.  Caller holds ctx->lock.
-static void kv_give_back(wr_cuda_kv *kv)
+void wr_kv_give_back(wr_cuda_kv *kv)
 {
     wr_cuda_ctx *ctx = kv->ctx;
+    // pages that other sessions go on holding stay; those it holds last go with its own
+    uint32_t held = 0;
+    for (; held < kv->columns.size(); ++held)
+        if (kv->columns[held]->holders.fetch_sub(1) == 1) break;
+    for (uint32_t i = held + 1; i < kv->columns.size(); ++i) kv->columns[i]->holders.fetch_sub(1);
+    for (uint32_t i = held; i < kv->columns.size(); ++i) delete kv->columns[i];
     for (uint32_t L = 0; L < kv->n_layers && !kv->pages.empty(); ++L) {
         const wr_kv_layer &lay = kv->layers[L];
         void **first = kv->pages.data() + (size_t)L * kv->n_pages;
-        if (!lay.geom.n_kv || !first[0]) continue;
-        if (kv->contig[L]) {
-            (void)cudaMemsetAsync(first[0], 0, lay.page_bytes * kv->n_pages, ctx->stream);
-        } else {
-            for (uint32_t i = 0; i < kv->n_pages; ++i)
+        if (!lay.geom.n_kv || !first[0] || held == kv->n_pages) continue;
+        // (pages back to back may still be of two allocations that happen to be neighbours, which one memset does not span)
+        if (!kv->contig[L] ||
+            cudaMemsetAsync(first[held], 0, lay.page_bytes * (kv->n_pages - held), ctx->stream) != cudaSuccess) {
+            (void)cudaGetLastError();
+            for (uint32_t i = held; i < kv->n_pages; ++i)
                 (void)cudaMemsetAsync(first[i], 0, lay.page_bytes, ctx->stream);
         }
         auto &fp = ctx->pools[lay.pool_index].free_pages;
-        for (uint32_t i = kv->n_pages; i-- > 0;) fp.push_back(first[i]);
+        for (uint32_t i = kv->n_pages; i-- > held;) fp.push_back(first[i]);
     }
     if (kv->state[0]) {
         auto &fp = ctx->pools[kv->state_pool].free_pages;
@@ -367,7 +398,7 @@ extern "C" int wr_cuda_kv_create_layout(wr_cuda_ctx *ctx, uint32_t n_layers, con
             if (kv->layers[M].geom.n_kv && kv->layers[M].page_bytes == kv->layers[L].page_bytes) same.push_back(M);
         std::vector<void *> got;
         size_t pool = 0;
-        rc = pool_take(ctx, kv->layers[L].page_bytes, same.size() * kv->n_pages, &pool, got);
+        rc = wr_pool_take(ctx, kv->layers[L].page_bytes, same.size() * kv->n_pages, &pool, got);
         if (rc != WR_CUDA_OK) break;
         for (size_t j = 0; j < same.size(); ++j) {
             const uint32_t M = same[j];
@@ -382,7 +413,7 @@ extern "C" int wr_cuda_kv_create_layout(wr_cuda_ctx *ctx, uint32_t n_layers, con
     }
     if (rc == WR_CUDA_OK && kv->state_bytes) {
         std::vector<void *> got;
-        rc = pool_take(ctx, kv->state_bytes, 2, &kv->state_pool, got);
+        rc = wr_pool_take(ctx, kv->state_bytes, 2, &kv->state_pool, got);
         if (rc == WR_CUDA_OK) {
             kv->state[0] = got[0];
             kv->state[1] = got[1];
@@ -400,7 +431,7 @@ extern "C" int wr_cuda_kv_create_layout(wr_cuda_ctx *ctx, uint32_t n_layers, con
         }
     }
     if (rc != WR_CUDA_OK) {
-        kv_give_back(kv);
+        wr_kv_give_back(kv);
         delete kv;
         return rc;
     }
@@ -430,7 +461,7 @@ extern "C" void wr_cuda_kv_destroy(wr_cuda_kv *kv)
     std::lock_guard<std::mutex> g(ctx->lock);
     (void)cudaSetDevice(ctx->device);
     (void)cudaStreamSynchronize(ctx->stream);
-    kv_give_back(kv);
+    wr_kv_give_back(kv);
     ctx->live_kv--;
     delete kv;
 }
@@ -497,6 +528,7 @@ static int kv_rows_xfer(wr_cuda_ctx *ctx, wr_cuda_kv *kv, uint32_t layer, int wh
     if (hd == 0) return WR_CUDA_ERR_UNSUPPORTED;
     if (n == 0) return WR_CUDA_OK;
     if ((uint64_t)row0 + n > kv->max_ctx) return WR_CUDA_ERR_CTX_FULL;
+    if (to_cache && !wr_kv_writable(kv, row0, n)) return WR_CUDA_ERR_STATE;
     if (mem != WR_CUDA_MEM_HOST && mem != WR_CUDA_MEM_DEVICE) return WR_CUDA_ERR_INVAL;
     // device rows move as 16-byte vectors when head_dim allows it
     if (mem == WR_CUDA_MEM_DEVICE && (hd & 7u) == 0 && ((uintptr_t)buf & 15u)) return WR_CUDA_ERR_INVAL;
@@ -829,6 +861,8 @@ int wr_append_validate(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv,
     if (mem != WR_CUDA_MEM_HOST && mem != WR_CUDA_MEM_DEVICE) return WR_CUDA_ERR_INVAL;
     for (uint32_t s = 0; s < n_sess; ++s)
         if ((uint64_t)positions[s] + n_tokens > kv[s]->max_ctx) return WR_CUDA_ERR_CTX_FULL;
+    for (uint32_t s = 0; s < n_sess; ++s)
+        if (!wr_kv_writable(kv[s], positions[s], n_tokens)) return WR_CUDA_ERR_STATE;
     return WR_CUDA_OK;
 }
 

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "gemm_f32.cuh"
+#include "kv_share.cuh"
 #include "wr_internal.cuh"
 
 struct wr_cuda_layer_dev {
@@ -34,6 +35,7 @@ struct wr_cuda_model {
     wr_split_scale *row_scale = nullptr;
     float *parts = nullptr;
     uint32_t *h_tokens = nullptr;        // pinned: token ids in, arg-max ids out
+    float *beam_host = nullptr, *beam_dev = nullptr;     // a beam step's scores in, its choice out (pinned, device); from the first one on
     uint32_t ffn_max = 0;
     uint64_t launches = 0;
     uint64_t last_enqueue_ns = 0;        // host time the last forward pass spent before it began to wait
@@ -48,9 +50,21 @@ constexpr int WR_ARGMAX_PARTS = 64;
 int wr_argmax_launch(cudaStream_t st, const float *logits, uint32_t ld, uint32_t vocab, uint32_t rows, float *part_v,
                      uint32_t *part_i, uint32_t *best);
 
+// What a beam search's step asks of a pass over groups * beams rows (host memory), and the choice from logits on the device: the
+// caller's row r is row row_at[r] of them.  finish: after the stream has been waited for.
+struct wr_beam_step {
+    uint32_t groups, beams, n_out;
+    const float *scores;
+    float *out_scores;
+    uint32_t *out_beams, *out_tokens;
+};
+int  wr_beam_step_launch(wr_cuda_ctx *ctx, wr_cuda_model *m, const wr_beam_step &b, const float *logits, size_t ld, uint32_t vocab,
+                         const uint32_t *row_at);
+void wr_beam_step_finish(wr_cuda_model *m, const wr_beam_step &b);
+
 int  wr_mixed_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_rows, wr_cuda_kv *const *kv,
                       const uint32_t *positions, const uint32_t *tokens, uint32_t out_from, float *hidden_out,
-                      float *normed_out, float *const *logits_out, uint32_t *argmax_out);
+                      float *normed_out, float *const *logits_out, uint32_t *argmax_out, const wr_beam_step *beam);
 void wr_mixed_destroy(wr_mixed *x);      // caller holds ctx->lock, device current, stream idle
 
 // A forward pass that returns early leaves none of its work in flight, on either stream: what it was given to fill may be

@@ -461,6 +461,8 @@ extern "C" void wr_cuda_model_destroy(wr_cuda_model *m)
         cudaFree(m->prompt);
         drop_side(m);
         cudaFreeHost(m->h_tokens);
+        if (m->beam_host) cudaFreeHost(m->beam_host);
+        if (m->beam_dev) cudaFree(m->beam_dev);
     }
     delete m;
 }
@@ -469,24 +471,22 @@ extern "C" uint64_t wr_cuda_model_bytes(const wr_cuda_model *m) { return m ? m->
 extern "C" uint64_t wr_cuda_model_launches(const wr_cuda_model *m) { return m ? m->launches : 0; }
 extern "C" uint64_t wr_cuda_model_last_enqueue_ns(const wr_cuda_model *m) { return m ? m->last_enqueue_ns : 0; }
 
-extern "C" int wr_cuda_model_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_rows,
-                                     wr_cuda_kv *const *kv, const uint32_t *positions,
-                                     const uint32_t *tokens, uint32_t out_from, float *hidden_out,
-                                     float *normed_out, float *const *logits_out, uint32_t *argmax_out,
-                                     float *attn_tap_out)
+// A forward pass; `beam`, when given, gets its choice from the logits of all rows (wr_cuda_model_beam_step).
+static int forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_rows, wr_cuda_kv *const *kv, const uint32_t *positions,
+                   const uint32_t *tokens, uint32_t out_from, float *hidden_out, float *normed_out, float *const *logits_out,
+                   uint32_t *argmax_out, float *attn_tap_out, const wr_beam_step *beam)
 {
-    if (!ctx || !m || m->ctx != ctx || !kv || !positions || !tokens) return WR_CUDA_ERR_INVAL;
-    if (mode != WR_CUDA_FWD_DECODE && mode != WR_CUDA_FWD_PREFILL) return WR_CUDA_ERR_INVAL;
     if (m->mixed) {
         if (attn_tap_out) return WR_CUDA_ERR_UNSUPPORTED;
         return wr_mixed_forward(ctx, m, mode, n_rows, kv, positions, tokens, out_from, hidden_out, normed_out,
-                                logits_out, argmax_out);
+                                logits_out, argmax_out, beam);
     }
     if (n_rows == 0 || n_rows > m->max_rows || out_from > n_rows) return WR_CUDA_ERR_LIMIT;
     if (mode == WR_CUDA_FWD_DECODE && n_rows > WR_CUDA_BATCH_MAX) return WR_CUDA_ERR_LIMIT;
     const uint32_t n_out = n_rows - out_from;
-    if ((logits_out || argmax_out) && n_out > kLogitRowsMax) return WR_CUDA_ERR_LIMIT;
-    if ((normed_out || logits_out || argmax_out) && n_out == 0) return WR_CUDA_ERR_INVAL;
+    const bool heads = logits_out || argmax_out || beam;
+    if (heads && n_out > kLogitRowsMax) return WR_CUDA_ERR_LIMIT;
+    if ((normed_out || heads) && n_out == 0) return WR_CUDA_ERR_INVAL;
     for (uint32_t r = 0; r < n_rows; ++r)
         if (tokens[r] >= m->vocab) return WR_CUDA_ERR_INVAL;      // refused before anything runs
     const uint32_t n_sess = (mode == WR_CUDA_FWD_DECODE) ? n_rows : 1;
@@ -494,6 +494,7 @@ extern "C" int wr_cuda_model_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mod
         if (!kv[s] || kv[s]->n_layers != m->n_layers) return WR_CUDA_ERR_INVAL;
         for (uint32_t L = 0; L < m->n_layers; ++L)
             if (kv[s]->n_kv_at(L) != m->n_kv || kv[s]->hd_at(L) != m->hd) return WR_CUDA_ERR_INVAL;
+        if (!wr_kv_writable(kv[s], positions[s], mode == WR_CUDA_FWD_DECODE ? 1 : n_rows)) return WR_CUDA_ERR_STATE;
     }
 
     std::lock_guard<std::mutex> fg(m->fwd);
@@ -670,7 +671,7 @@ extern "C" int wr_cuda_model_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mod
     // ones are copied out.
     const uint32_t o_lo = permuted ? 0u : out_from, n_fin = n_rows - o_lo;
     auto caller_row = [&](uint32_t i) { return permuted ? perm[i] : i; };
-    if ((logits_out || argmax_out) && n_fin > kLogitRowsMax) return WR_CUDA_ERR_LIMIT;
+    if (heads && n_fin > kLogitRowsMax) return WR_CUDA_ERR_LIMIT;
     const float *res_out = m->resid + (size_t)o_lo * hid;
     if (hidden_out && n_out) {
         if (!permuted) {
@@ -683,7 +684,7 @@ extern "C" int wr_cuda_model_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mod
                                                 cudaMemcpyDeviceToHost, st));
         }
     }
-    if ((normed_out || logits_out || argmax_out) && n_out) {
+    if ((normed_out || heads) && n_out) {
         // the final norm of at most 16 rows is kept for the LM head; more rows (normed_out only) go in passes
         for (uint32_t done = 0; done < n_fin; done += kLogitRowsMax) {
             const uint32_t nr = (n_fin - done < kLogitRowsMax) ? n_fin - done : kLogitRowsMax;
@@ -705,7 +706,7 @@ extern "C" int wr_cuda_model_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mod
             }
         }
     }
-    if ((logits_out || argmax_out) && n_out) {
+    if (heads && n_out) {
         GemvParams p{};
         p.seg[0] = {m->lm_head, m->logits, m->vocab, m->vocab};
         p.n_seg = 1;
@@ -718,6 +719,12 @@ extern "C" int wr_cuda_model_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mod
             m->launches += 2;
             WR_CUDA_TRY(cudaMemcpyAsync(m->h_tokens + m->max_rows, m->best, n_fin * sizeof(uint32_t),
                                         cudaMemcpyDeviceToHost, st));
+        }
+        if (beam) {
+            uint32_t at[WR_CUDA_BATCH_MAX];
+            for (uint32_t i = 0; i < n_fin; ++i) at[caller_row(o_lo + i)] = i;
+            rc = wr_beam_step_launch(ctx, m, *beam, m->logits, m->vocab, m->vocab, at);
+            if (rc != WR_CUDA_OK) return rc;
         }
         if (logits_out)
             for (uint32_t i = 0; i < n_fin; ++i) {
@@ -737,5 +744,74 @@ extern "C" int wr_cuda_model_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mod
             const uint32_t c = caller_row(o_lo + i);
             if (c >= out_from) argmax_out[c - out_from] = m->h_tokens[m->max_rows + i];
         }
+    if (beam) wr_beam_step_finish(m, *beam);
     return WR_CUDA_OK;
+}
+
+extern "C" int wr_cuda_model_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_rows,
+                                     wr_cuda_kv *const *kv, const uint32_t *positions,
+                                     const uint32_t *tokens, uint32_t out_from, float *hidden_out,
+                                     float *normed_out, float *const *logits_out, uint32_t *argmax_out,
+                                     float *attn_tap_out)
+{
+    if (!ctx || !m || m->ctx != ctx || !kv || !positions || !tokens) return WR_CUDA_ERR_INVAL;
+    if (mode != WR_CUDA_FWD_DECODE && mode != WR_CUDA_FWD_PREFILL) return WR_CUDA_ERR_INVAL;
+    return forward(ctx, m, mode, n_rows, kv, positions, tokens, out_from, hidden_out, normed_out, logits_out, argmax_out, attn_tap_out,
+                   nullptr);
+}
+
+// ---- a beam search's step: the choice from logits that stay where the pass has left them
+
+int wr_beam_step_launch(wr_cuda_ctx *ctx, wr_cuda_model *m, const wr_beam_step &b, const float *logits, size_t ld, uint32_t vocab,
+                        const uint32_t *row_at)
+{
+    const size_t rows = (size_t)b.groups * b.beams, outs = (size_t)b.groups * b.n_out;
+    if (!m->beam_dev) {
+        // (scores in; scores, beams, tokens out: a group has a beam at least and gives 32 continuations at most)
+        constexpr size_t bytes = (WR_CUDA_BATCH_MAX + 3 * WR_CUDA_BATCH_MAX * WR_CUDA_BEAM_MAX_OUT) * 4;
+        WR_CUDA_TRY(cudaHostAlloc((void **)&m->beam_host, bytes, cudaHostAllocDefault));
+        WR_CUDA_TRY(cudaMalloc((void **)&m->beam_dev, bytes));
+    }
+    wr_beam_args a{};
+    a.logits = logits;
+    a.ld = ld;
+    a.groups = b.groups;
+    a.beams = b.beams;
+    a.vocab = vocab;
+    a.n_out = b.n_out;
+    a.scores = m->beam_dev;
+    a.out_scores = m->beam_dev + WR_CUDA_BATCH_MAX;
+    a.out_beams = reinterpret_cast<uint32_t *>(a.out_scores + outs);
+    a.out_tokens = a.out_beams + outs;
+    a.mapped = true;
+    for (uint32_t r = 0; r < rows; ++r) a.map[r] = (uint8_t)row_at[r];
+    memcpy(m->beam_host, b.scores, rows * 4);
+    WR_CUDA_TRY(cudaMemcpyAsync(m->beam_dev, m->beam_host, rows * 4, cudaMemcpyHostToDevice, ctx->stream));
+    const int rc = wr_beam_launch(ctx, a);
+    if (rc != WR_CUDA_OK) return rc;
+    m->launches += 2;
+    WR_CUDA_TRY(cudaMemcpyAsync(m->beam_host + WR_CUDA_BATCH_MAX, a.out_scores, outs * 12, cudaMemcpyDeviceToHost, ctx->stream));
+    return WR_CUDA_OK;
+}
+
+void wr_beam_step_finish(wr_cuda_model *m, const wr_beam_step &b)
+{
+    const size_t outs = (size_t)b.groups * b.n_out;
+    const float *from = m->beam_host + WR_CUDA_BATCH_MAX;
+    memcpy(b.out_scores, from, outs * 4);
+    memcpy(b.out_beams, from + outs, outs * 4);
+    memcpy(b.out_tokens, from + 2 * outs, outs * 4);
+}
+
+extern "C" int wr_cuda_model_beam_step(wr_cuda_ctx *ctx, wr_cuda_model *m, uint32_t n_groups, uint32_t beams, wr_cuda_kv *const *kv,
+                                       const uint32_t *positions, const uint32_t *tokens, const float *scores, uint32_t n_out,
+                                       float *out_scores, uint32_t *out_beams, uint32_t *out_tokens)
+{
+    if (!ctx || !m || m->ctx != ctx || !kv || !positions || !tokens) return WR_CUDA_ERR_INVAL;
+    if (!scores || !out_scores || !out_beams || !out_tokens) return WR_CUDA_ERR_INVAL;
+    const int rc = wr_beam_validate(n_groups, beams, m->vocab, n_out);
+    if (rc != WR_CUDA_OK) return rc;
+    if (n_groups > WR_CUDA_BATCH_MAX || n_groups * beams > WR_CUDA_BATCH_MAX) return WR_CUDA_ERR_LIMIT;
+    const wr_beam_step b = {n_groups, beams, n_out, scores, out_scores, out_beams, out_tokens};
+    return forward(ctx, m, WR_CUDA_FWD_DECODE, n_groups * beams, kv, positions, tokens, 0, nullptr, nullptr, nullptr, nullptr, nullptr, &b);
 }

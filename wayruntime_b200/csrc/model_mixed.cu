@@ -1091,15 +1091,15 @@ struct Step {
 
 int wr_mixed_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_rows, wr_cuda_kv *const *kv,
                      const uint32_t *positions, const uint32_t *tokens, uint32_t out_from, float *hidden_out,
-                     float *normed_out, float *const *logits_out, uint32_t *argmax_out)
+                     float *normed_out, float *const *logits_out, uint32_t *argmax_out, const wr_beam_step *beam)
 {
     wr_mixed *x = m->mixed;
     const bool decode = mode == WR_CUDA_FWD_DECODE;
     if (n_rows == 0 || n_rows > m->max_rows || out_from > n_rows) return WR_CUDA_ERR_LIMIT;
     if (decode && n_rows > WR_CUDA_BATCH_MAX) return WR_CUDA_ERR_LIMIT;
     const uint32_t n_out = n_rows - out_from, n_seq = decode ? n_rows : 1, per_seq = decode ? 1 : n_rows;
-    if (argmax_out && n_out > WR_CUDA_BATCH_MAX) return WR_CUDA_ERR_LIMIT;
-    if ((normed_out || logits_out || argmax_out) && n_out == 0) return WR_CUDA_ERR_INVAL;
+    if ((argmax_out || beam) && n_out > WR_CUDA_BATCH_MAX) return WR_CUDA_ERR_LIMIT;
+    if ((normed_out || logits_out || argmax_out || beam) && n_out == 0) return WR_CUDA_ERR_INVAL;
     for (uint32_t r = 0; r < n_rows; ++r)
         if (tokens[r] >= m->vocab) return WR_CUDA_ERR_INVAL;      // refused before anything runs
 
@@ -1122,6 +1122,7 @@ int wr_mixed_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_ro
         }
         if ((uint64_t)positions[s] + per_seq > kv[s]->max_ctx) return WR_CUDA_ERR_CTX_FULL;
         if ((uint64_t)positions[s] + per_seq > ctx->attn_max_seq) return WR_CUDA_ERR_LIMIT;
+        if (!wr_kv_writable(kv[s], positions[s], per_seq)) return WR_CUDA_ERR_STATE;
         max_len = std::max(max_len, positions[s] + per_seq);
     }
     for (uint32_t s = 0; s < n_seq; ++s) {
@@ -1175,7 +1176,7 @@ int wr_mixed_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_ro
     // The rows somebody asked for, in passes of kHeadRows: final norm, head, copies out.
     uint32_t n_want = 0;
     for (uint32_t i = 0; i < n_out; ++i)
-        if (normed_out || argmax_out || (logits_out && logits_out[i])) x->h_gather[n_want++] = out_from + i;
+        if (normed_out || argmax_out || beam || (logits_out && logits_out[i])) x->h_gather[n_want++] = out_from + i;
     if (n_want) {
         const uint32_t ldv = wr_ld(m->vocab);
         WR_CUDA_TRY(cudaMemcpyAsync(x->gather, x->h_gather, n_want * sizeof(uint32_t), cudaMemcpyHostToDevice, st));
@@ -1187,7 +1188,7 @@ int wr_mixed_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_ro
             a.x = x->resid; a.gather = x->gather + done; a.w = x->final_norm;
             a.width = x->width; a.groups = x->groups; a.eps = x->eps; a.centre = x->centre;
             a.out = x->head_in; a.out_type = head.in_act();
-            if (logits_out || argmax_out) {
+            if (logits_out || argmax_out || beam) {
                 TRY(wr_group_norm_launch(ctx, head.rw, a));
                 TRY(head.product(x->head, x->head_in, x->ldw, x->logits, ldv, WR_ACT_F32));
                 ++m->launches;
@@ -1206,6 +1207,11 @@ int wr_mixed_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_ro
                 m->launches += 2;
                 WR_CUDA_TRY(cudaMemcpyAsync(x->h_best, x->best, head.rw.n_rows * sizeof(uint32_t), cudaMemcpyDeviceToHost, st));
             }
+            if (beam) {                                          // (all rows are asked for, and they are one pass)
+                uint32_t at[WR_CUDA_BATCH_MAX];
+                for (uint32_t i = 0; i < n_out; ++i) at[i] = i;
+                TRY(wr_beam_step_launch(ctx, m, *beam, x->logits, ldv, m->vocab, at));
+            }
             for (uint32_t i = 0; logits_out && i < head.rw.n_rows; ++i) {
                 float *dst = logits_out[x->h_gather[done + i] - out_from];
                 if (dst)
@@ -1221,5 +1227,6 @@ int wr_mixed_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_ro
     for (uint32_t s = 0; s < n_seq; ++s) kv[s]->state_len[slot_out[s]] = (int64_t)positions[s] + per_seq;
     if (argmax_out)
         for (uint32_t i = 0; i < n_out; ++i) argmax_out[i] = x->h_best[i];
+    if (beam) wr_beam_step_finish(m, *beam);
     return WR_CUDA_OK;
 }

@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <mutex>
 #include <vector>
 
@@ -113,6 +114,10 @@ struct wr_cuda_ctx {
     void *stage_host = nullptr;      // pinned
     size_t stage_host_bytes = 0;
     int live_kv = 0;
+    // scratch of wr_ctx_keep, and what it has outgrown: launches that a graph keeps may use either
+    char *kept = nullptr;
+    size_t kept_bytes = 0;
+    std::vector<void *> outgrown;
     uint32_t attr_flags = 0;         // per-device kernel attributes already set
     // SM clock cycles a device-side wait may last before the kernel gives up
     // (wr_cuda_ctx_set_wait_limit); every kernel of the context gets this value.
@@ -135,10 +140,13 @@ struct wr_kv_layer {
     uint64_t state_off = 0, state_bytes = 0;    // inside the session's state slot
 };
 
+struct wr_kv_column;                     // kv_share.cuh
+
 struct wr_cuda_kv {
     wr_cuda_ctx *ctx = nullptr;
     uint32_t n_layers = 0, max_ctx = 0, n_pages = 0;
     std::vector<wr_kv_layer> layers;
+    std::vector<wr_kv_column *> columns;    // the first pages, where they are or were held together with other sessions
     std::vector<void *> pages;       // n_layers * n_pages page pointers (host copy; null where a layer has none)
     uint64_t *d_pages = nullptr;     // same table on the device
     std::vector<uint8_t> contig;     // per layer: pages are consecutive in memory
@@ -218,6 +226,8 @@ int wr_ctx_sync_checked(wr_cuda_ctx *ctx);
 int wr_ctx_reserve_ws(wr_cuda_ctx *ctx, size_t ws_bytes, size_t tickets);
 // The workspace for callers that can do without: where memory does not suffice it stays as it is, and nothing waits.
 int wr_ctx_try_ws(wr_cuda_ctx *ctx, size_t ws_bytes);
+// Scratch that stays where it is for the context's life, all zeros at first: a larger call gets more, elsewhere.
+int wr_ctx_keep(wr_cuda_ctx *ctx, size_t bytes, char **out);
 int wr_kv_batch_check(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer);
 int wr_append_validate(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer,
                        const uint32_t *positions, uint32_t n_tokens, const float *k_rows,
