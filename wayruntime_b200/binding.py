@@ -703,6 +703,10 @@ class DeviceModel:
         return res
 
 
+    def kv_reorder(self, kvs, parents, rows):
+        """Context.kv_reorder for sessions of this model."""
+        self._ctx.kv_reorder(kvs, parents, rows)
+
     def beam_step(self, kvs, positions, tokens, scores, n_out):
         """wr_cuda_model_beam_step: one token for every beam, then the n_out best continuations of every group.  scores: float32
         [groups, beams], the rows of kvs, positions and tokens in that order.  Returns (scores, beams, tokens), [groups, n_out] each."""

@@ -1,7 +1,7 @@
 """Command line over the serving loop.
 
     python -m wayruntime_b200.cli models
-    python -m wayruntime_b200.cli generate --model DIR --prompt 1,2,3 [--prompt 7,8] --max-new 16
+    python -m wayruntime_b200.cli generate --model DIR --prompt 1,2,3 [--prompt 7,8] --max-new 16 [--beams 4]
 
 A model folder has no tokenizer: prompts and results are token ids.
 """
@@ -23,6 +23,12 @@ def generate(a) -> int:
     reqs = [Request(p, a.max_new, Sampling(a.temperature, a.top_k, a.top_p, a.seed + i), frozenset(a.stop))
             for i, p in enumerate(prompts)]
     try:
+        if a.beams:
+            for p in prompts:
+                best = Engine(model).beam_search(p, a.beams, a.max_new, a.stop, a.length_penalty)
+                print(json.dumps({"prompt": p, "output": best[0].tokens, "score": best[0].score,
+                                  "beams": [{"output": h.tokens, "score": h.score} for h in best]}))
+            return 0
         for r in Engine(model).run(reqs):
             print(json.dumps({"prompt": r.prompt, "output": r.output}))
     finally:
@@ -46,8 +52,12 @@ def main(argv=None) -> int:
     g.add_argument("--top-p", type=float, default=1.0)
     g.add_argument("--seed", type=int, default=0)
     g.add_argument("--stop", type=int, action="append", default=[])
+    g.add_argument("--beams", type=int, default=0, help="beam search with this many beams instead of sampling")
+    g.add_argument("--length-penalty", type=float, default=1.0, help="beams rank by score / length ** this")
     g.add_argument("--device", type=int, default=0)
     a = ap.parse_args(argv)
+    if a.command == "generate" and a.beams and a.temperature:
+        ap.error("--beams takes the most probable continuations: no --temperature")
     if a.command == "models":
         from . import models
         print("\n".join(models.architectures()))

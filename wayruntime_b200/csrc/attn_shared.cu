@@ -652,7 +652,7 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
 static int shared_call(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *positions,
                        const uint32_t *seq_lens, uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, float *q,
                        const float *k_rows, const float *v_rows, float *out, uint32_t n_q, float theta_base, uint32_t n_rot_pairs,
-                       uint32_t flags, float scale_override, int mem)
+                       uint32_t flags, float scale_override, int mem, bool dependent)
 {
     const bool append = positions != nullptr;
     const uint32_t n_kv = kv[0]->n_kv_at(layer);
@@ -675,7 +675,8 @@ static int shared_call(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv,
         WR_CUDA_TRY(cudaMemcpyAsync(dq, q, q_bytes, cudaMemcpyHostToDevice, ctx->stream));
     }
     if (append) {
-        rc = wr_append_launch(ctx, n_sess, kv, layer, positions, 1, dk, dv, dq, n_q, theta_base, n_rot_pairs, flags, nullptr);
+        rc = wr_append_launch(ctx, n_sess, kv, layer, positions, 1, dk, dv, dq, n_q, theta_base, n_rot_pairs, flags, nullptr, nullptr,
+                              dependent);
         if (rc != WR_CUDA_OK) return rc;
     }
     rc = wr_shared_launch(ctx, n_sess, kv, layer, seq_lens, n_groups, group_sess, group_rows, dq, dout, n_q, scale_override);
@@ -698,13 +699,13 @@ extern "C" int wr_cuda_attn_decode_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_
     if (rc != WR_CUDA_OK) return rc;
     WR_CUDA_TRY(cudaSetDevice(ctx->device));
     return shared_call(ctx, n_sess, kv, layer, nullptr, seq_lens, n_groups, group_sess, group_rows, const_cast<float *>(q), nullptr,
-                       nullptr, out, n_q_heads, 0.f, 0, 0, scale_override, mem);
+                       nullptr, out, n_q_heads, 0.f, 0, 0, scale_override, mem, true);
 }
 
 int wr_decode_step_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *positions,
                           uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, float *q, const float *k_rows,
                           const float *v_rows, float *out, uint32_t n_q_heads, float theta_base, uint32_t n_rot_pairs, uint32_t flags,
-                          float scale_override, int mem)
+                          float scale_override, int mem, bool dependent)
 {
     int rc = wr_append_validate(ctx, n_sess, kv, layer, positions, 1, k_rows, v_rows, q, n_q_heads, mem);
     if (rc != WR_CUDA_OK) return rc;
@@ -718,7 +719,7 @@ int wr_decode_step_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *
             if (group_rows[g] > positions[i]) return WR_CUDA_ERR_INVAL;
     WR_CUDA_TRY(cudaSetDevice(ctx->device));
     return shared_call(ctx, n_sess, kv, layer, positions, seq_lens, n_groups, group_sess, group_rows, q, k_rows, v_rows, out, n_q_heads,
-                       theta_base, n_rot_pairs, flags, scale_override, mem);
+                       theta_base, n_rot_pairs, flags, scale_override, mem, dependent);
 }
 
 extern "C" int wr_cuda_decode_step_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer,

@@ -37,11 +37,11 @@ int wr_shared_validate(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv,
 int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *seq_lens,
                      uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, const float *dq, float *dout,
                      uint32_t n_q, float scale_override);
-// wr_cuda_decode_step_shared; caller holds ctx->lock
+// wr_cuda_decode_step_shared; dependent: as wr_decode_step's.  Caller holds ctx->lock.
 int wr_decode_step_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *positions,
                           uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, float *q, const float *k_rows,
                           const float *v_rows, float *out, uint32_t n_q_heads, float theta_base, uint32_t n_rot_pairs, uint32_t flags,
-                          float scale_override, int mem);
+                          float scale_override, int mem, bool dependent = true);
 
 // kv_cache.cu: pages from the context's pool; everything a session holds back to it.  Caller holds ctx->lock.
 int wr_pool_take(wr_cuda_ctx *ctx, uint64_t page_bytes, size_t n, size_t *pool_index, std::vector<void *> &out);

@@ -471,6 +471,35 @@ extern "C" uint64_t wr_cuda_model_bytes(const wr_cuda_model *m) { return m ? m->
 extern "C" uint64_t wr_cuda_model_launches(const wr_cuda_model *m) { return m ? m->launches : 0; }
 extern "C" uint64_t wr_cuda_model_last_enqueue_ns(const wr_cuda_model *m) { return m ? m->last_enqueue_ns : 0; }
 
+// Rows of a decode pass whose sessions hold their first kTogether rows or more together: `rows` lists them group after group.
+// Returns how many there are.
+constexpr uint32_t kTogether = 256;
+static uint32_t rows_together(const wr_cuda_model *m, uint32_t n_rows, wr_cuda_kv *const *kv, uint32_t *rows, uint32_t *n_groups,
+                              uint32_t *group_sess, uint32_t *group_rows)
+{
+    uint32_t n = 0;
+    *n_groups = 0;
+    if (m->hd != 128) return 0;
+    bool taken[WR_CUDA_BATCH_MAX] = {};
+    for (uint32_t r = 0; r < n_rows; ++r) {
+        if (taken[r] || kv[r]->columns.empty()) continue;
+        uint32_t pages = ~0u, first = n;
+        for (uint32_t t = r + 1; t < n_rows; ++t) {
+            if (taken[t] || kv[t] == kv[r]) continue;
+            const uint32_t common = wr_kv_common_pages(kv[r], kv[t]);
+            if (common * kPageTokens < kTogether) continue;
+            if (n == first) rows[n++] = r;
+            rows[n++] = t;
+            taken[t] = true;
+            pages = std::min(pages, common);
+        }
+        if (n == first) continue;
+        group_sess[*n_groups] = n - first;
+        group_rows[(*n_groups)++] = pages * kPageTokens;
+    }
+    return n;
+}
+
 // A forward pass; `beam`, when given, gets its choice from the logits of all rows (wr_cuda_model_beam_step).
 static int forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_rows, wr_cuda_kv *const *kv, const uint32_t *positions,
                    const uint32_t *tokens, uint32_t out_from, float *hidden_out, float *normed_out, float *const *logits_out,
@@ -503,24 +532,34 @@ static int forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_rows
     const uint32_t hid = m->hidden, nq = m->n_q * m->hd, nkv = m->n_kv * m->hd;
 
     // Decode rows are processed in an order of their own: the sessions that the one-kernel
-    // short-context step covers first, the others after them, so that each kind is a contiguous
-    // block of rows.  Which kind a session is depends on that session alone.  perm[i] = caller's row.
-    uint32_t perm[WR_CUDA_BATCH_MAX], pos_p[WR_CUDA_BATCH_MAX], n_short = 0;
+    // short-context step covers first, the others after them, those that hold a long beginning
+    // together last, so that each kind is a contiguous block of rows.  Which of the first two kinds a session is
+    // depends on that session alone.  perm[i] = caller's row.
+    uint32_t perm[WR_CUDA_BATCH_MAX], pos_p[WR_CUDA_BATCH_MAX], n_short = 0, n_apart = 0, n_groups = 0;
+    uint32_t group_sess[WR_CUDA_BATCH_MAX], group_rows[WR_CUDA_BATCH_MAX];
     wr_cuda_kv *kv_p[WR_CUDA_BATCH_MAX];
     bool permuted = false;
     if (mode == WR_CUDA_FWD_DECODE) {
         const bool use_small = (getenv("WR_CUDA_STEP_SMALL_OFF") == nullptr);
+        uint32_t together[WR_CUDA_BATCH_MAX];            // rows
+        n_apart = n_rows - rows_together(m, n_rows, kv, together, &n_groups, group_sess, group_rows);
+        bool apart[WR_CUDA_BATCH_MAX];
+        std::fill(apart, apart + n_rows, true);
+        for (uint32_t i = 0; i < n_rows - n_apart; ++i) {
+            perm[n_apart + i] = together[i];
+            apart[together[i]] = false;
+        }
         uint32_t n = 0;
         for (int pass = 0; pass < 2; ++pass)
             for (uint32_t r = 0; r < n_rows; ++r) {
                 const bool small = use_small && wr_step_small_covers(kv[r], 0, m->n_q, positions[r]);
-                if (small == (pass == 0)) perm[n++] = r;
+                if (apart[r] && small == (pass == 0)) perm[n++] = r;
             }
         for (uint32_t i = 0; i < n_rows; ++i) {
             if (perm[i] != i) permuted = true;
             kv_p[i] = kv[perm[i]];
             pos_p[i] = positions[perm[i]];
-            if (use_small && wr_step_small_covers(kv_p[i], 0, m->n_q, pos_p[i])) n_short = i + 1;
+            if (i < n_apart && use_small && wr_step_small_covers(kv_p[i], 0, m->n_q, pos_p[i])) n_short = i + 1;
             if (pos_p[i] >= kv_p[i]->max_ctx) return WR_CUDA_ERR_CTX_FULL;
         }
     }
@@ -600,11 +639,21 @@ static int forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_rows
             if (n_short < n_rows) {
                 // (without head norms it is the append that has to be an ordinary launch beside the short sessions' kernel: 16
                 // sessions of 200 to 1900 tokens, 16 q and 8 kv heads: 106 -> 85 us a layer)
-                rc = wr_decode_step(ctx, n_rows - n_short, kv_p + n_short, L, pos_p + n_short, m->q + (size_t)n_short * nq,
-                                    m->k + (size_t)n_short * nkv, m->v + (size_t)n_short * nkv, m->attn + (size_t)n_short * nq,
-                                    m->n_q, m->theta, m->n_rot, WR_CUDA_APPEND_ROPE, m->scale, 0, WR_CUDA_MEM_DEVICE,
-                                    l.q_norm != nullptr || !n_short || !m->side);
-                if (rc != WR_CUDA_OK) return rc;
+                const bool dependent = l.q_norm != nullptr || !n_short || !m->side;
+                if (n_short < n_apart) {
+                    rc = wr_decode_step(ctx, n_apart - n_short, kv_p + n_short, L, pos_p + n_short, m->q + (size_t)n_short * nq,
+                                        m->k + (size_t)n_short * nkv, m->v + (size_t)n_short * nkv, m->attn + (size_t)n_short * nq,
+                                        m->n_q, m->theta, m->n_rot, WR_CUDA_APPEND_ROPE, m->scale, 0, WR_CUDA_MEM_DEVICE, dependent);
+                    if (rc != WR_CUDA_OK) return rc;
+                }
+                if (n_groups) {
+                    std::lock_guard<std::mutex> g(ctx->lock);
+                    rc = wr_decode_step_shared(ctx, n_rows - n_apart, kv_p + n_apart, L, pos_p + n_apart, n_groups, group_sess,
+                                               group_rows, m->q + (size_t)n_apart * nq, m->k + (size_t)n_apart * nkv,
+                                               m->v + (size_t)n_apart * nkv, m->attn + (size_t)n_apart * nq, m->n_q, m->theta,
+                                               m->n_rot, WR_CUDA_APPEND_ROPE, m->scale, WR_CUDA_MEM_DEVICE, dependent);
+                    if (rc != WR_CUDA_OK) return rc;
+                }
                 if (n_short && m->side) WR_CUDA_TRY(cudaStreamWaitEvent(st, m->join, 0));
             }
         } else {

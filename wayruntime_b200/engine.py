@@ -14,7 +14,7 @@ from dataclasses import dataclass, field
 
 import numpy as np
 
-from .binding import BATCH_MAX
+from .binding import BATCH_MAX, BEAM_MAX_OUT, NO_BEAM
 
 
 @dataclass
@@ -35,6 +35,22 @@ class Session:
 
     def close(self):
         self.kv.close()
+
+    def fork(self) -> "Session":
+        """A session that goes on from here; what both hold is kept once, page by page."""
+        s = Session.__new__(Session)
+        s.kv, s.max_ctx, s.pos = self.kv.fork(self.pos), self.max_ctx, self.pos
+        return s
+
+
+@dataclass
+class Hypothesis:
+    """A continuation that a beam search has found: its tokens and the sum of their log probabilities."""
+    tokens: list
+    score: float
+
+    def rank(self, length_penalty: float) -> float:
+        return self.score / len(self.tokens) ** length_penalty
 
 
 @dataclass
@@ -133,6 +149,66 @@ class Engine:
             return np.empty((0, m.vocab), np.float32)
         rows = parts[0] if len(parts) == 1 else np.concatenate(parts)
         return rows if order == list(want) else rows[[order.index(w) for w in want]]
+
+    # ---- beam search
+
+    def beam_search(self, prompt, beams: int, max_new: int, stop=frozenset(), length_penalty: float = 1.0) -> list:
+        """The best continuations of a prompt, at most `beams`, as Hypothesis, by score / length ** length_penalty.  One ends
+        with a stop id or after max_new tokens; the search ends when `beams` have ended and none that goes on ranks above
+        the last of them as it stands.  The beams' sessions are forks of the prompt's: its pages are kept once, and a step
+        attends to them once for all beams where the model's stack does that (wr_cuda_model_beam_step)."""
+        stop = frozenset(stop)
+        if not prompt or max_new < 1:
+            raise ValueError("a prompt token and a new one at least")
+        if not 1 <= beams <= BATCH_MAX:
+            raise ValueError(f"1 to {BATCH_MAX} beams")
+        m, n_out = self.model, min((1 + len(stop)) * beams, BEAM_MAX_OUT)
+        sessions, histories, ended = [self.session(len(prompt) + max_new)], [[]], []
+        rank = lambda h: h.rank(length_penalty)  # noqa: E731
+        try:
+            if len(prompt) > 1:
+                self.advance(sessions, [prompt[:-1]], [[]])
+            tokens, scores = [prompt[-1]], [0.0]
+            while True:
+                live = sessions[:len(tokens)]
+                found = m.beam_step([s.kv for s in live], [s.pos for s in live], tokens, [scores], n_out)
+                for s in live:
+                    s.pos += 1
+                going = []                               # (score, parent, token), best first
+                for place, (score, parent, token) in enumerate(zip(*(x[0].tolist() for x in found))):
+                    if parent == NO_BEAM or len(going) == beams:
+                        break
+                    if token not in stop:
+                        going.append((score, parent, token))
+                    elif place < beams:
+                        ended.append(Hypothesis(histories[parent] + [token], score))
+                length = len(histories[0]) + 1
+                if length == max_new:
+                    ended += [Hypothesis(histories[p] + [t], s) for s, p, t in going]
+                    break
+                ended = sorted(ended, key=rank, reverse=True)[:beams]
+                if not going or (len(ended) == beams and rank(ended[-1]) >= going[0][0] / length ** length_penalty):
+                    break
+                parents = [p for _, p, _ in going]
+                self._follow(sessions, parents, beams)
+                histories = [histories[p] + [t] for _, p, t in going]
+                tokens, scores = [t for _, _, t in going], [s for s, _, _ in going]
+        finally:
+            for s in sessions:
+                s.close()
+        return sorted(ended, key=rank, reverse=True)[:beams]
+
+    def _follow(self, sessions, parents, beams):
+        """Sessions [0, len(parents)) go on from those that parents names.  The others wait until there are more beams again."""
+        if len(sessions) < beams:                        # (the prompt's session: every beam goes on from it)
+            sessions += [sessions[0].fork() for _ in range(1, beams)]
+            return
+        spare = [i for i in range(beams) if i not in parents]            # (nobody goes on from these: who waits takes them)
+        order, at = parents + spare[:beams - len(parents)], [s.pos for s in sessions]
+        if order != list(range(beams)):
+            self.model.kv_reorder([s.kv for s in sessions], order, at)
+            for s, p in zip(sessions, order):
+                s.pos = at[p]
 
     # ---- scheduling
 
