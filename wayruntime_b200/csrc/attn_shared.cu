@@ -25,6 +25,7 @@
 // registers: the accumulator rounds towards zero, which over a long chunk would show.
 // Every wait is bounded by the context's wait limit.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_share.cuh"
 #include "tcgen05_dev.cuh"
@@ -32,12 +33,12 @@
 
 namespace {
 
-constexpr uint32_t kHd = 128, kTile = 128, kMaxQ = 64, kThreads = 224;
+constexpr uint32_t kHd = 128, kTile = 128, kMaxQ = 64, kThreads = 352;     // 3 warps of their own, two groups of four
 constexpr uint32_t kPageBlock = kPageTokens * kHd * 2, kSlot = 2 * kPageBlock;   // K or V of a page, of a tile
-constexpr uint32_t kBox = kTile * 128, kQBox = kMaxQ * 128;                      // 64 dims of a tile's keys, of the queries
-constexpr uint32_t kQBytes = 4 * kQBox, kPBytes = 2 * kTile * 128;               // high and low parts
+constexpr uint32_t kBox = kTile * 128;                                           // 64 dims of a tile's keys
+constexpr uint32_t kQBytes = 4 * kMaxQ * 128, kPBytes = 2 * kTile * 128;         // high and low parts
 constexpr uint32_t kKSlots = 2, kVSlots = 3, kItemSlots = 8;
-constexpr uint32_t kTmemCols = 256, kTmemO = 128;                                // two buffers of 64 columns each
+constexpr uint32_t kTmemCols = 512, kTmemO = 256;                                // two buffers of 128 columns each
 constexpr uint32_t kMaxSegs = 2 * WR_CUDA_BATCH_MAX, kMaxParts = 1024;
 constexpr float kGrow = 8.0f, kLog2e = 1.4426950408889634f;
 
@@ -73,7 +74,7 @@ struct Bars {
     Item item[kItemSlots];
     uint32_t tmem;
     alignas(16) float c[2][kMaxQ];       // per query: score to log2
-    alignas(16) float m[kMaxQ], a[kMaxQ];
+    alignas(16) float nm[kMaxQ], a[kMaxQ];           // reference, negative; factor of its last change
     alignas(16) float red[kMaxQ][4];
 };
 constexpr uint32_t kSmem = kKSlots * kSlot + kVSlots * kSlot + kQBytes + kPBytes + (uint32_t)sizeof(Bars);
@@ -100,12 +101,14 @@ __device__ __forceinline__ Item item_of(const SharedParams &p, uint32_t i)
     it.part = g.part0 + (chunk * p.n_kv + it.kvh) * g.queries + it.q0;
     return it;
 }
-__device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-__device__ __forceinline__ bool group_or(bool x)
+// The queries of an item, rounded up to what a group of threads has at its fixed sizes: half of them each.
+__host__ __device__ __forceinline__ uint32_t padded(uint32_t nq) { return nq <= 16 ? 16u : nq <= 32 ? 32u : 64u; }
+__device__ __forceinline__ void group_sync(uint32_t id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool group_or(uint32_t id, uint32_t threads, bool x)
 {
     uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                 : "=r"(r) : "r"((uint32_t)x) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbar.red.or.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"(id), "r"(threads), "r"((uint32_t)x) : "memory");
     return r != 0;
 }
 __device__ __forceinline__ float ex2(float x)
@@ -114,20 +117,31 @@ __device__ __forceinline__ float ex2(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Largest of the warp's 32 lanes for each of 32 values: v[0] holds that of the value whose index is returned.
-__device__ __forceinline__ uint32_t warp_max_32(float (&v)[32], uint32_t lane)
+// H consecutive columns of this thread's TMEM lane (no wait)
+template <uint32_t H> __device__ __forceinline__ void tmem_ld(uint32_t at, float (&v)[H])
+{
+    if constexpr (H == 32) tc5::ld32(at, v);
+    else if constexpr (H == 16) tc5::ld16(at, v);
+    else tc5::ld8(at, v);
+}
+// Largest of the warp's 32 lanes for each of H values: v[0] holds that of the value whose index is returned.
+template <uint32_t H> __device__ __forceinline__ uint32_t warp_max_many(float (&v)[H], uint32_t lane)
 {
     uint32_t idx = 0;
 #pragma unroll
-    for (uint32_t o = 16, half = 16; o >= 1; o >>= 1, half >>= 1) {
-        const bool upper = (lane & o) != 0;
+    for (uint32_t o = 16, half = H / 2; o >= 1; o >>= 1, half >>= 1) {
+        if (half) {
+            const bool upper = (lane & o) != 0;
 #pragma unroll
-        for (uint32_t i = 0; i < 16; ++i)
-            if (i < half) {
-                const float send = upper ? v[i] : v[i + half], keep = upper ? v[i + half] : v[i];
-                v[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, o));
-            }
-        if (upper) idx += half;
+            for (uint32_t i = 0; i < H / 2; ++i)
+                if (i < half) {
+                    const float send = upper ? v[i] : v[i + half], keep = upper ? v[i + half] : v[i];
+                    v[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, o));
+                }
+            if (upper) idx += half;
+        } else {
+            v[0] = fmaxf(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+        }
     }
     return idx;
 }
@@ -150,10 +164,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             mbar_init(&sm.v_free[i], 1);
         }
         for (uint32_t i = 0; i < kItemSlots; ++i) mbar_init(&sm.item_ready[i], 1);
-        mbar_init(&sm.q_full, 4);
+        mbar_init(&sm.q_full, 8);
         mbar_init(&sm.s_full[0], 1);
         mbar_init(&sm.s_full[1], 1);
-        mbar_init(&sm.p_full, 4);
+        mbar_init(&sm.p_full, 8);
         mbar_init(&sm.o_full, 1);
         mbar_init(&sm.drained, 1);
         fence_barrier_init();
@@ -211,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             for (uint32_t i = n - min(n, kKSlots); i < n; ++i) (void)mbar_wait(&sm.k_full[i % kKSlots], (i / kKSlots) & 1, limit);
         }
         __syncwarp();
-    } else if (warp == 6) {
+    } else if (warp == 2) {
         if (lane == 0) {                                         // V
             uint32_t n = 0;
             bool ok = true;
@@ -245,13 +259,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             const uint32_t st = n_s % kKSlots;
             if (!mbar_wait_warp(&sm.k_full[st], (n_s / kKSlots) & 1, limit)) return false;
             tc5::fence_after();
-            const uint32_t d = tmem + (n_s & 1) * kMaxQ, idesc = tc5::idesc_f16(128, n);
+            const uint32_t d = tmem + (n_s & 1) * 2 * kMaxQ, idesc = tc5::idesc_f16(128, n);
             const uint64_t a = tc5::desc_kmajor(k_addr + st * kSlot), b = tc5::desc_kmajor(q_addr);
 #pragma unroll
-            for (uint32_t kk = 0; kk < 16; ++kk) {               // the queries' low parts, then the high ones
-                const uint32_t half = (kk >> 2) & 1, step = 2 * (kk & 3);
-                if (lead) tc5::mma_ss(d, a + half * (kBox >> 4) + step, b + ((kk >> 2) ^ 2) * (kQBox >> 4) + step, idesc, kk != 0);
-            }
+            for (uint32_t kk = 0; kk < 8; ++kk)                  // 16 dims a step
+                if (lead) tc5::mma_ss(d, a + (kk >> 2) * (kBox >> 4) + 2 * (kk & 3), b + (kk >> 2) * (n * 128 >> 4) + 2 * (kk & 3), idesc, kk != 0);
             if (lead) {
                 tc5::commit(&sm.k_free[st]);
                 tc5::commit(&sm.s_full[n_s & 1]);
@@ -262,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
         for (uint32_t it = 0; ok; ++it) {
             const Item im = item_at(it, ok, true);
             if (!im.tiles) break;
-            const uint32_t n = (im.nq + 15) & ~15u;
+            const uint32_t n = 2 * padded(im.nq);
             ok = mbar_wait_warp(&sm.q_full, it & 1, limit) && score(n);
             for (uint32_t t = 0; t < im.tiles && ok; ++t) {
                 // (the scores two tiles ago have been read: their P has been waited for)
@@ -272,15 +284,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                 ok = ok && mbar_wait_warp(&sm.v_full[st], (n_o / kVSlots) & 1, limit);
                 if (!ok) break;
                 tc5::fence_after();
-                const uint32_t d = tmem + kTmemO + (n_o & 1) * kMaxQ, idesc = idesc_values(n);
-                const uint64_t a = tc5::desc_mnmajor(v_addr + st * kSlot, 8192), b = tc5::desc_mnmajor(p_addr, 8192);
+                const uint32_t d = tmem + kTmemO + (n_o & 1) * 2 * kMaxQ, idesc = idesc_values(n);
+                const uint64_t a = tc5::desc_mnmajor(v_addr + st * kSlot, 8192), b = tc5::desc_mnmajor(p_addr, kTile * 128);
 #pragma unroll
-                for (uint32_t kk = 0; kk < 16; ++kk) {           // 16 keys a step; P's low parts, then the high ones
-                    const uint32_t step = kk & 7;
+                for (uint32_t kk = 0; kk < 8; ++kk)              // 16 keys a step
                     if (lead)
-                        tc5::mma_ss(d, a + (step >> 2) * (kPageBlock >> 4) + (step & 3) * (2048 >> 4),
-                                    b + ((kk >> 3) ^ 1) * (kTile * 128 >> 4) + step * (2048 >> 4), idesc, kk != 0);
-                }
+                        tc5::mma_ss(d, a + (kk >> 2) * (kPageBlock >> 4) + (kk & 3) * (2048 >> 4), b + kk * (2048 >> 4), idesc, kk != 0);
                 if (lead) {
                     tc5::commit(&sm.v_free[st]);
                     tc5::commit(&sm.o_full);
@@ -293,19 +302,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
         if (lead) tc5::commit(&sm.drained);                      // no product is running when the TMEM is given back
         (void)mbar_wait_warp(&sm.drained, 0, limit);
     } else {
-        // a thread per key (scores) and per value dimension (output): its TMEM lane either way
-        const uint32_t quarter = warp & 3, key = quarter * 32 + lane, tid = threadIdx.x - 64, lanes = (quarter * 32) << 16;
+        // a thread per key (scores) and per value dimension (output): its TMEM lane either way; each group has half of the queries
+        const uint32_t quarter = warp & 3, group = (warp - 3) >> 2, key = quarter * 32 + lane, tid = (threadIdx.x - 96) & 127;
+        const uint32_t bar = 1 + group, lanes = (quarter * 32) << 16;
         uint32_t n = 0;                                          // tiles so far
         bool ok = true;
         // The item's queries as operands: against the power of two of their row, high and low F16 parts.
         auto queries = [&](const Item &im, uint32_t it) {
-            const uint32_t rows = (im.nq + 15) & ~15u;
+            const uint32_t rows = padded(im.nq);
 #pragma unroll 1
-            for (uint32_t r0 = tid >> 5; r0 < rows; r0 += 16) {
+            for (uint32_t r0 = warp - 3; r0 < rows; r0 += 32) {
                 float4 x[4];
 #pragma unroll
                 for (uint32_t u = 0; u < 4; ++u) {
-                    const uint32_t r = r0 + 4 * u, qi = im.q0 + r;
+                    const uint32_t r = r0 + 8 * u, qi = im.q0 + r;
                     x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (r < im.nq)
                         x[u] = __ldg(reinterpret_cast<const float4 *>(
@@ -313,143 +323,140 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                 }
 #pragma unroll
                 for (uint32_t u = 0; u < 4; ++u) {
-                    const uint32_t r = r0 + 4 * u;
+                    const uint32_t r = r0 + 8 * u;
                     float top = fmaxf(fmaxf(fabsf(x[u].x), fabsf(x[u].y)), fmaxf(fabsf(x[u].z), fabsf(x[u].w)));
 #pragma unroll
                     for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                     const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 126);
                     const float down = __int_as_float((127 - e) << 23);
-                    const float y[4] = {x[u].x * down, x[u].y * down, x[u].z * down, x[u].w * down};
                     uint32_t hi[2], lo[2];
-                    split_half2(y[0], y[1], hi[0], lo[0]);
-                    split_half2(y[2], y[3], hi[1], lo[1]);
+                    split_half2(x[u].x * down, x[u].y * down, hi[0], lo[0]);
+                    split_half2(x[u].z * down, x[u].w * down, hi[1], lo[1]);
                     if (r < rows) {
-                        uint8_t *at = qs + (lane >> 4) * kQBox + r * 128 + ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
+                        // (rows and rows more: a multiple of 16, so the swizzle is the same)
+                        uint8_t *at = qs + (lane >> 4) * (2 * rows * 128) + r * 128 + ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
                         *reinterpret_cast<uint2 *>(at) = make_uint2(hi[0], hi[1]);
-                        *reinterpret_cast<uint2 *>(at + 2 * kQBox) = make_uint2(lo[0], lo[1]);
+                        *reinterpret_cast<uint2 *>(at + rows * 128) = make_uint2(lo[0], lo[1]);
                         if (lane == 0) sm.c[it & 1][r] = p.scale_log2 * __int_as_float((127 + e) << 23);
                     }
                 }
             }
             fence_proxy_async();
-            group_sync();
+            asm volatile("bar.sync 3, 256;" ::: "memory");       // (sm.c, for all of both groups)
             if (lane == 0) mbar_arrive(&sm.q_full);
         };
         Item im = item_at(0, ok, true);
-        // (a warp whose wait ran out stays with the others: they leave together, and the group's barriers count on all four)
-        ok = !group_or(!ok);
+        // (a warp whose wait ran out stays with the others: they leave together, and the groups' barriers count on all of them)
+        ok = !group_or(3, 256, !ok);
         if (ok && im.tiles) queries(im, 0);
-        for (uint32_t it = 0; ok && im.tiles; ++it) {
-            const uint32_t nb = (im.nq + 15) >> 4;               // blocks of 16 queries
-            const float4 *const c4 = reinterpret_cast<const float4 *>(sm.c[it & 1]), *const m4 = reinterpret_cast<const float4 *>(sm.m);
-            const float4 *const a4 = reinterpret_cast<const float4 *>(sm.a);
-            float o[kMaxQ], l[kMaxQ];
+        Item following{};
+        auto work = [&](auto size, uint32_t it) {
+            constexpr uint32_t NQ = decltype(size)::value, H = NQ / 2;
+            const uint32_t q0 = group * H;                       // this group's first query
+            const float4 *const c4 = reinterpret_cast<const float4 *>(sm.c[it & 1] + q0), *const nm4 = reinterpret_cast<const float4 *>(sm.nm + q0);
+            const float4 *const a4 = reinterpret_cast<const float4 *>(sm.a + q0);
+            float o[H], l[H];
 #pragma unroll
-            for (uint32_t j = 0; j < kMaxQ; ++j) o[j] = l[j] = 0.f;
+            for (uint32_t j = 0; j < H; ++j) o[j] = l[j] = 0.f;
             auto add_values = [&](uint32_t tile, bool scaled) {  // O^T of a finished tile; then the change of reference
-                const uint32_t at = tmem + kTmemO + (tile & 1) * kMaxQ + lanes;
+                const uint32_t at = tmem + kTmemO + (tile & 1) * 2 * kMaxQ + lanes + q0;
+                float hi[H], lo[H];
+                tmem_ld(at, hi);
+                tmem_ld(at + NQ, lo);
+                tc5::wait_ld();
 #pragma unroll
-                for (uint32_t b = 0; b < 4; ++b)
-                    if (b < nb) {
-                        float v[16];
-                        tc5::ld16(at + 16 * b, v);
-                        tc5::wait_ld();
-#pragma unroll
-                        for (uint32_t j = 0; j < 16; ++j) o[16 * b + j] += v[j];
-                    }
+                for (uint32_t j = 0; j < H; ++j) o[j] += hi[j] + lo[j];
                 if (scaled) {
 #pragma unroll
-                    for (uint32_t j = 0; j < kMaxQ; j += 4)
-                        if (j < 16 * nb) {
-                            const float4 a = a4[j / 4];
-                            o[j] *= a.x; o[j + 1] *= a.y; o[j + 2] *= a.z; o[j + 3] *= a.w;
-                        }
+                    for (uint32_t j = 0; j < H; j += 4) {
+                        const float4 a = a4[j / 4];
+                        o[j] *= a.x; o[j + 1] *= a.y; o[j + 2] *= a.z; o[j + 3] *= a.w;
+                    }
                 }
             };
             for (uint32_t t = 0; t < im.tiles; ++t, ++n) {
                 if (ok) ok = mbar_wait_warp(&sm.s_full[n & 1], (n >> 1) & 1, limit);
                 tc5::fence_after();
-                const uint32_t at = tmem + (n & 1) * kMaxQ + lanes, here = im.rows - (im.tile0 + t) * kTile;
+                const uint32_t at = tmem + (n & 1) * 2 * kMaxQ + lanes + q0, here = im.rows - (im.tile0 + t) * kTile;
                 const bool seen = key < here;
-                float s[kMaxQ];
+                float s[H];
                 auto scores = [&]() {
-#pragma unroll
-                    for (uint32_t b = 0; b < 4; ++b)
-                        if (b < nb) tc5::ld16(at + 16 * b, s + 16 * b);
+                    float lo[H];
+                    tmem_ld(at, s);
+                    tmem_ld(at + NQ, lo);
                     tc5::wait_ld();
+#pragma unroll
+                    for (uint32_t j = 0; j < H; ++j) s[j] += lo[j];
                 };
                 scores();
                 bool moved = t == 0;
                 if (!moved) {
-                    bool above = false;
+                    float top = -INFINITY;
 #pragma unroll
-                    for (uint32_t j = 0; j < kMaxQ; j += 4)
-                        if (j < 16 * nb) {
-                            const float4 c = c4[j / 4], m = m4[j / 4];
-                            s[j] = fmaf(s[j], c.x, -m.x);
-                            s[j + 1] = fmaf(s[j + 1], c.y, -m.y);
-                            s[j + 2] = fmaf(s[j + 2], c.z, -m.z);
-                            s[j + 3] = fmaf(s[j + 3], c.w, -m.w);
-                            above |= fmaxf(fmaxf(s[j], s[j + 1]), fmaxf(s[j + 2], s[j + 3])) > kGrow;
-                        }
-                    moved = group_or(above && seen);
+                    for (uint32_t j = 0; j < H; j += 4) {
+                        const float4 c = c4[j / 4], m = nm4[j / 4];
+                        s[j] = fmaf(s[j], c.x, m.x);
+                        s[j + 1] = fmaf(s[j + 1], c.y, m.y);
+                        s[j + 2] = fmaf(s[j + 2], c.z, m.z);
+                        s[j + 3] = fmaf(s[j + 3], c.w, m.w);
+                        top = fmaxf(fmaxf(top, fmaxf(s[j], s[j + 1])), fmaxf(s[j + 2], s[j + 3]));
+                    }
+                    moved = group_or(bar, 128, seen && top > kGrow);
                     if (moved) scores();
                 }
-                if (moved) {                                     // (the same in all threads)
+                if (moved) {                                     // (the same in all threads of the group)
 #pragma unroll
-                    for (uint32_t j = 0; j < kMaxQ; j += 4)
-                        if (j < 16 * nb) {
-                            const float4 c = c4[j / 4];
-                            s[j] = seen ? s[j] * c.x : WR_NEG_SENTINEL;
-                            s[j + 1] = seen ? s[j + 1] * c.y : WR_NEG_SENTINEL;
-                            s[j + 2] = seen ? s[j + 2] * c.z : WR_NEG_SENTINEL;
-                            s[j + 3] = seen ? s[j + 3] * c.w : WR_NEG_SENTINEL;
-                        }
-#pragma unroll
-                    for (uint32_t h = 0; h < 2; ++h)
-                        if (2 * h < nb) {
-                            float v[32];
-#pragma unroll
-                            for (uint32_t j = 0; j < 32; ++j) v[j] = j < 16 || 2 * h + 1 < nb ? s[32 * h + j] : WR_NEG_SENTINEL;
-                            const uint32_t idx = warp_max_32(v, lane);
-                            sm.red[32 * h + idx][quarter] = v[0];
-                        }
-                    group_sync();
-                    if (tid < kMaxQ) {
-                        const float4 w = *reinterpret_cast<const float4 *>(sm.red[tid]);
-                        const float top = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), WR_NEG_SENTINEL), old = sm.m[tid];
-                        const bool up = t == 0 || top > old + kGrow;
-                        sm.a[tid] = t == 0 ? 0.f : up ? ex2(old - top) : 1.f;
-                        if (up) sm.m[tid] = top;
+                    for (uint32_t j = 0; j < H; j += 4) {
+                        const float4 c = c4[j / 4];
+                        s[j] = seen ? s[j] * c.x : WR_NEG_SENTINEL;
+                        s[j + 1] = seen ? s[j + 1] * c.y : WR_NEG_SENTINEL;
+                        s[j + 2] = seen ? s[j + 2] * c.z : WR_NEG_SENTINEL;
+                        s[j + 3] = seen ? s[j + 3] * c.w : WR_NEG_SENTINEL;
                     }
-                    group_sync();
+                    float v[H];
 #pragma unroll
-                    for (uint32_t j = 0; j < kMaxQ; j += 4)
-                        if (j < 16 * nb) {
-                            const float4 m = m4[j / 4], a = a4[j / 4];
-                            s[j] -= m.x; s[j + 1] -= m.y; s[j + 2] -= m.z; s[j + 3] -= m.w;
-                            l[j] *= a.x; l[j + 1] *= a.y; l[j + 2] *= a.z; l[j + 3] *= a.w;
-                        }
+                    for (uint32_t j = 0; j < H; ++j) v[j] = s[j];
+                    const uint32_t idx = warp_max_many<H>(v, lane);
+                    sm.red[q0 + idx][quarter] = v[0];            // (lanes that share an index hold one value)
+                    group_sync(bar);
+                    if (tid < H) {
+                        const float4 w = *reinterpret_cast<const float4 *>(sm.red[q0 + tid]);
+                        const float top = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), WR_NEG_SENTINEL), old = -sm.nm[q0 + tid];
+                        const bool up = t == 0 || top > old + kGrow;
+                        sm.a[q0 + tid] = t == 0 ? 0.f : up ? ex2(old - top) : 1.f;
+                        if (up) sm.nm[q0 + tid] = -top;
+                    }
+                    group_sync(bar);
+#pragma unroll
+                    for (uint32_t j = 0; j < H; j += 4) {
+                        const float4 m = nm4[j / 4], a = a4[j / 4];
+                        s[j] += m.x; s[j + 1] += m.y; s[j + 2] += m.z; s[j + 3] += m.w;
+                        l[j] *= a.x; l[j + 1] *= a.y; l[j + 2] *= a.z; l[j + 3] *= a.w;
+                    }
                 }
                 // the tile before has been multiplied: P is free, its O^T is there
                 if (ok && n > 0) ok = mbar_wait_warp(&sm.o_full, (n - 1) & 1, limit);
                 tc5::fence_after();
 #pragma unroll
-                for (uint32_t j = 0; j < kMaxQ; j += 8)
-                    if (j < 16 * nb) {
-                        uint32_t hi[4], lo[4];
+                for (uint32_t j = 0; j < H; j += 8) {
+                    uint32_t hi[4], lo[4];
 #pragma unroll
-                        for (uint32_t e = 0; e < 4; ++e) {
-                            const float w0 = seen ? ex2(s[j + 2 * e]) : 0.f, w1 = seen ? ex2(s[j + 2 * e + 1]) : 0.f;
-                            l[j + 2 * e] += w0;
-                            l[j + 2 * e + 1] += w1;
-                            split_half2(w0, w1, hi[e], lo[e]);
-                        }
-                        uint8_t *to = ps + key * 128 + (((j >> 3) ^ (key & 7)) << 4);
-                        *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4 *>(to + kTile * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        const float w0 = seen ? ex2(s[j + 2 * e]) : 0.f, w1 = seen ? ex2(s[j + 2 * e + 1]) : 0.f;
+                        l[j + 2 * e] += w0;
+                        l[j + 2 * e + 1] += w1;
+                        split_half2(w0, w1, hi[e], lo[e]);
                     }
-                if (here < kTile) {
+                    // a key's row: the high parts of up to 64 queries, the low ones behind them or in rows of their own
+                    const uint32_t c = (q0 + j) >> 3;
+                    uint8_t *const row = ps + key * 128;
+                    *reinterpret_cast<uint4 *>(row + ((c ^ (key & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if constexpr (NQ == 64)
+                        *reinterpret_cast<uint4 *>(row + kTile * 128 + ((c ^ (key & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    else
+                        *reinterpret_cast<uint4 *>(row + (((c + NQ / 8) ^ (key & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+                if (here < kTile && group == 0) {
                     // rows behind the last one may hold anything, and a weight of zero does not take a NaN out
                     const uint32_t st = n % kVSlots;
                     if (ok) ok = mbar_wait_warp(&sm.v_full[st], (n / kVSlots) & 1, limit);
@@ -468,31 +475,31 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             }
             // the next item's queries (the last scores have been read), then this one's results
             bool more = true;
-            const Item following = item_at(it + 1, more, true);
-            ok = !group_or(!(ok && more));
+            following = item_at(it + 1, more, true);
+            ok = !group_or(3, 256, !(ok && more));
             if (ok && following.tiles) queries(following, it + 1);
             if (ok) ok = mbar_wait_warp(&sm.o_full, (n - 1) & 1, limit);
             tc5::fence_after();
             add_values(n - 1, false);
-            float *to = p.o + (size_t)im.part * kHd + key;
+            float *to = p.o + (size_t)(im.part + q0) * kHd + key;
 #pragma unroll
-            for (uint32_t j = 0; j < kMaxQ; ++j)
-                if (j < im.nq) to[(size_t)j * kHd] = o[j];
-#pragma unroll
-            for (uint32_t h = 0; h < 2; ++h)
-                if (2 * h < nb) {
-                    float v[32];
-#pragma unroll
-                    for (uint32_t j = 0; j < 32; ++j) v[j] = l[32 * h + j];
-                    const int idx = warp_reduce_many<32>(v, (int)lane);
-                    sm.red[32 * h + idx][quarter] = v[0];
-                }
-            group_sync();
-            if (tid < im.nq) {
-                const float4 w = *reinterpret_cast<const float4 *>(sm.red[tid]);
-                p.ml[im.part + tid] = make_float2(sm.m[tid], (w.x + w.y) + (w.z + w.w));
+            for (uint32_t j = 0; j < H; ++j)
+                if (q0 + j < im.nq) to[(size_t)j * kHd] = o[j];
+            const int idx = warp_reduce_many<(int)H>(l, (int)lane);
+            sm.red[q0 + idx][quarter] = l[0];
+            group_sync(bar);
+            if (tid < H && q0 + tid < im.nq) {
+                const float4 w = *reinterpret_cast<const float4 *>(sm.red[q0 + tid]);
+                p.ml[im.part + q0 + tid] = make_float2(-sm.nm[q0 + tid], (w.x + w.y) + (w.z + w.w));
             }
-            ok = !group_or(!ok);
+            ok = !group_or(3, 256, !ok);
+        };
+        for (uint32_t it = 0; ok && im.tiles; ++it) {
+            switch (padded(im.nq)) {
+            case 16: work(std::integral_constant<uint32_t, 16>{}, it); break;
+            case 32: work(std::integral_constant<uint32_t, 32>{}, it); break;
+            default: work(std::integral_constant<uint32_t, 64>{}, it);
+            }
             im = following;
         }
         if (!ok && lane == 0) atomicCAS(p.err, 0, 84);
