@@ -33,7 +33,7 @@
 
 namespace {
 
-constexpr uint32_t kHd = 128, kTile = 128, kMaxQ = 64, kThreads = 352;     // 3 warps of their own, two groups of four
+constexpr uint32_t kHd = 128, kTile = 128, kMaxQ = 64, kGroups = 4, kThreads = 96 + kGroups * 128;
 constexpr uint32_t kPageBlock = kPageTokens * kHd * 2, kSlot = 2 * kPageBlock;   // K or V of a page, of a tile
 constexpr uint32_t kBox = kTile * 128;                                           // 64 dims of a tile's keys
 constexpr uint32_t kQBytes = 4 * kMaxQ * 128, kPBytes = 2 * kTile * 128;         // high and low parts
@@ -73,7 +73,8 @@ struct Bars {
     uint64_t item_ready[kItemSlots];
     Item item[kItemSlots];
     uint32_t tmem;
-    alignas(16) float c[2][kMaxQ];       // per query: score to log2
+    alignas(16) float up[2][kMaxQ];      // per query: what its scores still lack
+    uint32_t large[2];                   // an item with an `up` that is not 1
     alignas(16) float nm[kMaxQ], a[kMaxQ];           // reference, negative; factor of its last change
     alignas(16) float red[kMaxQ][4];
 };
@@ -117,12 +118,18 @@ __device__ __forceinline__ float ex2(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3_nan(float a, float b, float c)
+{
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 // H consecutive columns of this thread's TMEM lane (no wait)
 template <uint32_t H> __device__ __forceinline__ void tmem_ld(uint32_t at, float (&v)[H])
 {
-    if constexpr (H == 32) tc5::ld32(at, v);
-    else if constexpr (H == 16) tc5::ld16(at, v);
-    else tc5::ld8(at, v);
+    if constexpr (H == 16) tc5::ld16(at, v);
+    else if constexpr (H == 8) tc5::ld8(at, v);
+    else tc5::ld4(at, v);
 }
 // Largest of the warp's 32 lanes for each of H values: v[0] holds that of the value whose index is returned.
 template <uint32_t H> __device__ __forceinline__ uint32_t warp_max_many(float (&v)[H], uint32_t lane)
@@ -164,10 +171,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             mbar_init(&sm.v_free[i], 1);
         }
         for (uint32_t i = 0; i < kItemSlots; ++i) mbar_init(&sm.item_ready[i], 1);
-        mbar_init(&sm.q_full, 8);
+        mbar_init(&sm.q_full, 4 * kGroups);
         mbar_init(&sm.s_full[0], 1);
         mbar_init(&sm.s_full[1], 1);
-        mbar_init(&sm.p_full, 8);
+        mbar_init(&sm.p_full, 4 * kGroups);
         mbar_init(&sm.o_full, 1);
         mbar_init(&sm.drained, 1);
         fence_barrier_init();
@@ -302,59 +309,68 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
         if (lead) tc5::commit(&sm.drained);                      // no product is running when the TMEM is given back
         (void)mbar_wait_warp(&sm.drained, 0, limit);
     } else {
-        // a thread per key (scores) and per value dimension (output): its TMEM lane either way; each group has half of the queries
+        // a thread per key (scores) and per value dimension (output): its TMEM lane either way; each group has a share of the queries
         const uint32_t quarter = warp & 3, group = (warp - 3) >> 2, key = quarter * 32 + lane, tid = (threadIdx.x - 96) & 127;
         const uint32_t bar = 1 + group, lanes = (quarter * 32) << 16;
         uint32_t n = 0;                                          // tiles so far
         bool ok = true;
-        // The item's queries as operands: against the power of two of their row, high and low F16 parts.
+        auto all_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"n"(1 + kGroups), "n"(128 * kGroups) : "memory"); };
+        auto all_or = [&](bool x) { return group_or(1 + kGroups, 128 * kGroups, x); };
+        // The item's queries as operands: scaled so that scores are powers of two's exponents, in a high and a low F16 part.  Up to
+        // 2^15 that leaves 2^-22 of an element or 2^-25, whichever is more; rows with larger ones are brought below it by a power of two.
         auto queries = [&](const Item &im, uint32_t it) {
             const uint32_t rows = padded(im.nq);
-#pragma unroll 1
-            for (uint32_t r0 = warp - 3; r0 < rows; r0 += 32) {
-                float4 x[4];
+            float4 x[kMaxQ / (4 * kGroups)];
 #pragma unroll
-                for (uint32_t u = 0; u < 4; ++u) {
-                    const uint32_t r = r0 + 8 * u, qi = im.q0 + r;
-                    x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (r < im.nq)
-                        x[u] = __ldg(reinterpret_cast<const float4 *>(
-                                         p.q + ((size_t)(im.row0 + qi / p.per) * p.n_q + im.kvh * p.per + qi % p.per) * kHd) + lane);
-                }
+            for (uint32_t u = 0; u < kMaxQ / (4 * kGroups); ++u) {
+                const uint32_t r = warp - 3 + 4 * kGroups * u, qi = im.q0 + r;
+                x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r < im.nq)
+                    x[u] = __ldg(reinterpret_cast<const float4 *>(
+                                     p.q + ((size_t)(im.row0 + qi / p.per) * p.n_q + im.kvh * p.per + qi % p.per) * kHd) + lane);
+            }
+            if (threadIdx.x == 96) sm.large[it & 1] = 0;
+            all_sync();
 #pragma unroll
-                for (uint32_t u = 0; u < 4; ++u) {
-                    const uint32_t r = r0 + 8 * u;
-                    float top = fmaxf(fmaxf(fabsf(x[u].x), fabsf(x[u].y)), fmaxf(fabsf(x[u].z), fabsf(x[u].w)));
+            for (uint32_t u = 0; u < kMaxQ / (4 * kGroups); ++u) {
+                const uint32_t r = warp - 3 + 4 * kGroups * u;
+                if (r >= rows) continue;
+                float y[4] = {x[u].x * p.scale_log2, x[u].y * p.scale_log2, x[u].z * p.scale_log2, x[u].w * p.scale_log2}, up = 1.f;
+                const float top = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
+                if (__any_sync(0xffffffffu, top >= 32768.f)) {
+                    float most = top;
 #pragma unroll
-                    for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 126);
+                    for (int o = 16; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                    const int e = min((int)(__float_as_uint(most) >> 23) - 127, 126);
                     const float down = __int_as_float((127 - e) << 23);
-                    uint32_t hi[2], lo[2];
-                    split_half2(x[u].x * down, x[u].y * down, hi[0], lo[0]);
-                    split_half2(x[u].z * down, x[u].w * down, hi[1], lo[1]);
-                    if (r < rows) {
-                        // (rows and rows more: a multiple of 16, so the swizzle is the same)
-                        uint8_t *at = qs + (lane >> 4) * (2 * rows * 128) + r * 128 + ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
-                        *reinterpret_cast<uint2 *>(at) = make_uint2(hi[0], hi[1]);
-                        *reinterpret_cast<uint2 *>(at + rows * 128) = make_uint2(lo[0], lo[1]);
-                        if (lane == 0) sm.c[it & 1][r] = p.scale_log2 * __int_as_float((127 + e) << 23);
-                    }
+                    up = __int_as_float((127 + e) << 23);
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) y[j] *= down;
+                    if (lane == 0) sm.large[it & 1] = 1;
                 }
+                uint32_t hi[2], lo[2];
+                split_half2(y[0], y[1], hi[0], lo[0]);
+                split_half2(y[2], y[3], hi[1], lo[1]);
+                // (rows and rows more: a multiple of 16, so the swizzle is the same)
+                uint8_t *at = qs + (lane >> 4) * (2 * rows * 128) + r * 128 + ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
+                *reinterpret_cast<uint2 *>(at) = make_uint2(hi[0], hi[1]);
+                *reinterpret_cast<uint2 *>(at + rows * 128) = make_uint2(lo[0], lo[1]);
+                if (lane == 0) sm.up[it & 1][r] = up;
             }
             fence_proxy_async();
-            asm volatile("bar.sync 3, 256;" ::: "memory");       // (sm.c, for all of both groups)
+            all_sync();                                          // (sm.up, sm.large)
             if (lane == 0) mbar_arrive(&sm.q_full);
         };
         Item im = item_at(0, ok, true);
         // (a warp whose wait ran out stays with the others: they leave together, and the groups' barriers count on all of them)
-        ok = !group_or(3, 256, !ok);
+        ok = !all_or(!ok);
         if (ok && im.tiles) queries(im, 0);
         Item following{};
         auto work = [&](auto size, uint32_t it) {
-            constexpr uint32_t NQ = decltype(size)::value, H = NQ / 2;
+            constexpr uint32_t NQ = decltype(size)::value, H = NQ / kGroups;
             const uint32_t q0 = group * H;                       // this group's first query
-            const float4 *const c4 = reinterpret_cast<const float4 *>(sm.c[it & 1] + q0), *const nm4 = reinterpret_cast<const float4 *>(sm.nm + q0);
-            const float4 *const a4 = reinterpret_cast<const float4 *>(sm.a + q0);
+            const float4 *const nm4 = reinterpret_cast<const float4 *>(sm.nm + q0), *const a4 = reinterpret_cast<const float4 *>(sm.a + q0);
+            const bool large = sm.large[it & 1] != 0;
             float o[H], l[H];
 #pragma unroll
             for (uint32_t j = 0; j < H; ++j) o[j] = l[j] = 0.f;
@@ -380,42 +396,39 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                 const uint32_t at = tmem + (n & 1) * 2 * kMaxQ + lanes + q0, here = im.rows - (im.tile0 + t) * kTile;
                 const bool seen = key < here;
                 float s[H];
-                auto scores = [&]() {
+                auto scores = [&](bool infinite) {
                     float lo[H];
                     tmem_ld(at, s);
                     tmem_ld(at + NQ, lo);
                     tc5::wait_ld();
 #pragma unroll
-                    for (uint32_t j = 0; j < H; ++j) s[j] += lo[j];
+                    for (uint32_t j = 0; j < H; ++j) {
+                        // (a key with an infinity: the high part has its score, the low one may have the other sign of it or a NaN)
+                        if (infinite && fabsf(s[j]) == INFINITY) continue;
+                        s[j] += lo[j];
+                    }
+                    if (large) {
+#pragma unroll
+                        for (uint32_t j = 0; j < H; ++j) s[j] *= sm.up[it & 1][q0 + j];
+                    }
                 };
-                scores();
                 bool moved = t == 0;
                 if (!moved) {
+                    scores(false);
                     float top = -INFINITY;
 #pragma unroll
                     for (uint32_t j = 0; j < H; j += 4) {
-                        const float4 c = c4[j / 4], m = nm4[j / 4];
-                        s[j] = fmaf(s[j], c.x, m.x);
-                        s[j + 1] = fmaf(s[j + 1], c.y, m.y);
-                        s[j + 2] = fmaf(s[j + 2], c.z, m.z);
-                        s[j + 3] = fmaf(s[j + 3], c.w, m.w);
-                        top = fmaxf(fmaxf(top, fmaxf(s[j], s[j + 1])), fmaxf(s[j + 2], s[j + 3]));
+                        const float4 m = nm4[j / 4];
+                        s[j] += m.x; s[j + 1] += m.y; s[j + 2] += m.z; s[j + 3] += m.w;
+                        top = max3_nan(max3_nan(top, s[j], s[j + 1]), s[j + 2], s[j + 3]);
                     }
-                    moved = group_or(bar, 128, seen && top > kGrow);
-                    if (moved) scores();
+                    moved = group_or(bar, 128, seen && !(top <= kGrow));         // (or not a number)
                 }
                 if (moved) {                                     // (the same in all threads of the group)
-#pragma unroll
-                    for (uint32_t j = 0; j < H; j += 4) {
-                        const float4 c = c4[j / 4];
-                        s[j] = seen ? s[j] * c.x : WR_NEG_SENTINEL;
-                        s[j + 1] = seen ? s[j + 1] * c.y : WR_NEG_SENTINEL;
-                        s[j + 2] = seen ? s[j + 2] * c.z : WR_NEG_SENTINEL;
-                        s[j + 3] = seen ? s[j + 3] * c.w : WR_NEG_SENTINEL;
-                    }
+                    scores(true);
                     float v[H];
 #pragma unroll
-                    for (uint32_t j = 0; j < H; ++j) v[j] = s[j];
+                    for (uint32_t j = 0; j < H; ++j) v[j] = s[j] = seen ? s[j] : WR_NEG_SENTINEL;
                     const uint32_t idx = warp_max_many<H>(v, lane);
                     sm.red[q0 + idx][quarter] = v[0];            // (lanes that share an index hold one value)
                     group_sync(bar);
@@ -437,24 +450,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                 // the tile before has been multiplied: P is free, its O^T is there
                 if (ok && n > 0) ok = mbar_wait_warp(&sm.o_full, (n - 1) & 1, limit);
                 tc5::fence_after();
+                constexpr uint32_t V = H < 8 ? H : 8;            // queries to a store
 #pragma unroll
-                for (uint32_t j = 0; j < H; j += 8) {
-                    uint32_t hi[4], lo[4];
+                for (uint32_t j = 0; j < H; j += V) {
+                    uint32_t hi[V / 2], lo[V / 2];
 #pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e) {
+                    for (uint32_t e = 0; e < V / 2; ++e) {
                         const float w0 = seen ? ex2(s[j + 2 * e]) : 0.f, w1 = seen ? ex2(s[j + 2 * e + 1]) : 0.f;
                         l[j + 2 * e] += w0;
                         l[j + 2 * e + 1] += w1;
                         split_half2(w0, w1, hi[e], lo[e]);
                     }
                     // a key's row: the high parts of up to 64 queries, the low ones behind them or in rows of their own
-                    const uint32_t c = (q0 + j) >> 3;
-                    uint8_t *const row = ps + key * 128;
-                    *reinterpret_cast<uint4 *>(row + ((c ^ (key & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if constexpr (NQ == 64)
-                        *reinterpret_cast<uint4 *>(row + kTile * 128 + ((c ^ (key & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    else
-                        *reinterpret_cast<uint4 *>(row + (((c + NQ / 8) ^ (key & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    auto put = [&](uint32_t at, const uint32_t (&x)[V / 2]) {
+                        uint8_t *to = ps + key * 128 + (at >> 7) * (kTile * 128) + ((((at >> 4) & 7) ^ (key & 7)) << 4) + (at & 15);
+                        if constexpr (V == 8) *reinterpret_cast<uint4 *>(to) = make_uint4(x[0], x[1], x[2], x[3]);
+                        else *reinterpret_cast<uint2 *>(to) = make_uint2(x[0], x[1]);
+                    };
+                    put(2 * (q0 + j), hi);
+                    put(2 * (q0 + j + NQ), lo);
                 }
                 if (here < kTile && group == 0) {
                     // rows behind the last one may hold anything, and a weight of zero does not take a NaN out
@@ -476,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             // the next item's queries (the last scores have been read), then this one's results
             bool more = true;
             following = item_at(it + 1, more, true);
-            ok = !group_or(3, 256, !(ok && more));
+            ok = !all_or(!(ok && more));
             if (ok && following.tiles) queries(following, it + 1);
             if (ok) ok = mbar_wait_warp(&sm.o_full, (n - 1) & 1, limit);
             tc5::fence_after();
@@ -492,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                 const float4 w = *reinterpret_cast<const float4 *>(sm.red[q0 + tid]);
                 p.ml[im.part + q0 + tid] = make_float2(-sm.nm[q0 + tid], (w.x + w.y) + (w.z + w.w));
             }
-            ok = !group_or(3, 256, !ok);
+            ok = !all_or(!ok);
         };
         for (uint32_t it = 0; ok && im.tiles; ++it) {
             switch (padded(im.nq)) {
