@@ -39,7 +39,7 @@ constexpr uint32_t kBox = kTile * 128;                                          
 constexpr uint32_t kQBytes = 4 * kMaxQ * 128, kPBytes = 2 * kTile * 128;         // high and low parts
 constexpr uint32_t kKSlots = 2, kVSlots = 3, kItemSlots = 8;
 constexpr uint32_t kTmemCols = 512, kTmemO = 256;                                // two buffers of 128 columns each
-constexpr uint32_t kMaxSegs = 2 * WR_CUDA_BATCH_MAX, kMaxParts = 1024;
+constexpr uint32_t kMaxSegs = 2 * WR_CUDA_BATCH_MAX;
 constexpr float kGrow = 8.0f, kLog2e = 1.4426950408889634f;
 
 struct Segment {
@@ -524,19 +524,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
     if (warp == 1) tc5::dealloc(tmem, kTmemCols);
 }
 
-// The chunks of a row added up: those of its group's shared rows, then those of its own.
+// The chunks of a row added up: those of its group's shared rows, then those of its own.  Warp w has chunks w, w + 4, ...: the loads of
+// up to 32 chunks are one round trip, which bounds it (two: maxima and sums first, 2.5 us longer).
+constexpr uint32_t kMergeAhead = 8;
 __global__ void __launch_bounds__(kHd) shared_merge_kernel(const __grid_constant__ SharedParams p)
 {
-    __shared__ float w[kMaxParts];
-    __shared__ float sum;
+    __shared__ float4 sums[3][32];
     pdl_wait();
     pdl_trigger();
-    const uint32_t head = blockIdx.x, s = blockIdx.y, kvh = head / p.per, lane = threadIdx.x & 31;
+    const uint32_t head = blockIdx.x, s = blockIdx.y, kvh = head / p.per, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t first[2], step[2], count[2];
 #pragma unroll
     for (uint32_t i = 0; i < 2; ++i) {
         const uint32_t at = i ? p.own_seg[s] : p.group_seg[s];
-        count[i] = 0;
+        count[i] = first[i] = step[i] = 0;
         if (at >= kMaxSegs) continue;
         const Segment &g = p.seg[at];
         count[i] = g.chunks;
@@ -545,28 +546,55 @@ __global__ void __launch_bounds__(kHd) shared_merge_kernel(const __grid_constant
     }
     const uint32_t n = count[0] + count[1];
     auto part = [&](uint32_t i) { return i < count[0] ? first[0] + i * step[0] : first[1] + (i - count[0]) * step[1]; };
-    if (threadIdx.x < 32) {
-        float top = WR_NEG_SENTINEL;
-        for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, p.ml[part(i)].x);
+    float4 o[kMergeAhead];
+    float m[kMergeAhead];
+    auto load = [&](uint32_t i0) {
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        float l = 0.f;
-        for (uint32_t i = lane; i < n; i += 32) {
-            const float2 ml = p.ml[part(i)];
-            const float f = ex2(ml.x - top);
-            w[i] = f;
-            l += f * ml.y;
+        for (uint32_t u = 0; u < kMergeAhead; ++u) {
+            const uint32_t i = i0 + 4 * u;
+            if (i >= n) continue;
+            o[u] = *reinterpret_cast<const float4 *>(p.o + (size_t)part(i) * kHd + 4 * lane);
+            m[u] = p.ml[part(i)].x;
         }
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (lane == 0) sum = l;
+    };
+    load(warp);
+    float top = WR_NEG_SENTINEL, l = 0.f;
+    for (uint32_t i = lane; i < n; i += 32) {
+        const float2 ml = p.ml[part(i)];
+        const float t = fmaxf(top, ml.x);
+        l = l * ex2(top - t) + ml.y * ex2(ml.x - t);
+        top = t;
     }
+    const float mine = top;
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    l *= ex2(mine - top);
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t i0 = warp;; load(i0)) {
+#pragma unroll
+        for (uint32_t u = 0; u < kMergeAhead; ++u) {
+            if (i0 + 4 * u >= n) continue;
+            const float w = ex2(m[u] - top);
+            acc.x = fmaf(w, o[u].x, acc.x); acc.y = fmaf(w, o[u].y, acc.y);
+            acc.z = fmaf(w, o[u].z, acc.z); acc.w = fmaf(w, o[u].w, acc.w);
+        }
+        i0 += 4 * kMergeAhead;
+        if (i0 >= n) break;
+    }
+    if (warp) sums[warp - 1][lane] = acc;
     __syncthreads();
-    float acc = 0.f;
-#pragma unroll 8
-    for (uint32_t i = 0; i < n; ++i) acc = fmaf(w[i], p.o[(size_t)part(i) * kHd + threadIdx.x], acc);
+    if (warp) return;
+#pragma unroll
+    for (uint32_t w = 0; w < 3; ++w) {
+        const float4 x = sums[w][lane];
+        acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+    }
     // (a row of which no key counts, all scores -inf, is zeros)
-    p.out[((size_t)s * p.n_q + head) * kHd + threadIdx.x] = sum == 0.f ? 0.f : acc / sum;
+    if (l == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    else acc = make_float4(acc.x / l, acc.y / l, acc.z / l, acc.w / l);
+    *reinterpret_cast<float4 *>(p.out + ((size_t)s * p.n_q + head) * kHd + 4 * lane) = acc;
 }
 
 }  // namespace
