@@ -209,6 +209,12 @@ def test_nan_and_infinite_rows_stay_with_their_sessions(ctx):
     got = call(ctx, [f], q, 8)
     assert np.isnan(got[1, 4:]).all() and np.isfinite(got[1, :4]).all()
     assert np.array_equal(got[[0, 2]], want[[0, 2]])
+    f.kvs[1].write_rows(0, 0, 256 + 3, f.k[1][256 + 3:256 + 4])
+    row[0, 0, 9], row[0, 1, 7] = 0x7C00, 0x3C00                      # an infinite value of session 1, kv head 0
+    f.kvs[1].write_rows(0, 1, 256 + 3, row)
+    got = call(ctx, [f], q, 8)
+    assert np.isposinf(got[1, :4, 9]).all() and np.isfinite(np.delete(got[1, :4], 9, axis=1)).all()
+    assert np.array_equal(got[[0, 2]], want[[0, 2]])
     f.close()
 
 

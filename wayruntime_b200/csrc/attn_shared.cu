@@ -7,16 +7,19 @@
 // (m_i the largest score of a part, in powers of two, l_i and o_i its sums against it), so the shared part is worked out once
 // for all queries of the group: a page is fetched from HBM once for up to 64 of them.
 //
-// A SEGMENT is a run of keys with the queries that attend it: per kv head the queries of all sessions of a group (shared
-// rows), or of one session (its own rows).  A segment is cut into chunks; a WORK ITEM is (segment, chunk, kv head, 64 of its
-// queries).  Persistent CTAs, one per SM, draw items from a counter, longest first; shared_merge_kernel adds the chunks
-// of a row up in order, so results do not hang on who worked what out.  Operands are swapped, as in attn_latent.cu: keys
-// (128, two pages) are the tensor core's M, queries its N, so a tile costs what its queries cost.  Per tile
+// A BUNDLE is up to 64 queries of one kv head: some sessions of a group, with the query heads that share the kv head.  Its keys
+// are a list of tiles of 128 (two pages): the group's shared rows, then each session's own.  The queries stay where they are for
+// the whole list; in a session's own tiles the other sessions' columns get weights of zero.  (Work items of their own for own
+// rows took 3 to 4 us each for a tile or two: 20.7 us for four groups of four behind 4096 rows, 36.0 for 16 sessions behind
+// 32768; with one list 16.8 and 30.6.)  A WORK ITEM is an even share of a bundle's tiles for one kv head.  Persistent CTAs, one per SM,
+// draw items from a counter, longest first; when none is left they add the shares of a row up in order (add_up), so results do
+// not hang on who worked what out.  Operands are swapped, as in attn_latent.cu: keys are the tensor core's M, queries
+// its N, so a tile costs what its queries cost.  Per tile
 //   * two loading warps bring K and V in with linear bulk copies (a page's blocks are the operand's layout);
 //   * one warp issues S^T[key][query] = K . Q^T and O^T[dim][query] = V^T . P^T; the scores of the next tile are issued
 //     before this tile's values, so both buffers of S are in use;
-//   * four warps, a thread per key: exponentials against a running reference, P^T to shared memory (queries contiguous:
-//     the MN-major operand, a thread writes 16 bytes at a time); then, a thread per value dimension, the tile's O^T is added
+//   * four groups of four warps, each with a quarter of the queries, a thread per key: exponentials against a running reference,
+//     P^T to shared memory (queries contiguous: the MN-major operand); then, a thread per value dimension, the tile's O^T is added
 //     to sums in registers.  The reference moves when a score is more than 2^8 above it: the threads vote, and only then
 //     is the maximum over keys worked out (a segment's first tile always does).
 // Queries and probabilities are split in two F16 numbers (22 bits; queries against a power of two of their row), two
@@ -36,40 +39,70 @@ namespace {
 constexpr uint32_t kHd = 128, kTile = 128, kMaxQ = 64, kGroups = 4, kThreads = 96 + kGroups * 128;
 constexpr uint32_t kPageBlock = kPageTokens * kHd * 2, kSlot = 2 * kPageBlock;   // K or V of a page, of a tile
 constexpr uint32_t kBox = kTile * 128;                                           // 64 dims of a tile's keys
-constexpr uint32_t kQBytes = 4 * kMaxQ * 128, kPBytes = 2 * kTile * 128;         // high and low parts
-constexpr uint32_t kKSlots = 2, kVSlots = 3, kItemSlots = 8;
+constexpr uint32_t kQBytes = 4 * kMaxQ * 128;                                    // high and low parts
+constexpr uint32_t kKSlots = 2, kMaxVSlots = 3, kItemSlots = 8;
 constexpr uint32_t kTmemCols = 512, kTmemO = 256;                                // two buffers of 128 columns each
-constexpr uint32_t kMaxSegs = 2 * WR_CUDA_BATCH_MAX;
+constexpr uint32_t kMaxBundles = 64;
 constexpr float kGrow = 8.0f, kLog2e = 1.4426950408889634f;
 
-struct Segment {
-    const uint64_t *pages;               // page table from the segment's first page on
-    uint32_t rows;                       // keys
-    uint32_t row0, queries;              // first session; queries per kv head
-    uint32_t chunks, qtiles, item0, part0;
+struct Bundle {
+    uint32_t group, row0, sessions;      // its group; its first session, how many
+    uint32_t head0, heads;               // which of a kv head's query heads
+    uint32_t tiles, chunks, item0, part0;
 };
 struct SharedParams {
-    Segment seg[kMaxSegs];
-    uint8_t group_seg[WR_CUDA_BATCH_MAX], own_seg[WR_CUDA_BATCH_MAX];            // of a session; kMaxSegs: none
-    uint32_t n_segs, items, n_q, n_kv, per;                                      // per: query heads to a kv head
+    Bundle bundle[kMaxBundles];
+    const uint64_t *shared_pages[WR_CUDA_BATCH_MAX], *own_pages[WR_CUDA_BATCH_MAX];      // of a group; of a session, from its own rows on
+    uint32_t shared_rows[WR_CUDA_BATCH_MAX], own_rows[WR_CUDA_BATCH_MAX];
+    uint8_t first_bundle[WR_CUDA_BATCH_MAX];     // of a session; the next ones have its further heads
+    uint32_t n_bundles, items, rows, n_q, n_kv, per;     // rows: of the result; per: query heads to a kv head
     const float *q;
     float *out;
     float2 *ml;                          // [part]: reference (log2), sum
     float *o;                            // [part][128]
     int *sched;                          // next item, CTAs that have left
+    int *done;                           // [bundle][kv head]: parts that are there, then rows that have been added up
+    uint32_t team;                       // warps that add up a row
+    uint32_t widest;                     // most queries of a bundle
     float scale_log2;
     long long wait_limit;
     int *err;
 };
 struct Item {
-    const uint64_t *pages;
-    uint32_t tiles, tile0, rows;         // tiles 0: no more work
-    uint32_t row0, kvh, q0, nq;
-    uint32_t part;
+    uint32_t tiles, tile0;               // tiles 0: no more work
+    uint32_t bundle, kvh, nq, part;
 };
+// Where a role is in a bundle's list: segment 0 is the shared rows, 1 + i the i-th session's own.
+struct Place {
+    uint32_t segment, tile;
+};
+__device__ __forceinline__ uint32_t rows_of(const SharedParams &p, const Bundle &b, uint32_t segment)
+{
+    return segment ? p.own_rows[b.row0 + segment - 1] : p.shared_rows[b.group];
+}
+__device__ __forceinline__ Place place_at(const SharedParams &p, const Bundle &b, uint32_t tile)
+{
+    Place at = {0, tile};
+    for (uint32_t n; at.segment < b.sessions && at.tile >= (n = (rows_of(p, b, at.segment) + kTile - 1) / kTile); ++at.segment) at.tile -= n;
+    return at;
+}
+__device__ __forceinline__ void step(const SharedParams &p, const Bundle &b, Place &at)
+{
+    ++at.tile;
+    while (at.segment < b.sessions && at.tile * kTile >= rows_of(p, b, at.segment)) {
+        at.tile = 0;
+        ++at.segment;
+    }
+}
+// the tile's pages of one layer: the first one's address in the table, and whether there is a second
+__device__ __forceinline__ const uint64_t *pages_of(const SharedParams &p, const Bundle &b, const Place &at, bool &two)
+{
+    two = rows_of(p, b, at.segment) > at.tile * kTile + kPageTokens;
+    return (at.segment ? p.own_pages[b.row0 + at.segment - 1] : p.shared_pages[b.group]) + 2 * at.tile;
+}
 struct Bars {
-    uint64_t k_full[kKSlots], k_free[kKSlots], v_full[kVSlots], v_free[kVSlots];
-    uint64_t q_full, s_full[2], p_full, o_full, drained;
+    uint64_t k_full[kKSlots], k_free[kKSlots], v_full[kMaxVSlots], v_free[kMaxVSlots];
+    uint64_t q_full, s_full[2], p_full[2], o_full[2], drained;
     uint64_t item_ready[kItemSlots];
     Item item[kItemSlots];
     uint32_t tmem;
@@ -78,28 +111,26 @@ struct Bars {
     alignas(16) float nm[kMaxQ], a[kMaxQ];           // reference, negative; factor of its last change
     alignas(16) float red[kMaxQ][4];
 };
-constexpr uint32_t kSmem = kKSlots * kSlot + kVSlots * kSlot + kQBytes + kPBytes + (uint32_t)sizeof(Bars);
+// two buffers of P: high and low parts in one row of 128 bytes, or (more than 32 queries) in two
+__host__ __device__ constexpr uint32_t p_bytes(uint32_t queries) { return queries > 32 ? 2 * kTile * 128 : kTile * 128; }
+__host__ __device__ constexpr uint32_t v_slots(uint32_t queries) { return queries > 32 ? 2 : 3; }
+constexpr uint32_t kSmem = kKSlots * kSlot + 2 * kSlot + kQBytes + 2 * p_bytes(64) + (uint32_t)sizeof(Bars);
+static_assert(v_slots(32) * kSlot + 2 * p_bytes(32) == v_slots(64) * kSlot + 2 * p_bytes(64), "");
 static_assert(kSmem <= 232448, "the CTA's shared memory is 227 KB at most");
 
 __device__ __forceinline__ Item item_of(const SharedParams &p, uint32_t i)
 {
     Item it{};
     if (i >= p.items) return it;
-    uint32_t s = 0;
-    while (s + 1 < p.n_segs && i >= p.seg[s + 1].item0) ++s;
-    const Segment &g = p.seg[s];
-    i -= g.item0;
+    while (it.bundle + 1 < p.n_bundles && i >= p.bundle[it.bundle + 1].item0) ++it.bundle;
+    const Bundle &b = p.bundle[it.bundle];
+    i -= b.item0;
     it.kvh = i % p.n_kv;
     i /= p.n_kv;
-    it.q0 = i % g.qtiles * kMaxQ;
-    const uint32_t chunk = i / g.qtiles, tiles = (g.rows + kTile - 1) / kTile;
-    it.tile0 = tiles * chunk / g.chunks;
-    it.tiles = tiles * (chunk + 1) / g.chunks - it.tile0;
-    it.pages = g.pages;
-    it.rows = g.rows;
-    it.row0 = g.row0;
-    it.nq = min(g.queries - it.q0, kMaxQ);
-    it.part = g.part0 + (chunk * p.n_kv + it.kvh) * g.queries + it.q0;
+    it.tile0 = b.tiles * i / b.chunks;
+    it.tiles = b.tiles * (i + 1) / b.chunks - it.tile0;
+    it.nq = b.sessions * b.heads;
+    it.part = b.part0 + (i * p.n_kv + it.kvh) * it.nq;
     return it;
 }
 // The queries of an item, rounded up to what a group of threads has at its fixed sizes: half of them each.
@@ -123,6 +154,14 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c)
     float d;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
+}
+__device__ __forceinline__ void all_sync() { asm volatile("bar.sync %0, %1;" ::"n"(1 + kGroups), "n"(128 * kGroups) : "memory"); }
+__device__ __forceinline__ bool all_or(bool x) { return group_or(1 + kGroups, 128 * kGroups, x); }
+// two F32 additions in one issue slot
+__device__ __forceinline__ void add2(float &a, float &b, float x, float y)
+{
+    asm("{\n\t.reg .b64 s, t;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 t, {%2, %3};\n\tadd.rn.f32x2 s, s, t;\n\tmov.b64 {%0, %1}, s;\n\t}"
+        : "+f"(a), "+f"(b) : "f"(x), "f"(y));
 }
 // H consecutive columns of this thread's TMEM lane (no wait)
 template <uint32_t H> __device__ __forceinline__ void tmem_ld(uint32_t at, float (&v)[H])
@@ -155,18 +194,109 @@ template <uint32_t H> __device__ __forceinline__ uint32_t warp_max_many(float (&
 // kind::f16, F16 x F16 -> F32: V^T (its dims contiguous) times P^T (its queries contiguous)
 __device__ __forceinline__ uint32_t idesc_values(uint32_t n) { return tc5::idesc_f16(128, n) | tc5::kIdescAMnMajor | (1u << 16); }
 
+// The parts of a row added up, in order.  The CTAs do this when there is
+// no item left to draw; a team of warps takes a row, waits for its parts (bounded), and has up to 8 x team of them under way at once.
+// (A kernel of its own behind this one: 2 to 3 us more, and the host's time for a launch.)
+constexpr uint32_t kMergeAhead = 8, kMergeWarps = 4 * kGroups;
+__device__ __forceinline__ bool add_up(const SharedParams &p, float4 *sums, uint32_t warp, uint32_t lane)
+{
+    const uint32_t team = p.team, teams = kMergeWarps / team, sub = warp % team;
+    bool ok = true;
+    for (uint32_t j = blockIdx.x; j * teams < p.rows; j += gridDim.x) {
+        const uint32_t row = j * teams + warp / team;
+        const bool mine = row < p.rows;
+        const uint32_t s = mine ? row / p.n_q : 0, head = mine ? row % p.n_q : 0, kvh = head / p.per;
+        const uint32_t which = p.first_bundle[s] + head % p.per / kMaxQ;
+        const Bundle &b = p.bundle[which];
+        const uint32_t nq = b.sessions * b.heads, stride = p.n_kv * nq;
+        const uint32_t first = b.part0 + kvh * nq + (s - b.row0) * b.heads + head % p.per - b.head0;
+        int *const done = p.done + which * p.n_kv + kvh;
+        uint32_t n = mine && ok ? b.chunks : 0;
+        if (n && sub == 0) {                                     // (few ask: thousands of warps at these words held up what they wait for)
+            long long t0 = 0;
+            for (bool again = false;; again = true) {
+                int there;
+                asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(there) : "l"(done) : "memory");
+                if (__all_sync(0xffffffffu, (uint32_t)there >= n)) break;
+                if (!again) t0 = clock64();
+                else if (__any_sync(0xffffffffu, clock64() - t0 > p.wait_limit)) {
+                    ok = false;
+                    break;
+                }
+            }
+        }
+        ok = !all_or(!ok);
+        if (!ok) n = 0;
+        auto part = [&](uint32_t i) { return first + i * stride; };
+        float4 o[kMergeAhead], acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float m[kMergeAhead], top = WR_NEG_SENTINEL, l = 0.f;
+        auto load = [&](uint32_t i0) {
+#pragma unroll
+            for (uint32_t u = 0; u < kMergeAhead; ++u) {
+                const uint32_t i = i0 + u * team;
+                if (i >= n) continue;
+                o[u] = __ldcg(reinterpret_cast<const float4 *>(p.o + (size_t)part(i) * kHd) + lane);
+                m[u] = __ldcg(&p.ml[part(i)].x);
+            }
+        };
+        load(sub);
+        for (uint32_t i = lane; i < n; i += 32) {
+            const float2 ml = __ldcg(p.ml + part(i));
+            const float t = fmaxf(top, ml.x);
+            l = l * ex2(top - t) + ml.y * ex2(ml.x - t);
+            top = t;
+        }
+        const float before = top;
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        l *= ex2(before - top);
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+        for (uint32_t i0 = sub; i0 < n;) {
+#pragma unroll
+            for (uint32_t u = 0; u < kMergeAhead; ++u) {
+                if (i0 + u * team >= n) continue;
+                const float w = ex2(m[u] - top);
+                acc.x = fmaf(w, o[u].x, acc.x); acc.y = fmaf(w, o[u].y, acc.y);
+                acc.z = fmaf(w, o[u].z, acc.z); acc.w = fmaf(w, o[u].w, acc.w);
+            }
+            i0 += kMergeAhead * team;
+            load(i0);
+        }
+        if (team > 1) {
+            sums[warp * 32 + lane] = acc;
+            all_sync();
+            for (uint32_t w = 1; w < team && sub == 0; ++w) {
+                const float4 x = sums[(warp + w) * 32 + lane];
+                acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+            }
+        }
+        if (sub == 0 && n && ok) {
+            // (a row of which no key counts, all scores -inf, is zeros)
+            if (l == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            else acc = make_float4(acc.x / l, acc.y / l, acc.z / l, acc.w / l);
+            *(reinterpret_cast<float4 *>(p.out + (size_t)row * kHd) + lane) = acc;
+            // the last row leaves the counter as it was
+            if (lane == 0 && atomicAdd(done, 1) == (int)(n + nq) - 1) *done = 0;
+        }
+        if (team > 1) all_sync();
+    }
+    return ok;
+}
+
 __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_constant__ SharedParams p)
 {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t *const ks = smem_raw, *const vs = ks + kKSlots * kSlot, *const qs = vs + kVSlots * kSlot, *const ps = qs + kQBytes;
-    Bars &sm = *reinterpret_cast<Bars *>(ps + kPBytes);
+    const uint32_t v_ring = v_slots(p.widest), p_size = p_bytes(p.widest);
+    uint8_t *const ks = smem_raw, *const qs = ks + kKSlots * kSlot, *const vs = qs + kQBytes, *const ps = vs + v_ring * kSlot;
+    Bars &sm = *reinterpret_cast<Bars *>(ps + 2 * p_size);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kKSlots; ++i) {
             mbar_init(&sm.k_full[i], 1);
             mbar_init(&sm.k_free[i], 1);
         }
-        for (uint32_t i = 0; i < kVSlots; ++i) {
+        for (uint32_t i = 0; i < kMaxVSlots; ++i) {
             mbar_init(&sm.v_full[i], 1);
             mbar_init(&sm.v_free[i], 1);
         }
@@ -174,8 +304,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
         mbar_init(&sm.q_full, 4 * kGroups);
         mbar_init(&sm.s_full[0], 1);
         mbar_init(&sm.s_full[1], 1);
-        mbar_init(&sm.p_full, 4 * kGroups);
-        mbar_init(&sm.o_full, 1);
+        mbar_init(&sm.p_full[0], 4 * kGroups);
+        mbar_init(&sm.p_full[1], 4 * kGroups);
+        mbar_init(&sm.o_full[0], 1);
+        mbar_init(&sm.o_full[1], 1);
         mbar_init(&sm.drained, 1);
         fence_barrier_init();
     }
@@ -187,8 +319,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
     pdl_trigger();                       // (only now: what starts early behind this may rely on everything before it)
     const uint32_t tmem = sm.tmem;
     const long long limit = p.wait_limit;
-    // Item number `it` of this CTA; the loading warp is at most four items ahead of the slowest reader.
+    // Item number `it` of this CTA (the first is its own number); the loading warp is at most four items ahead of the slowest reader.
     auto item_at = [&](uint32_t it, bool &ok, bool whole_warp) -> Item {
+        if (it == 0) return item_of(p, blockIdx.x);
         uint64_t *bar = &sm.item_ready[it % kItemSlots];
         const uint32_t parity = (it / kItemSlots) & 1;
         ok = whole_warp ? mbar_wait_warp(bar, parity, limit) : mbar_wait(bar, parity, limit);
@@ -203,13 +336,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             for (uint32_t it = 0; ok; ++it) {
                 const Item im = item_of(p, next);
                 sm.item[it % kItemSlots] = im;
-                mbar_arrive(&sm.item_ready[it % kItemSlots]);
+                mbar_arrive(&sm.item_ready[it % kItemSlots]);     // (the first one's for the phases' sake)
                 if (!im.tiles) break;
-                for (uint32_t t = 0; t < im.tiles; ++t, ++n) {
-                    const uint32_t st = n % kKSlots, pg = 2 * (im.tile0 + t);
-                    const uint32_t pages = im.rows > (pg + 1) * kPageTokens ? 2u : 1u;
-                    const char *src[2] = {reinterpret_cast<const char *>(im.pages[pg]), nullptr};
-                    if (pages > 1) src[1] = reinterpret_cast<const char *>(im.pages[pg + 1]);
+                const Bundle &bd = p.bundle[im.bundle];
+                Place at = place_at(p, bd, im.tile0);
+                for (uint32_t t = 0; t < im.tiles; ++t, ++n, step(p, bd, at)) {
+                    const uint32_t st = n % kKSlots;
+                    bool two;
+                    const uint64_t *table = pages_of(p, bd, at, two);
+                    const uint32_t pages = two ? 2u : 1u;
+                    const char *src[2] = {reinterpret_cast<const char *>(table[0]), nullptr};
+                    if (two) src[1] = reinterpret_cast<const char *>(table[1]);
                     if (n >= kKSlots && !mbar_wait(&sm.k_free[st], (n / kKSlots - 1) & 1, limit)) {
                         ok = false;
                         break;
@@ -239,12 +376,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             for (uint32_t it = 0; ok; ++it) {
                 const Item im = item_at(it, ok, false);
                 if (!im.tiles) break;
-                for (uint32_t t = 0; t < im.tiles; ++t, ++n) {
-                    const uint32_t st = n % kVSlots, pg = 2 * (im.tile0 + t);
-                    const uint32_t pages = im.rows > (pg + 1) * kPageTokens ? 2u : 1u;
-                    const char *src[2] = {reinterpret_cast<const char *>(im.pages[pg]), nullptr};
-                    if (pages > 1) src[1] = reinterpret_cast<const char *>(im.pages[pg + 1]);
-                    if (n >= kVSlots && !mbar_wait(&sm.v_free[st], (n / kVSlots - 1) & 1, limit)) {
+                const Bundle &bd = p.bundle[im.bundle];
+                Place at = place_at(p, bd, im.tile0);
+                for (uint32_t t = 0; t < im.tiles; ++t, ++n, step(p, bd, at)) {
+                    const uint32_t st = n % v_ring;
+                    bool two;
+                    const uint64_t *table = pages_of(p, bd, at, two);
+                    const uint32_t pages = two ? 2u : 1u;
+                    const char *src[2] = {reinterpret_cast<const char *>(table[0]), nullptr};
+                    if (two) src[1] = reinterpret_cast<const char *>(table[1]);
+                    if (n >= v_ring && !mbar_wait(&sm.v_free[st], (n / v_ring - 1) & 1, limit)) {
                         ok = false;
                         break;
                     }
@@ -254,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                 }
             }
             if (!ok) atomicCAS(p.err, 0, 82);
-            for (uint32_t i = n - min(n, kVSlots); i < n; ++i) (void)mbar_wait(&sm.v_full[i % kVSlots], (i / kVSlots) & 1, limit);
+            for (uint32_t i = n - min(n, v_ring); i < n; ++i) (void)mbar_wait(&sm.v_full[i % v_ring], (i / v_ring) & 1, limit);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -282,24 +423,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             const Item im = item_at(it, ok, true);
             if (!im.tiles) break;
             const uint32_t n = 2 * padded(im.nq);
+            const Bundle &bd = p.bundle[im.bundle];
+            Place at = place_at(p, bd, im.tile0);
             ok = mbar_wait_warp(&sm.q_full, it & 1, limit) && score(n);
-            for (uint32_t t = 0; t < im.tiles && ok; ++t) {
-                // (the scores two tiles ago have been read: their P has been waited for)
+            for (uint32_t t = 0; t < im.tiles && ok; ++t, step(p, bd, at)) {
+                // (the scores two tiles ago have been read: their P has been waited for.  Issued behind the values of the tile before:
+                // whoever sees these scores knows those to be there.)
                 if (t + 1 < im.tiles) ok = score(n);
-                ok = ok && mbar_wait_warp(&sm.p_full, n_o & 1, limit);
-                const uint32_t st = n_o % kVSlots;
-                ok = ok && mbar_wait_warp(&sm.v_full[st], (n_o / kVSlots) & 1, limit);
+                ok = ok && mbar_wait_warp(&sm.p_full[n_o & 1], (n_o >> 1) & 1, limit);
+                const uint32_t st = n_o % v_ring;
+                ok = ok && mbar_wait_warp(&sm.v_full[st], (n_o / v_ring) & 1, limit);
                 if (!ok) break;
                 tc5::fence_after();
-                const uint32_t d = tmem + kTmemO + (n_o & 1) * 2 * kMaxQ, idesc = idesc_values(n);
-                const uint64_t a = tc5::desc_mnmajor(v_addr + st * kSlot, 8192), b = tc5::desc_mnmajor(p_addr, kTile * 128);
+                const uint32_t d = tmem + kTmemO + (n_o & 1) * 2 * kMaxQ, idesc = idesc_values(n), here = rows_of(p, bd, at.segment) - at.tile * kTile;
+                const uint64_t a = tc5::desc_mnmajor(v_addr + st * kSlot, 8192), b = tc5::desc_mnmajor(p_addr + (n_o & 1) * p_size, kTile * 128);
 #pragma unroll
-                for (uint32_t kk = 0; kk < 8; ++kk)              // 16 keys a step
-                    if (lead)
+                for (uint32_t kk = 0; kk < 8; ++kk)              // 16 keys a step, as far as there are any
+                    if (lead && 16 * kk < here)
                         tc5::mma_ss(d, a + (kk >> 2) * (kPageBlock >> 4) + (kk & 3) * (2048 >> 4), b + kk * (2048 >> 4), idesc, kk != 0);
                 if (lead) {
                     tc5::commit(&sm.v_free[st]);
-                    tc5::commit(&sm.o_full);
+                    tc5::commit(&sm.o_full[n_o & 1]);
                 }
                 ++n_o;
             }
@@ -314,20 +458,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
         const uint32_t bar = 1 + group, lanes = (quarter * 32) << 16;
         uint32_t n = 0;                                          // tiles so far
         bool ok = true;
-        auto all_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"n"(1 + kGroups), "n"(128 * kGroups) : "memory"); };
-        auto all_or = [&](bool x) { return group_or(1 + kGroups, 128 * kGroups, x); };
         // The item's queries as operands: scaled so that scores are powers of two's exponents, in a high and a low F16 part.  Up to
         // 2^15 that leaves 2^-22 of an element or 2^-25, whichever is more; rows with larger ones are brought below it by a power of two.
         auto queries = [&](const Item &im, uint32_t it) {
             const uint32_t rows = padded(im.nq);
+            const Bundle &bd = p.bundle[im.bundle];
             float4 x[kMaxQ / (4 * kGroups)];
 #pragma unroll
             for (uint32_t u = 0; u < kMaxQ / (4 * kGroups); ++u) {
-                const uint32_t r = warp - 3 + 4 * kGroups * u, qi = im.q0 + r;
+                const uint32_t r = warp - 3 + 4 * kGroups * u;
                 x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (r < im.nq)
                     x[u] = __ldg(reinterpret_cast<const float4 *>(
-                                     p.q + ((size_t)(im.row0 + qi / p.per) * p.n_q + im.kvh * p.per + qi % p.per) * kHd) + lane);
+                                     p.q + ((size_t)(bd.row0 + r / bd.heads) * p.n_q + im.kvh * p.per + bd.head0 + r % bd.heads) * kHd) + lane);
             }
             if (threadIdx.x == 96) sm.large[it & 1] = 0;
             all_sync();
@@ -367,22 +510,38 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
         if (ok && im.tiles) queries(im, 0);
         Item following{};
         auto work = [&](auto size, uint32_t it) {
-            constexpr uint32_t NQ = decltype(size)::value, H = NQ / kGroups;
+            constexpr uint32_t NQ = decltype(size)::value, H = NQ / kGroups, V = H < 8 ? H : 8;     // V: queries to a store
             const uint32_t q0 = group * H;                       // this group's first query
             const float4 *const nm4 = reinterpret_cast<const float4 *>(sm.nm + q0), *const a4 = reinterpret_cast<const float4 *>(sm.a + q0);
             const bool large = sm.large[it & 1] != 0;
+            const Bundle &bd = p.bundle[im.bundle];
+            bool fresh = true, moved = false;                    // no tile of these queries yet; the last one moved the reference
+            uint32_t zeros = 0;                                  // buffers of P that hold zeros for these queries
             float o[H], l[H];
 #pragma unroll
             for (uint32_t j = 0; j < H; ++j) o[j] = l[j] = 0.f;
-            auto add_values = [&](uint32_t tile, bool scaled) {  // O^T of a finished tile; then the change of reference
-                const uint32_t at = tmem + kTmemO + (tile & 1) * 2 * kMaxQ + lanes + q0;
-                float hi[H], lo[H];
-                tmem_ld(at, hi);
-                tmem_ld(at + NQ, lo);
-                tc5::wait_ld();
+            // O^T of a finished tile, which columns [lo, hi) attended to (another session's values stay out of the others' sums even
+            // where they are not numbers); then the change of reference that the tile behind it made.
+            auto add_values = [&](uint32_t tile, bool own, int lo, int hi) {
+                if (!own || (hi > 0 && lo < (int)H)) {
+                    const uint32_t at = tmem + kTmemO + (tile & 1) * 2 * kMaxQ + lanes + q0;
+                    float high[H], low[H];
+                    tmem_ld(at, high);
+                    tmem_ld(at + NQ, low);
+                    tc5::wait_ld();
 #pragma unroll
-                for (uint32_t j = 0; j < H; ++j) o[j] += hi[j] + lo[j];
-                if (scaled) {
+                    for (uint32_t j = 0; j < H; ++j)
+                        if (fabsf(high[j]) != INFINITY) high[j] += low[j];       // (as in scores)
+                    if (!own) {
+#pragma unroll
+                        for (uint32_t j = 0; j < H; j += 2) add2(o[j], o[j + 1], high[j], high[j + 1]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < (int)H; ++j)
+                            if (j >= lo && j < hi) o[j] += high[j];
+                    }
+                }
+                if (moved) {
 #pragma unroll
                     for (uint32_t j = 0; j < H; j += 4) {
                         const float4 a = a4[j / 4];
@@ -390,53 +549,96 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                     }
                 }
             };
-            for (uint32_t t = 0; t < im.tiles; ++t, ++n) {
+            // P of the tile is written: the tensor core may go on.
+            auto hand_over = [&]() {
+                fence_proxy_async();
+                tc5::fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.p_full[n & 1]);
+            };
+            auto put = [&](uint32_t at, const uint32_t (&x)[V / 2]) {
+                // a key's row: the high parts of up to 64 queries, the low ones behind them or in rows of their own
+                uint8_t *to = ps + (n & 1) * p_size + key * 128 + (at >> 7) * (kTile * 128) + ((((at >> 4) & 7) ^ (key & 7)) << 4) + (at & 15);
+                if constexpr (V == 8) *reinterpret_cast<uint4 *>(to) = make_uint4(x[0], x[1], x[2], x[3]);
+                else *reinterpret_cast<uint2 *>(to) = make_uint2(x[0], x[1]);
+            };
+            // Rows behind the last one may hold anything, and a weight of zero does not take a NaN out: those that the last step
+            // multiplies are cleared.
+            auto clear_rows = [&](uint32_t here) {
+                const uint32_t st = n % v_ring;
+                if (ok) ok = mbar_wait_warp(&sm.v_full[st], (n / v_ring) & 1, limit);
+                if (key >= here && key < ((here + 15) & ~15u)) {
+                    uint8_t *row = vs + st * kSlot + (key >> 6) * kPageBlock + (key & 63) * 128;
+#pragma unroll
+                    for (uint32_t e = 0; e < 16; ++e)
+                        *reinterpret_cast<uint4 *>(row + (e >> 3) * 8192 + ((e ^ key) & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+            };
+            // The scores of a tile are there, and with them O^T of the tile two before it; P's buffer is free.
+            auto await_scores = [&]() {
                 if (ok) ok = mbar_wait_warp(&sm.s_full[n & 1], (n >> 1) & 1, limit);
                 tc5::fence_after();
-                const uint32_t at = tmem + (n & 1) * 2 * kMaxQ + lanes + q0, here = im.rows - (im.tile0 + t) * kTile;
-                const bool seen = key < here;
+            };
+            // One tile of `here` keys or more: shared rows, or one session's own, which columns [lo, hi) of this group attend to.
+            auto tile = [&](auto which, uint32_t here, int lo, int hi) {
+                constexpr bool OWN = decltype(which)::value;
+                const uint32_t at = tmem + (n & 1) * 2 * kMaxQ + lanes + q0;
                 float s[H];
-                auto scores = [&](bool infinite) {
-                    float lo[H];
-                    tmem_ld(at, s);
-                    tmem_ld(at + NQ, lo);
-                    tc5::wait_ld();
+                auto mask = [&]() {
+                    if (!OWN && here >= kTile) return;
+                    const bool seen = key < here;
 #pragma unroll
-                    for (uint32_t j = 0; j < H; ++j) {
-                        // (a key with an infinity: the high part has its score, the low one may have the other sign of it or a NaN)
-                        if (infinite && fabsf(s[j]) == INFINITY) continue;
-                        s[j] += lo[j];
+                    for (int j = 0; j < (int)H; ++j) s[j] = seen && (!OWN || (j >= lo && j < hi)) ? s[j] : -INFINITY;
+                };
+                auto scores = [&](bool infinite) {
+                    float low[H];
+                    tmem_ld(at, s);
+                    tmem_ld(at + NQ, low);
+                    tc5::wait_ld();
+                    if (infinite) {
+                        // (a row with an infinity: the high part has its product, the low one may have the other sign of it or a NaN)
+#pragma unroll
+                        for (uint32_t j = 0; j < H; ++j)
+                            if (fabsf(s[j]) != INFINITY) s[j] += low[j];
+                    } else {
+#pragma unroll
+                        for (uint32_t j = 0; j < H; j += 2) add2(s[j], s[j + 1], low[j], low[j + 1]);
                     }
                     if (large) {
 #pragma unroll
                         for (uint32_t j = 0; j < H; ++j) s[j] *= sm.up[it & 1][q0 + j];
                     }
                 };
-                bool moved = t == 0;
-                if (!moved) {
+                moved = fresh;
+                if (!fresh) {
                     scores(false);
                     float top = -INFINITY;
 #pragma unroll
                     for (uint32_t j = 0; j < H; j += 4) {
                         const float4 m = nm4[j / 4];
-                        s[j] += m.x; s[j + 1] += m.y; s[j + 2] += m.z; s[j + 3] += m.w;
-                        top = max3_nan(max3_nan(top, s[j], s[j + 1]), s[j + 2], s[j + 3]);
+                        add2(s[j], s[j + 1], m.x, m.y);
+                        add2(s[j + 2], s[j + 3], m.z, m.w);
                     }
-                    moved = group_or(bar, 128, seen && !(top <= kGrow));         // (or not a number)
+                    mask();
+#pragma unroll
+                    for (uint32_t j = 0; j < H; j += 4) top = max3_nan(max3_nan(top, s[j], s[j + 1]), s[j + 2], s[j + 3]);
+                    moved = group_or(bar, 128, !(top <= kGrow));     // (or not a number)
                 }
                 if (moved) {                                     // (the same in all threads of the group)
                     scores(true);
+                    mask();
                     float v[H];
 #pragma unroll
-                    for (uint32_t j = 0; j < H; ++j) v[j] = s[j] = seen ? s[j] : WR_NEG_SENTINEL;
+                    for (uint32_t j = 0; j < H; ++j) v[j] = s[j];
                     const uint32_t idx = warp_max_many<H>(v, lane);
                     sm.red[q0 + idx][quarter] = v[0];            // (lanes that share an index hold one value)
                     group_sync(bar);
                     if (tid < H) {
                         const float4 w = *reinterpret_cast<const float4 *>(sm.red[q0 + tid]);
-                        const float top = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), WR_NEG_SENTINEL), old = -sm.nm[q0 + tid];
-                        const bool up = t == 0 || top > old + kGrow;
-                        sm.a[q0 + tid] = t == 0 ? 0.f : up ? ex2(old - top) : 1.f;
+                        const float top = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), WR_NEG_SENTINEL);
+                        const float old = fresh ? WR_NEG_SENTINEL : -sm.nm[q0 + tid];
+                        const bool up = fresh || top > old + kGrow;
+                        sm.a[q0 + tid] = up ? ex2(old - top) : 1.f;
                         if (up) sm.nm[q0 + tid] = -top;
                     }
                     group_sync(bar);
@@ -446,55 +648,69 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                         s[j] += m.x; s[j + 1] += m.y; s[j + 2] += m.z; s[j + 3] += m.w;
                         l[j] *= a.x; l[j + 1] *= a.y; l[j + 2] *= a.z; l[j + 3] *= a.w;
                     }
+                    fresh = false;
                 }
-                // the tile before has been multiplied: P is free, its O^T is there
-                if (ok && n > 0) ok = mbar_wait_warp(&sm.o_full, (n - 1) & 1, limit);
-                tc5::fence_after();
-                constexpr uint32_t V = H < 8 ? H : 8;            // queries to a store
 #pragma unroll
                 for (uint32_t j = 0; j < H; j += V) {
-                    uint32_t hi[V / 2], lo[V / 2];
+                    uint32_t high[V / 2], low[V / 2];
 #pragma unroll
                     for (uint32_t e = 0; e < V / 2; ++e) {
-                        const float w0 = seen ? ex2(s[j + 2 * e]) : 0.f, w1 = seen ? ex2(s[j + 2 * e + 1]) : 0.f;
-                        l[j + 2 * e] += w0;
-                        l[j + 2 * e + 1] += w1;
-                        split_half2(w0, w1, hi[e], lo[e]);
+                        const float w0 = ex2(s[j + 2 * e]), w1 = ex2(s[j + 2 * e + 1]);
+                        add2(l[j + 2 * e], l[j + 2 * e + 1], w0, w1);
+                        split_half2(w0, w1, high[e], low[e]);
                     }
-                    // a key's row: the high parts of up to 64 queries, the low ones behind them or in rows of their own
-                    auto put = [&](uint32_t at, const uint32_t (&x)[V / 2]) {
-                        uint8_t *to = ps + key * 128 + (at >> 7) * (kTile * 128) + ((((at >> 4) & 7) ^ (key & 7)) << 4) + (at & 15);
-                        if constexpr (V == 8) *reinterpret_cast<uint4 *>(to) = make_uint4(x[0], x[1], x[2], x[3]);
-                        else *reinterpret_cast<uint2 *>(to) = make_uint2(x[0], x[1]);
-                    };
-                    put(2 * (q0 + j), hi);
-                    put(2 * (q0 + j + NQ), lo);
+                    put(2 * (q0 + j), high);
+                    put(2 * (q0 + j + NQ), low);
                 }
-                if (here < kTile && group == 0) {
-                    // rows behind the last one may hold anything, and a weight of zero does not take a NaN out
-                    const uint32_t st = n % kVSlots;
-                    if (ok) ok = mbar_wait_warp(&sm.v_full[st], (n / kVSlots) & 1, limit);
-                    if (!seen) {
-                        uint8_t *row = vs + st * kSlot + (key >> 6) * kPageBlock + (key & 63) * 128;
-#pragma unroll
-                        for (uint32_t e = 0; e < 16; ++e)
-                            *reinterpret_cast<uint4 *>(row + (e >> 3) * 8192 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                }
-                fence_proxy_async();
-                tc5::fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.p_full);
-                if (t > 0) add_values(n - 1, moved);
+                zeros &= ~(1u << (n & 1));
+            };
+            const uint32_t rows = p.shared_rows[bd.group], n0 = n, n_end = n + im.tiles;
+            uint32_t left = (rows + kTile - 1) / kTile;          // shared tiles of this item
+            left = min(left - min(left, im.tile0), im.tiles);
+            for (uint32_t here = rows - im.tile0 * kTile, t = 0; t < left; ++t, ++n, here -= kTile) {
+                await_scores();
+                if (t >= 2) add_values(n - 2, false, 0, 0);
+                tile(std::false_type{}, here, 0, 0);
+                if (here < kTile && group == 0) clear_rows(here);
+                hand_over();
             }
+            int lo1 = 0, hi1 = 0, lo2 = 0, hi2 = 0;              // columns of the last own tile, of the one before it
+            const uint32_t n_own = n;
+            if (n < n_end)
+                for (Place at = place_at(p, bd, im.tile0 + left); n < n_end; ++n, step(p, bd, at)) {
+                    const int lo = (int)((at.segment - 1) * bd.heads) - (int)q0, hi = lo + (int)bd.heads;
+                    const uint32_t here = p.own_rows[bd.row0 + at.segment - 1] - at.tile * kTile;
+                    await_scores();
+                    if (n >= n0 + 2) add_values(n - 2, n >= n_own + 2, lo2, hi2);
+                    moved = false;
+                    if (hi > 0 && lo < (int)H) {
+                        tile(std::true_type{}, here, lo, hi);
+                    } else if (!(zeros >> (n & 1) & 1)) {
+                        const uint32_t none[V / 2] = {};
+#pragma unroll
+                        for (uint32_t j = 0; j < H; j += V) {
+                            put(2 * (q0 + j), none);
+                            put(2 * (q0 + j + NQ), none);
+                        }
+                        zeros |= 1u << (n & 1);
+                    }
+                    if (here < kTile && group == 0) clear_rows(here);
+                    hand_over();
+                    lo2 = lo1; hi2 = hi1;
+                    lo1 = lo; hi1 = hi;
+                }
             // the next item's queries (the last scores have been read), then this one's results
             bool more = true;
             following = item_at(it + 1, more, true);
             ok = !all_or(!(ok && more));
             if (ok && following.tiles) queries(following, it + 1);
-            if (ok) ok = mbar_wait_warp(&sm.o_full, (n - 1) & 1, limit);
+            // (of either barrier the phase before is known to be over: the scores seen last came behind those values)
+            if (ok && n > n0 + 1) ok = mbar_wait_warp(&sm.o_full[n & 1], ((n - 2) >> 1) & 1, limit);
+            if (ok) ok = mbar_wait_warp(&sm.o_full[(n - 1) & 1], ((n - 1) >> 1) & 1, limit);
             tc5::fence_after();
-            add_values(n - 1, false);
+            if (n > n0 + 1) add_values(n - 2, n >= n_own + 2, lo2, hi2);
+            moved = false;
+            add_values(n - 1, n > n_own, lo1, hi1);
             float *to = p.o + (size_t)(im.part + q0) * kHd + key;
 #pragma unroll
             for (uint32_t j = 0; j < H; ++j)
@@ -504,9 +720,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             group_sync(bar);
             if (tid < H && q0 + tid < im.nq) {
                 const float4 w = *reinterpret_cast<const float4 *>(sm.red[q0 + tid]);
-                p.ml[im.part + q0 + tid] = make_float2(-sm.nm[q0 + tid], (w.x + w.y) + (w.z + w.w));
+                p.ml[im.part + q0 + tid] = make_float2(fresh ? WR_NEG_SENTINEL : -sm.nm[q0 + tid], (w.x + w.y) + (w.z + w.w));
             }
             ok = !all_or(!ok);
+            if (ok && threadIdx.x == 96) {                       // a part of these rows is there
+                __threadfence();
+                atomicAdd(p.done + im.bundle * p.n_kv + im.kvh, 1);
+            }
         };
         for (uint32_t it = 0; ok && im.tiles; ++it) {
             switch (padded(im.nq)) {
@@ -516,85 +736,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             }
             im = following;
         }
+        if (ok) ok = add_up(p, reinterpret_cast<float4 *>(ps), warp - 3, lane);
         if (!ok && lane == 0) atomicCAS(p.err, 0, 84);
     }
     tc5::fence_before();
     __syncthreads();
     tc5::fence_after();
     if (warp == 1) tc5::dealloc(tmem, kTmemCols);
-}
-
-// The chunks of a row added up: those of its group's shared rows, then those of its own.  Warp w has chunks w, w + 4, ...: the loads of
-// up to 32 chunks are one round trip, which bounds it (two: maxima and sums first, 2.5 us longer).
-constexpr uint32_t kMergeAhead = 8;
-__global__ void __launch_bounds__(kHd) shared_merge_kernel(const __grid_constant__ SharedParams p)
-{
-    __shared__ float4 sums[3][32];
-    pdl_wait();
-    pdl_trigger();
-    const uint32_t head = blockIdx.x, s = blockIdx.y, kvh = head / p.per, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint32_t first[2], step[2], count[2];
-#pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-        const uint32_t at = i ? p.own_seg[s] : p.group_seg[s];
-        count[i] = first[i] = step[i] = 0;
-        if (at >= kMaxSegs) continue;
-        const Segment &g = p.seg[at];
-        count[i] = g.chunks;
-        step[i] = p.n_kv * g.queries;
-        first[i] = g.part0 + kvh * g.queries + (s - g.row0) * p.per + head % p.per;
-    }
-    const uint32_t n = count[0] + count[1];
-    auto part = [&](uint32_t i) { return i < count[0] ? first[0] + i * step[0] : first[1] + (i - count[0]) * step[1]; };
-    float4 o[kMergeAhead];
-    float m[kMergeAhead];
-    auto load = [&](uint32_t i0) {
-#pragma unroll
-        for (uint32_t u = 0; u < kMergeAhead; ++u) {
-            const uint32_t i = i0 + 4 * u;
-            if (i >= n) continue;
-            o[u] = *reinterpret_cast<const float4 *>(p.o + (size_t)part(i) * kHd + 4 * lane);
-            m[u] = p.ml[part(i)].x;
-        }
-    };
-    load(warp);
-    float top = WR_NEG_SENTINEL, l = 0.f;
-    for (uint32_t i = lane; i < n; i += 32) {
-        const float2 ml = p.ml[part(i)];
-        const float t = fmaxf(top, ml.x);
-        l = l * ex2(top - t) + ml.y * ex2(ml.x - t);
-        top = t;
-    }
-    const float mine = top;
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    l *= ex2(mine - top);
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t i0 = warp;; load(i0)) {
-#pragma unroll
-        for (uint32_t u = 0; u < kMergeAhead; ++u) {
-            if (i0 + 4 * u >= n) continue;
-            const float w = ex2(m[u] - top);
-            acc.x = fmaf(w, o[u].x, acc.x); acc.y = fmaf(w, o[u].y, acc.y);
-            acc.z = fmaf(w, o[u].z, acc.z); acc.w = fmaf(w, o[u].w, acc.w);
-        }
-        i0 += 4 * kMergeAhead;
-        if (i0 >= n) break;
-    }
-    if (warp) sums[warp - 1][lane] = acc;
-    __syncthreads();
-    if (warp) return;
-#pragma unroll
-    for (uint32_t w = 0; w < 3; ++w) {
-        const float4 x = sums[w][lane];
-        acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
-    }
-    // (a row of which no key counts, all scores -inf, is zeros)
-    if (l == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    else acc = make_float4(acc.x / l, acc.y / l, acc.z / l, acc.w / l);
-    *reinterpret_cast<float4 *>(p.out + ((size_t)s * p.n_q + head) * kHd + 4 * lane) = acc;
 }
 
 }  // namespace
@@ -621,7 +769,7 @@ int wr_shared_validate(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv,
     return s == n_sess ? WR_CUDA_OK : WR_CUDA_ERR_INVAL;
 }
 
-// Enqueue both kernels on device-resident q / out.  Caller holds ctx->lock and has validated the arguments.
+// Enqueue the kernel on device-resident q / out.  Caller holds ctx->lock and has validated the arguments.
 int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *seq_lens,
                      uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, const float *dq, float *dout,
                      uint32_t n_q, float scale_override)
@@ -630,54 +778,68 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
     p.n_q = n_q;
     p.n_kv = kv[0]->n_kv_at(layer);
     p.per = n_q / p.n_kv;
-    uint64_t tiles = 0;
-    auto add = [&](const wr_cuda_kv *of, uint32_t first_page, uint32_t rows, uint32_t row0, uint32_t sessions) {
-        Segment &g = p.seg[p.n_segs++];
-        g.pages = of->d_pages + (size_t)layer * of->n_pages + first_page;
-        g.rows = rows;
-        g.row0 = row0;
-        g.queries = sessions * p.per;
-        g.qtiles = (g.queries + kMaxQ - 1) / kMaxQ;
-        tiles += (uint64_t)((rows + kTile - 1) / kTile) * p.n_kv * g.qtiles;
-    };
+    const uint32_t splits = (p.per + kMaxQ - 1) / kMaxQ, most = std::max(kMaxQ / p.per, 1u);     // bundles to a session, or sessions to a bundle
+    uint32_t longest = 0;
     for (uint32_t g = 0, s = 0; g < n_groups; s += group_sess[g++]) {
-        if (group_rows[g]) add(kv[s], 0, group_rows[g], s, group_sess[g]);
-        for (uint32_t i = s; i < s + group_sess[g]; ++i)
-            if (seq_lens[i] > group_rows[g]) add(kv[i], group_rows[g] / kPageTokens, seq_lens[i] - group_rows[g], i, 1);
+        p.shared_pages[g] = kv[s]->d_pages + (size_t)layer * kv[s]->n_pages;
+        p.shared_rows[g] = group_rows[g];
+        for (uint32_t i = s; i < s + group_sess[g]; ++i) {
+            p.own_pages[i] = kv[i]->d_pages + (size_t)layer * kv[i]->n_pages + group_rows[g] / kPageTokens;
+            p.own_rows[i] = seq_lens[i] - group_rows[g];
+        }
+        for (uint32_t i = s; i < s + group_sess[g]; i += most) {
+            const uint32_t n = std::min(most, s + group_sess[g] - i);
+            if (p.n_bundles + splits > kMaxBundles) return WR_CUDA_ERR_LIMIT;
+            uint32_t tiles = (group_rows[g] + kTile - 1) / kTile;
+            for (uint32_t t = i; t < i + n; ++t) {
+                tiles += (p.own_rows[t] + kTile - 1) / kTile;
+                p.first_bundle[t] = (uint8_t)p.n_bundles;
+            }
+            for (uint32_t h = 0; h < splits; ++h)
+                p.bundle[p.n_bundles++] = {g, i, n, h * kMaxQ, std::min(kMaxQ, p.per - h * kMaxQ), tiles, 0, 0, 0};
+            longest = std::max(longest, tiles);
+        }
     }
-    // Chunks as long as the SMs' even share of all tiles: then there is about one item per SM, and what is left over is
-    // short and comes last.
-    const uint32_t per = (uint32_t)((tiles + ctx->sm_count - 1) / ctx->sm_count);
-    for (uint32_t i = 0; i < p.n_segs; ++i) p.seg[i].chunks = ((p.seg[i].rows + kTile - 1) / kTile + per - 1) / per;
-    std::stable_sort(p.seg, p.seg + p.n_segs, [](const Segment &a, const Segment &b) {
-        return (uint64_t)a.rows * b.chunks > (uint64_t)b.rows * a.chunks;
-    });
-    std::fill(p.group_seg, p.group_seg + WR_CUDA_BATCH_MAX, (uint8_t)kMaxSegs);
-    std::fill(p.own_seg, p.own_seg + WR_CUDA_BATCH_MAX, (uint8_t)kMaxSegs);
+    // Items are even shares of the bundles' lists, in one round of the SMs or a few: the fewer tiles one after the other, an item's
+    // beginning and end counted as two, the sooner.
+    auto items_of = [&](uint32_t share) {
+        uint64_t n = 0;
+        for (uint32_t i = 0; i < p.n_bundles; ++i) n += (uint64_t)((p.bundle[i].tiles + share - 1) / share) * p.n_kv;
+        return n;
+    };
+    uint32_t share = longest, best = ~0u;
+    for (uint32_t rounds = 1; rounds <= 4; ++rounds) {
+        uint32_t lo = 1, hi = longest;                           // the smallest share that makes no more items than that
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (items_of(mid) <= (uint64_t)rounds * ctx->sm_count) hi = mid;
+            else lo = mid + 1;
+        }
+        const uint32_t time = (uint32_t)((items_of(lo) + ctx->sm_count - 1) / ctx->sm_count) * (lo + 2);
+        if (time < best) {
+            best = time;
+            share = lo;
+        }
+    }
     uint64_t parts = 0;
-    for (uint32_t i = 0; i < p.n_segs; ++i) {
-        Segment &g = p.seg[i];
-        g.item0 = p.items;
-        g.part0 = (uint32_t)parts;
-        p.items += g.chunks * g.qtiles * p.n_kv;
-        parts += (uint64_t)g.chunks * p.n_kv * g.queries;
+    for (uint32_t i = 0; i < p.n_bundles; ++i) {
+        Bundle &b = p.bundle[i];
+        b.chunks = (b.tiles + share - 1) / share;
+        b.item0 = p.items;
+        b.part0 = (uint32_t)parts;
+        p.items += b.chunks * p.n_kv;
+        parts += (uint64_t)b.chunks * p.n_kv * b.sessions * b.heads;
     }
     if (parts > 0x7fffffffu) return WR_CUDA_ERR_LIMIT;
-    for (uint32_t g = 0, s = 0; g < n_groups; s += group_sess[g++])
-        for (uint32_t i = 0; i < p.n_segs; ++i) {
-            const Segment &x = p.seg[i];
-            const bool of_group = group_rows[g] && x.row0 == s && x.queries == group_sess[g] * p.per && x.rows == group_rows[g] &&
-                                  x.pages == kv[s]->d_pages + (size_t)layer * kv[s]->n_pages;
-            for (uint32_t r = s; r < s + group_sess[g]; ++r) {
-                if (of_group) p.group_seg[r] = (uint8_t)i;
-                else if (x.row0 == r && x.queries == p.per) p.own_seg[r] = (uint8_t)i;
-            }
-        }
-    const size_t head = 256, ml = ((size_t)parts * sizeof(float2) + 255) & ~(size_t)255;
+    // counters first: they are zeros between launches
+    if ((size_t)p.n_bundles * p.n_kv * sizeof(int) + 256 > WR_KEPT_HEAD) return WR_CUDA_ERR_LIMIT;
+    const size_t head = WR_KEPT_HEAD, ml = ((size_t)parts * sizeof(float2) + 255) & ~(size_t)255;
     char *ws = nullptr;
     int rc = wr_ctx_keep(ctx, head + ml + (size_t)parts * kHd * sizeof(float), &ws);
     if (rc != WR_CUDA_OK) return rc;
     p.sched = reinterpret_cast<int *>(ws);
+    p.done = reinterpret_cast<int *>(ws + 256);
+    p.rows = n_sess * n_q;
     p.ml = reinterpret_cast<float2 *>(ws + head);
     p.o = reinterpret_cast<float *>(ws + head + ml);
     p.q = dq;
@@ -689,10 +851,12 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
         WR_CUDA_TRY(cudaFuncSetAttribute(attn_shared_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
         ctx->attr_flags |= 0x100u;
     }
-    WR_CUDA_TRY(wr_launch_pdl(attn_shared_kernel, dim3(std::min<uint32_t>(p.items, (uint32_t)ctx->sm_count)), dim3(kThreads),
-                              (size_t)kSmem, ctx->stream, p));
-    WR_CUDA_TRY(wr_launch_pdl(shared_merge_kernel, dim3(n_q, n_sess), dim3(kHd), (size_t)0, ctx->stream, p));
-    ctx->launches += 2;
+    const uint32_t grid = std::min<uint32_t>(p.items, (uint32_t)ctx->sm_count);
+    for (uint32_t i = 0; i < p.n_bundles; ++i) p.widest = std::max(p.widest, p.bundle[i].sessions * p.bundle[i].heads);
+    // a row's team: as many warps as there are for all rows at once
+    for (p.team = kMergeWarps; p.team > 1 && (uint64_t)p.rows * p.team > (uint64_t)grid * kMergeWarps;) p.team /= 2;
+    WR_CUDA_TRY(wr_launch_pdl(attn_shared_kernel, dim3(grid), dim3(kThreads), (size_t)kSmem, ctx->stream, p));
+    ctx->launches++;
     WR_CUDA_TRY(cudaGetLastError());
     return WR_CUDA_OK;
 }

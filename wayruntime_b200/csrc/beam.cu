@@ -363,10 +363,10 @@ int wr_beam_launch(wr_cuda_ctx *ctx, const wr_beam_args &a)
     p.parts = (most + p.batches - 1) / p.batches;
     const size_t n = (size_t)rows * p.parts, sums = (n * sizeof(float2) + 255) & ~(size_t)255;
     char *ws = nullptr;
-    int rc = wr_ctx_keep(ctx, 256 + sums + n * a.n_out * sizeof(uint2), &ws);
+    int rc = wr_ctx_keep(ctx, WR_KEPT_HEAD + sums + n * a.n_out * sizeof(uint2), &ws);
     if (rc != WR_CUDA_OK) return rc;
-    p.sums = reinterpret_cast<float2 *>(ws + 256);               // (the first bytes are attn_shared.cu's counters)
-    p.best = reinterpret_cast<uint2 *>(ws + 256 + sums);
+    p.sums = reinterpret_cast<float2 *>(ws + WR_KEPT_HEAD);
+    p.best = reinterpret_cast<uint2 *>(ws + WR_KEPT_HEAD + sums);
     WR_CUDA_TRY(wr_launch_pdl(beam_part_kernel, dim3(p.parts, rows), dim3(kThreads), (size_t)0, ctx->stream, p));
     WR_CUDA_TRY(wr_launch_pdl(beam_final_kernel, dim3(a.groups), dim3(kThreads), (size_t)0, ctx->stream, p));
     ctx->launches += 2;

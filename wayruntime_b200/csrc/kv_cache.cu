@@ -108,6 +108,8 @@ int wr_ctx_sync_checked(wr_cuda_ctx *ctx)
             WR_CUDA_TRY(cudaMemsetAsync(ctx->tickets, 0, ctx->ticket_count * sizeof(int), ctx->stream));
         if (ctx->prefill_sched)
             WR_CUDA_TRY(cudaMemsetAsync(ctx->prefill_sched, 0, 2 * sizeof(int), ctx->stream));
+        if (ctx->kept) WR_CUDA_TRY(cudaMemsetAsync(ctx->kept, 0, WR_KEPT_HEAD, ctx->stream));
+        for (void *p : ctx->outgrown) WR_CUDA_TRY(cudaMemsetAsync(p, 0, WR_KEPT_HEAD, ctx->stream));
         WR_CUDA_TRY(cudaStreamSynchronize(ctx->stream));
         return WR_CUDA_ERR_INTERNAL;
     }
@@ -265,7 +267,7 @@ int wr_ctx_keep(wr_cuda_ctx *ctx, size_t bytes, char **out)
         const size_t want = std::max({bytes, 2 * ctx->kept_bytes, (size_t)8 << 20});
         void *p = nullptr;
         WR_CUDA_TRY(cudaMalloc(&p, want));
-        const cudaError_t e = cudaMemsetAsync(p, 0, want, ctx->stream);
+        const cudaError_t e = cudaMemsetAsync(p, 0, WR_KEPT_HEAD, ctx->stream);
         if (e != cudaSuccess) {
             (void)cudaGetLastError();
             (void)cudaFree(p);
