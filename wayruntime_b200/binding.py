@@ -223,6 +223,17 @@ def _buf(x):
     raise TypeError(f"unsupported buffer {type(x)}")
 
 
+_KINDS = {}                              # dtype -> "f": float32, "i": 32-bit integer, "": neither
+
+
+def _kind(x):
+    k = _KINDS.get(x.dtype)
+    if k is None:
+        name = str(x.dtype).split(".")[-1]
+        k = _KINDS[x.dtype] = "f" if name == "float32" else "i" if name in ("int32", "uint32") else ""
+    return k
+
+
 def _same_mem(*kinds):
     ks = {k for k in kinds if k is not None}
     if len(ks) != 1:
@@ -510,17 +521,21 @@ class Context:
         [groups, beams]; out_scores float32, out_beams and out_tokens 32-bit integers, [groups, n_out] each (0xffffffff, or -1,
         where there is no continuation)."""
         groups, beams, vocab = logits.shape
-        if tuple(scores.shape) != (groups, beams):
+        if scores.shape != (groups, beams):
             raise ValueError("scores: one per row of logits")
-        if any(tuple(x.shape) != tuple(out_scores.shape) for x in (out_beams, out_tokens)) or out_scores.shape[0] != groups:
+        if not out_scores.shape == out_beams.shape == out_tokens.shape or out_scores.shape[0] != groups:
             raise ValueError("results: [groups, n_out] each")
-        for x, kind in ((logits, "float32"), (scores, "float32"), (out_scores, "float32"), (out_beams, "int32"), (out_tokens, "int32")):
-            if not str(x.dtype).endswith(kind):                  # (uint32 too)
-                raise ValueError(f"{kind} expected, got {x.dtype}")
-        bufs = [_buf(x) for x in (logits, scores, out_scores, out_beams, out_tokens)]
-        (lp, sp, a, b, t), mem = (x[0] for x in bufs), _same_mem(*(x[1] for x in bufs))
-        _check(self._lib.wr_cuda_beam_select(self._h, groups, beams, vocab, lp, sp, out_scores.shape[1], a, b, t, mem),
-               "wr_cuda_beam_select")
+        if _kind(logits) != "f" or _kind(scores) != "f" or _kind(out_scores) != "f":
+            raise ValueError("logits, scores and out_scores: float32 expected")
+        if _kind(out_beams) != "i" or _kind(out_tokens) != "i":
+            raise ValueError("out_beams and out_tokens: 32-bit integers expected")
+        lp, lm, _l = _buf(logits)
+        sp, sm, _s = _buf(scores)
+        ap, am, _a = _buf(out_scores)
+        bp, bm, _b = _buf(out_beams)
+        tp, tm, _t = _buf(out_tokens)
+        _check(self._lib.wr_cuda_beam_select(self._h, groups, beams, vocab, lp, sp, out_scores.shape[1], ap, bp, tp,
+                                             _same_mem(lm, sm, am, bm, tm)), "wr_cuda_beam_select")
 
     def attn_prefill(self, kv, layer, p0, n, q, out, n_q_heads, scale=0.0, window=0):
         qp, qm, qa = _buf(q)

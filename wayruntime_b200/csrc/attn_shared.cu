@@ -832,7 +832,7 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
     }
     if (parts > 0x7fffffffu) return WR_CUDA_ERR_LIMIT;
     // counters first: they are zeros between launches
-    if ((size_t)p.n_bundles * p.n_kv * sizeof(int) + 256 > WR_KEPT_HEAD) return WR_CUDA_ERR_LIMIT;
+    if ((size_t)p.n_bundles * p.n_kv * sizeof(int) + 256 > WR_KEPT_HEAD / 2) return WR_CUDA_ERR_LIMIT;
     const size_t head = WR_KEPT_HEAD, ml = ((size_t)parts * sizeof(float2) + 255) & ~(size_t)255;
     char *ws = nullptr;
     int rc = wr_ctx_keep(ctx, head + ml + (size_t)parts * kHd * sizeof(float), &ws);

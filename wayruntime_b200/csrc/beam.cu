@@ -2,26 +2,25 @@
 //     total(b, v) = score_b + logit(b, v) - log sum_u exp(logit(b, u))
 // The reference has no beam search; its sampler takes one row of logits (src/core/sample.c:239).
 //
-// One pass over the logits: beam_part_kernel gives a part of a row to a CTA, which leaves the part's sum of exponentials
-// (against the part's maximum) and its n_out best logits; within a row totals are in the order of logits, so nothing else of
-// the part can be among the row's best.  beam_final_kernel puts a request's parts together: sums and totals in 64 bits,
-// since candidates of two beams may lie closer than an F32 rounding.  HBM bounds the first (4 bytes a logit), launches and
-// round trips the calls of few rows.
+// One pass over the logits: a CTA takes a part of a row and leaves the part's sum of exponentials (against the part's
+// maximum) and its n_out best logits; within a row totals are in the order of logits, so nothing else of the part can be
+// among the row's best.  The CTA that is the last of its request puts the parts together: sums and totals in 64 bits,
+// since candidates of two beams may lie closer than an F32 rounding.  HBM bounds it (4 bytes a logit) where there are many
+// rows, round trips where there are few; a second kernel for the parts took 2 us more.
 //
 // Candidates are found with a threshold that is sure to keep n_out of them: of 32 lanes' maxima (distinct elements) the
-// n_out-th largest.  What reaches it goes to a list, and an entry's place in the result is the number of better ones.
-// Where a list runs over (rows of few values) the best are taken one after the other instead.
+// n_out-th largest.  What reaches it goes to a list, what still reaches the last threshold to another, and an entry's place in
+// the result is the number of better ones there.  Where a list runs over (rows of few values) the best are taken one after the
+// other instead.
 // Ties go to the lower beam, then the lower token.  Logits of -inf are no candidates, nor is anything of a beam whose score is
 // -inf or NaN (its row is not read) or whose sum is not finite (a NaN or +inf among its logits).
-#include <cfloat>
-
 #include "kv_share.cuh"
 #include "rows_dev.cuh"
 
 namespace {
 
 constexpr uint32_t kThreads = 256, kWarps = kThreads / 32, kVecs = 4, kBatch = kThreads * kVecs * 4;   // logits a CTA has in hand
-constexpr uint32_t kPartList = 1024, kFinalList = 1024;
+constexpr uint32_t kList = 1024, kMaxLists = 1024;
 constexpr uint32_t kNone = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -30,6 +29,21 @@ struct BeamParams {
     uint32_t parts, batches;             // parts of a row; batches of a part
     float2 *sums;                        // [row][part]: largest logit, sum of exponentials against it
     uint2 *best;                         // [row][part][n_out]: logit's bits, token; in order
+    int *done;                           // [request]: parts that are there
+};
+// A CTA's shared memory: while it works on its part, and on a request's parts.
+struct PartMemory {
+    float v[kList], lane_top[kThreads], warp_m[kWarps], warp_s[kWarps], kept_v[kList];
+    uint32_t i[kList], kept_i[kList], count, kept;
+    int least;                           // the threshold, as a whole number in the order of floats
+};
+struct FinalMemory {
+    double offset[WR_CUDA_BATCH_MAX], head[kMaxLists], t[kList], warp_t[kWarps];
+    uint32_t b[kList], i[kList], count;
+};
+union Memory {
+    PartMemory part;
+    FinalMemory all;
 };
 
 __device__ __forceinline__ float ex2(float x)
@@ -57,14 +71,24 @@ __device__ __forceinline__ bool before(float v, uint32_t i, float w, uint32_t j)
 
 __device__ __forceinline__ const float *row_of(const wr_beam_args &a, uint32_t r) { return a.logits + (size_t)(a.mapped ? a.map[r] : r) * a.ld; }
 
-__global__ void __launch_bounds__(kThreads) beam_part_kernel(const __grid_constant__ BeamParams p)
+// a < b in the order of results: the logit or total, then the beam, then the token
+__device__ __forceinline__ bool before(double v, uint32_t b, uint32_t i, double w, uint32_t c, uint32_t j)
 {
-    __shared__ float list_v[kPartList], lane_top[kThreads], warp_m[kWarps], warp_s[kWarps];
-    __shared__ uint32_t list_i[kPartList], count;
-    __shared__ int least;                // the threshold, as a whole number in the order of floats
-    pdl_wait();
-    pdl_trigger();
-    const uint32_t part = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = p.a.n_out;
+    return v > w || (v == w && (b < c || (b == c && i < j)));
+}
+__device__ __forceinline__ int order(float v) { const int i = __float_as_int(v); return i ^ ((i >> 31) & 0x7fffffff); }
+__device__ __forceinline__ float value(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
+// sums of exponentials against two maxima as one
+__device__ __forceinline__ void join(float &m, float &s, float m2, float s2)
+{
+    const float t = fmaxf(m, m2), base = t == -INFINITY ? 0.f : t;
+    s = s * ex2((m - base) * kLog2e) + s2 * ex2((m2 - base) * kLog2e);
+    m = t;
+}
+
+__device__ __forceinline__ void part_of_row(const BeamParams &p, PartMemory &sm, uint32_t part, uint32_t row)
+{
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = p.a.n_out;
     uint2 *const best = p.best + ((size_t)row * p.parts + part) * k;
     const float score = p.a.scores[row];
     if (!(score > -INFINITY)) {          // (NaN too)
@@ -75,32 +99,32 @@ __global__ void __launch_bounds__(kThreads) beam_part_kernel(const __grid_consta
     // Vectors are aligned in memory: the row begins `lead` elements into the first one.
     const float *const x = row_of(p.a, row);
     const uint32_t lead = (uint32_t)((uintptr_t)x >> 2) & 3u;
-    const uint64_t first = (uint64_t)part * p.batches * kBatch;
+    const uint64_t first = (uint64_t)part * p.batches * kBatch, end = (uint64_t)p.a.vocab + lead;
     auto load = [&](uint32_t b, float (&v)[4 * kVecs]) {
 #pragma unroll
         for (uint32_t u = 0; u < kVecs; ++u) {
             const uint64_t at = first + (uint64_t)b * kBatch + (u * kThreads + threadIdx.x) * 4u;
-            if (at >= lead && at + 4 <= (uint64_t)p.a.vocab + lead) {
+            if (at >= lead && at + 4 <= end) {
                 const float4 w = __ldcs(reinterpret_cast<const float4 *>(x + (at - lead)));
                 v[4 * u] = w.x; v[4 * u + 1] = w.y; v[4 * u + 2] = w.z; v[4 * u + 3] = w.w;
             } else {
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e)
-                    v[4 * u + e] = at + e >= lead && at + e < (uint64_t)p.a.vocab + lead ? __ldcs(x + (at + e - lead)) : -INFINITY;
+                for (uint32_t e = 0; e < 4; ++e) v[4 * u + e] = at + e >= lead && at + e < end ? __ldcs(x + (at + e - lead)) : -INFINITY;
             }
         }
     };
-    auto order = [](float v) { const int i = __float_as_int(v); return i ^ ((i >> 31) & 0x7fffffff); };
-    auto value = [](int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); };
-    if (threadIdx.x == 0) {
-        count = 0;
-        least = order(-INFINITY);
-    }
+    auto token_of = [&](uint32_t b, uint32_t e) {
+        return (uint32_t)(first + (uint64_t)b * kBatch + ((e / 4) * kThreads + threadIdx.x) * 4u + (e & 3) - lead);
+    };
     float v[4 * kVecs], next[4 * kVecs], m = -INFINITY, s = 0.f;
     load(0, v);
+    if (threadIdx.x == 0) {
+        sm.count = sm.kept = 0;
+        sm.least = order(-INFINITY);
+    }
     __syncthreads();
     for (uint32_t b = 0; b < p.batches; ++b) {
-        if (first + (uint64_t)b * kBatch >= (uint64_t)p.a.vocab + lead) break;
+        if (first + (uint64_t)b * kBatch >= end) break;
         if (b + 1 < p.batches) load(b + 1, next);
         float top = -INFINITY;
 #pragma unroll
@@ -115,32 +139,34 @@ __global__ void __launch_bounds__(kThreads) beam_part_kernel(const __grid_consta
         // asks all the CTA's.)
         float bound;
         if (k > 16 && b == 0) {
-            lane_top[threadIdx.x] = m;
+            sm.lane_top[threadIdx.x] = m;
             __syncthreads();
             uint32_t larger_ones = 0;
             for (uint32_t i = 0; i < kThreads; i += 4) {
-                const float4 w = *reinterpret_cast<const float4 *>(lane_top + i);
+                const float4 w = *reinterpret_cast<const float4 *>(sm.lane_top + i);
                 larger_ones += (w.x > m || (w.x == m && i < threadIdx.x)) + (w.y > m || (w.y == m && i + 1 < threadIdx.x)) +
                                (w.z > m || (w.z == m && i + 2 < threadIdx.x)) + (w.w > m || (w.w == m && i + 3 < threadIdx.x));
             }
-            if (larger_ones == k - 1) least = order(m);
+            if (larger_ones == k - 1) sm.least = order(m);
             __syncthreads();
-            bound = value(least);
+            bound = value(sm.least);
         } else {
-            const float kth = __shfl_sync(0xffffffffu, warp_sort(m, lane), k - 1);
-            if (lane == 0) atomicMax(&least, order(kth));
+            // (a warp's threshold moves when one of its lanes' maxima does)
+            if (__any_sync(0xffffffffu, m > was)) {
+                const float kth = __shfl_sync(0xffffffffu, warp_sort(m, lane), k - 1);
+                if (lane == 0) atomicMax(&sm.least, order(kth));
+            }
             if (b == 0) __syncthreads();
-            else __syncwarp();
-            bound = value(*(volatile int *)&least);              // (whichever warps have answered: any of their bounds is one)
+            bound = value(*(volatile int *)&sm.least);           // (whichever warps have answered: any of their bounds is one)
         }
         if (top >= bound) {
 #pragma unroll
             for (uint32_t e = 0; e < 4 * kVecs; ++e)
                 if (v[e] >= bound && v[e] > -INFINITY) {
-                    const uint32_t at = atomicAdd(&count, 1);
-                    if (at < kPartList) {
-                        list_v[at] = v[e];
-                        list_i[at] = (uint32_t)(first + (uint64_t)b * kBatch + ((e / 4) * kThreads + threadIdx.x) * 4u + (e & 3) - lead);
+                    const uint32_t at = atomicAdd(&sm.count, 1);
+                    if (at < kList) {
+                        sm.v[at] = v[e];
+                        sm.i[at] = token_of(b, e);
                     }
                 }
         }
@@ -148,34 +174,37 @@ __global__ void __launch_bounds__(kThreads) beam_part_kernel(const __grid_consta
         for (uint32_t e = 0; e < 4 * kVecs; ++e) v[e] = next[e];
     }
     // the part's sum: lanes, then warps, in order
-    auto join = [](float &m1, float &s1, float m2, float s2) {
-        const float t = fmaxf(m1, m2), base = t == -INFINITY ? 0.f : t;
-        s1 = s1 * ex2((m1 - base) * kLog2e) + s2 * ex2((m2 - base) * kLog2e);
-        m1 = t;
-    };
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) {
         const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
         join(m, s, m2, s2);
     }
     if (lane == 0) {
-        warp_m[warp] = m;
-        warp_s[warp] = s;
+        sm.warp_m[warp] = m;
+        sm.warp_s[warp] = s;
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (uint32_t w = 1; w < kWarps; ++w) join(m, s, warp_m[w], warp_s[w]);
+        for (uint32_t w = 1; w < kWarps; ++w) join(m, s, sm.warp_m[w], sm.warp_s[w]);
         p.sums[(size_t)row * p.parts + part] = make_float2(m, s);
     }
-    const uint32_t n = count;
-    if (n <= kPartList) {
-        const float bound = value(least);                        // (it has grown since most entries were listed)
+    const uint32_t listed = sm.count;
+    if (listed <= kList) {
+        const float bound = value(sm.least);                     // (it has grown since most entries were listed)
+        for (uint32_t i = threadIdx.x; i < listed; i += kThreads)
+            if (sm.v[i] >= bound) {
+                const uint32_t at = atomicAdd(&sm.kept, 1);
+                sm.kept_v[at] = sm.v[i];
+                sm.kept_i[at] = sm.i[i];
+            }
+        __syncthreads();
+        const uint32_t n = sm.kept;
         for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-            const float w = list_v[i];
-            if (w < bound) continue;
-            const uint32_t at = list_i[i];
+            const float w = sm.kept_v[i];
+            const uint32_t at = sm.kept_i[i];
             uint32_t place = 0;
-            for (uint32_t j = 0; j < n; ++j) place += before(list_v[j], list_i[j], w, at);
+#pragma unroll 4
+            for (uint32_t j = 0; j < n; ++j) place += before(sm.kept_v[j], sm.kept_i[j], w, at);
             if (place < k) best[place] = make_uint2(__float_as_uint(w), at);
         }
         if (threadIdx.x >= n && threadIdx.x < k) best[threadIdx.x] = make_uint2(__float_as_uint(-INFINITY), kNone);
@@ -192,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) beam_part_kernel(const __grid_consta
             load(b, v);
 #pragma unroll
             for (uint32_t e = 0; e < 4 * kVecs; ++e) {
-                const uint32_t at = (uint32_t)(first + (uint64_t)b * kBatch + ((e / 4) * kThreads + threadIdx.x) * 4u + (e & 3) - lead);
+                const uint32_t at = token_of(b, e);
                 if (v[e] > -INFINITY && (!started || before(last_v, last_i, v[e], at)) && before(v[e], at, top_v, top_i)) {
                     top_v = v[e];
                     top_i = at;
@@ -207,12 +236,12 @@ __global__ void __launch_bounds__(kThreads) beam_part_kernel(const __grid_consta
         }
         __syncthreads();
         if (lane == 0) {
-            list_v[warp] = top_v;
-            list_i[warp] = top_i;
+            sm.v[warp] = top_v;
+            sm.i[warp] = top_i;
         }
         __syncthreads();
         for (uint32_t w = 0; w < kWarps; ++w)
-            if (before(list_v[w], list_i[w], top_v, top_i)) top_v = list_v[w], top_i = list_i[w];
+            if (before(sm.v[w], sm.i[w], top_v, top_i)) top_v = sm.v[w], top_i = sm.i[w];
         if (threadIdx.x == 0) best[j] = make_uint2(__float_as_uint(top_v), top_i);
         started = true;
         last_v = top_v;
@@ -220,78 +249,76 @@ __global__ void __launch_bounds__(kThreads) beam_part_kernel(const __grid_consta
     }
 }
 
-__device__ __forceinline__ bool before(double v, uint32_t b, uint32_t i, double w, uint32_t c, uint32_t j)
+__device__ __forceinline__ void parts_of_request(const BeamParams &p, FinalMemory &sm, uint32_t group)
 {
-    return v > w || (v == w && (b < c || (b == c && i < j)));
-}
-
-__global__ void __launch_bounds__(kThreads) beam_final_kernel(const __grid_constant__ BeamParams p)
-{
-    __shared__ double offset[WR_CUDA_BATCH_MAX], list_t[kFinalList], warp_t[kWarps];
-    __shared__ uint32_t list_b[kFinalList], list_i[kFinalList], count;
-    pdl_wait();
-    pdl_trigger();
-    const uint32_t group = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = p.a.n_out, beams = p.a.beams;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = p.a.n_out, beams = p.a.beams;
     const size_t row0 = (size_t)group * beams;
-    if (threadIdx.x == 0) count = 0;
+    const uint32_t lists = beams * p.parts;
+    const uint2 *const best = p.best + row0 * p.parts * k;
+    // every list's best, on its way while the sums are put together
+    float mine[(kMaxLists + kThreads - 1) / kThreads];
+#pragma unroll
+    for (uint32_t u = 0; u < kMaxLists / kThreads; ++u) {
+        const uint32_t i = threadIdx.x + u * kThreads;
+        if (i < lists) mine[u] = __uint_as_float(__ldcg(&best[(size_t)i * k].x));
+    }
+    if (threadIdx.x == 0) sm.count = 0;
     // score less the logarithm of the row's sum
     for (uint32_t b = warp; b < beams; b += kWarps) {
         const float2 *sums = p.sums + (row0 + b) * p.parts;
         float top = -INFINITY;
-        for (uint32_t i = lane; i < p.parts; i += 32) top = fmaxf(top, sums[i].x);
+        for (uint32_t i = lane; i < p.parts; i += 32) top = fmaxf(top, __ldcg(sums + i).x);
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         double s = 0.0;
         for (uint32_t i = lane; i < p.parts; i += 32) {
-            const float2 ms = sums[i];
+            const float2 ms = __ldcg(sums + i);
             if (ms.y != 0.f) s += (double)ms.y * exp((double)ms.x - (double)top);
         }
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         const double t = (double)p.a.scores[row0 + b] - ((double)top + log(s));
-        if (lane == 0) offset[b] = t > -INFINITY && t < INFINITY ? t : -INFINITY;            // (no sum, or none that is finite)
+        if (lane == 0) sm.offset[b] = t > -INFINITY && t < INFINITY ? t : -INFINITY;         // (no sum, or none that is finite)
     }
     __syncthreads();
-    const uint32_t lists = beams * p.parts;
-    const uint2 *const best = p.best + row0 * p.parts * k;
-    auto total = [&](uint32_t list, uint32_t j, uint32_t &token) -> double {
-        const uint2 c = best[(size_t)list * k + j];
-        token = c.y;
-        return offset[list / p.parts] + (double)__uint_as_float(c.x);
-    };
-    // every list begins with its best: a bound from 32 threads' best beginnings
+    // a bound from 32 threads' best
     double top = -INFINITY;
-    for (uint32_t i = threadIdx.x; i < lists; i += kThreads) {
-        uint32_t token;
-        top = larger(top, total(i, 0, token));
+#pragma unroll
+    for (uint32_t u = 0; u < kMaxLists / kThreads; ++u) {
+        const uint32_t i = threadIdx.x + u * kThreads;
+        if (i >= lists) continue;
+        sm.head[i] = sm.offset[i / p.parts] + (double)mine[u];
+        top = larger(top, sm.head[i]);
     }
     const double kth = __shfl_sync(0xffffffffu, warp_sort(top, lane), k - 1);
-    if (lane == 0) warp_t[warp] = kth;
+    if (lane == 0) sm.warp_t[warp] = kth;
     __syncthreads();
-    double bound = warp_t[0];
-    for (uint32_t w = 1; w < kWarps; ++w) bound = larger(bound, warp_t[w]);
-    for (uint32_t i = threadIdx.x; i < lists; i += kThreads)
-        for (uint32_t j = 0; j < k; ++j) {
-            uint32_t token;
-            const double t = total(i, j, token);
-            if (!(t >= bound && t > -INFINITY)) break;
-            const uint32_t at = atomicAdd(&count, 1);
-            if (at < kFinalList) {
-                list_t[at] = t;
-                list_b[at] = i / p.parts;
-                list_i[at] = token;
-            }
+    double bound = sm.warp_t[0];
+    for (uint32_t w = 1; w < kWarps; ++w) bound = larger(bound, sm.warp_t[w]);
+    // a warp to a list that reaches it
+    for (uint32_t i = warp; i < lists; i += kWarps) {
+        if (!(sm.head[i] >= bound && sm.head[i] > -INFINITY) || lane >= k) continue;
+        const uint2 c = __ldcg(best + (size_t)i * k + lane);
+        const double t = sm.offset[i / p.parts] + (double)__uint_as_float(c.x);
+        if (!(t >= bound && t > -INFINITY)) continue;
+        const uint32_t at = atomicAdd(&sm.count, 1);
+        if (at < kList) {
+            sm.t[at] = t;
+            sm.b[at] = i / p.parts;
+            sm.i[at] = c.y;
         }
+    }
     __syncthreads();
-    const uint32_t n = count;
+    const uint32_t n = sm.count;
     float *const out_s = p.a.out_scores + (size_t)group * k;
     uint32_t *const out_b = p.a.out_beams + (size_t)group * k, *const out_t = p.a.out_tokens + (size_t)group * k;
-    if (n <= kFinalList) {
+    if (n <= kList) {
         for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-            const double t = list_t[i];
-            const uint32_t b = list_b[i], at = list_i[i];
+            const double t = sm.t[i];
+            const uint32_t b = sm.b[i], at = sm.i[i];
             uint32_t place = 0;
-            for (uint32_t j = 0; j < n; ++j) place += before(list_t[j], list_b[j], list_i[j], t, b, at);
+#pragma unroll 4
+            for (uint32_t j = 0; j < n; ++j) place += before(sm.t[j], sm.b[j], sm.i[j], t, b, at);
             if (place < k) {
                 out_s[place] = (float)t;
                 out_b[place] = b;
@@ -310,11 +337,10 @@ __global__ void __launch_bounds__(kThreads) beam_final_kernel(const __grid_const
         double t = -INFINITY;
         uint32_t b = kNone, at = kNone;
         for (uint32_t i = threadIdx.x; i < lists * k; i += kThreads) {
-            uint32_t token;
-            const double c = total(i / k, i % k, token);
+            const uint2 e = __ldcg(best + i);
             const uint32_t of = i / k / p.parts;
-            if (c > -INFINITY && (!place || before(last, last_b, last_i, c, of, token)) && before(c, of, token, t, b, at))
-                t = c, b = of, at = token;
+            const double c = sm.offset[of] + (double)__uint_as_float(e.x);
+            if (c > -INFINITY && (!place || before(last, last_b, last_i, c, of, e.y)) && before(c, of, e.y, t, b, at)) t = c, b = of, at = e.y;
         }
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) {
@@ -324,13 +350,13 @@ __global__ void __launch_bounds__(kThreads) beam_final_kernel(const __grid_const
         }
         __syncthreads();
         if (lane == 0) {
-            list_t[warp] = t;
-            list_b[warp] = b;
-            list_i[warp] = at;
+            sm.t[warp] = t;
+            sm.b[warp] = b;
+            sm.i[warp] = at;
         }
         __syncthreads();
         for (uint32_t w = 0; w < kWarps; ++w)
-            if (before(list_t[w], list_b[w], list_i[w], t, b, at)) t = list_t[w], b = list_b[w], at = list_i[w];
+            if (before(sm.t[w], sm.b[w], sm.i[w], t, b, at)) t = sm.t[w], b = sm.b[w], at = sm.i[w];
         if (threadIdx.x == 0) {
             out_s[place] = (float)t;
             out_b[place] = b;
@@ -340,6 +366,27 @@ __global__ void __launch_bounds__(kThreads) beam_final_kernel(const __grid_const
         last_b = b;
         last_i = at;
     }
+}
+
+__global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_constant__ BeamParams p)
+{
+    __shared__ Memory sm;
+    __shared__ bool last;
+    pdl_wait();
+    pdl_trigger();
+    part_of_row(p, sm.part, blockIdx.x, blockIdx.y);
+    // the request's last part to be there finds all the others
+    const uint32_t group = blockIdx.y / p.a.beams, parts = p.a.beams * p.parts;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(p.done + group, 1) == (int)parts - 1;
+        __threadfence();
+    }
+    __syncthreads();
+    if (!last) return;
+    if (threadIdx.x == 0) p.done[group] = 0;
+    parts_of_request(p, sm.all, group);
 }
 
 }  // namespace
@@ -358,20 +405,18 @@ int wr_beam_launch(wr_cuda_ctx *ctx, const wr_beam_args &a)
     p.a = a;
     const uint32_t rows = a.groups * a.beams, most = (uint32_t)(((uint64_t)a.vocab + 3 + kBatch - 1) / kBatch);
     // four CTAs to an SM are enough to keep its loads under way
-    const uint32_t want = std::min(std::max(4u * (uint32_t)ctx->sm_count / rows, 1u), most);
+    const uint32_t want = std::min(std::max(4u * (uint32_t)ctx->sm_count / rows, 1u), std::min(most, kMaxLists / a.beams));
     p.batches = (most + want - 1) / want;
     p.parts = (most + p.batches - 1) / p.batches;
     const size_t n = (size_t)rows * p.parts, sums = (n * sizeof(float2) + 255) & ~(size_t)255;
     char *ws = nullptr;
     int rc = wr_ctx_keep(ctx, WR_KEPT_HEAD + sums + n * a.n_out * sizeof(uint2), &ws);
     if (rc != WR_CUDA_OK) return rc;
+    p.done = reinterpret_cast<int *>(ws + WR_KEPT_HEAD / 2);
     p.sums = reinterpret_cast<float2 *>(ws + WR_KEPT_HEAD);
     p.best = reinterpret_cast<uint2 *>(ws + WR_KEPT_HEAD + sums);
-    WR_CUDA_TRY(wr_launch_pdl(beam_part_kernel, dim3(p.parts, rows), dim3(kThreads), (size_t)0, ctx->stream, p));
-    WR_CUDA_TRY(wr_launch_pdl(beam_final_kernel, dim3(a.groups), dim3(kThreads), (size_t)0, ctx->stream, p));
-    ctx->launches += 2;
-    WR_CUDA_TRY(cudaGetLastError());
-    return WR_CUDA_OK;
+    WR_CUDA_TRY(wr_launch_pdl(beam_select_kernel, dim3(p.parts, rows), dim3(kThreads), (size_t)0, ctx->stream, p));
+    return finish_launch(ctx);
 }
 
 extern "C" int wr_cuda_beam_select(wr_cuda_ctx *ctx, uint32_t n_groups, uint32_t beams, uint32_t vocab, const float *logits,

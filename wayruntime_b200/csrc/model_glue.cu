@@ -838,7 +838,7 @@ int wr_beam_step_launch(wr_cuda_ctx *ctx, wr_cuda_model *m, const wr_beam_step &
     WR_CUDA_TRY(cudaMemcpyAsync(m->beam_dev, m->beam_host, rows * 4, cudaMemcpyHostToDevice, ctx->stream));
     const int rc = wr_beam_launch(ctx, a);
     if (rc != WR_CUDA_OK) return rc;
-    m->launches += 2;
+    ++m->launches;
     WR_CUDA_TRY(cudaMemcpyAsync(m->beam_host + WR_CUDA_BATCH_MAX, a.out_scores, outs * 12, cudaMemcpyDeviceToHost, ctx->stream));
     return WR_CUDA_OK;
 }

@@ -227,8 +227,9 @@ int wr_ctx_reserve_ws(wr_cuda_ctx *ctx, size_t ws_bytes, size_t tickets);
 // The workspace for callers that can do without: where memory does not suffice it stays as it is, and nothing waits.
 int wr_ctx_try_ws(wr_cuda_ctx *ctx, size_t ws_bytes);
 // Scratch that stays where it is for the context's life: a larger call gets more, elsewhere.  Its first WR_KEPT_HEAD bytes are
-// counters that every launch leaves as zeros (and wr_ctx_sync_checked makes zeros again when a kernel has given up).
-#define WR_KEPT_HEAD (64u << 10)
+// counters that every launch leaves as zeros (and wr_ctx_sync_checked makes zeros again when a kernel has given up): shared
+// attention's in the first half, those of 65536 requests' beams in the second.
+#define WR_KEPT_HEAD (512u << 10)
 int wr_ctx_keep(wr_cuda_ctx *ctx, size_t bytes, char **out);
 int wr_kv_batch_check(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer);
 int wr_append_validate(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer,
