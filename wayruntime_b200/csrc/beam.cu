@@ -8,19 +8,22 @@
 // since candidates of two beams may lie closer than an F32 rounding.  HBM bounds it (4 bytes a logit) where there are many
 // rows, round trips where there are few; a second kernel for the parts took 2 us more.
 //
-// Candidates are found with a threshold that is sure to keep n_out of them: of 32 lanes' maxima (distinct elements) the
+// Candidates are found with a threshold that is sure to keep n_out of them: of 32 threads' maxima (distinct elements) the
 // n_out-th largest.  What reaches it goes to a list, what still reaches the last threshold to another, and an entry's place in
 // the result is the number of better ones there.  Where a list runs over (rows of few values) the best are taken one after the
 // other instead.
 // Ties go to the lower beam, then the lower token.  Logits of -inf are no candidates, nor is anything of a beam whose score is
 // -inf or NaN (its row is not read) or whose sum is not finite (a NaN or +inf among its logits).
+#include <cfloat>
+
 #include "kv_share.cuh"
 #include "rows_dev.cuh"
 
 namespace {
 
 constexpr uint32_t kThreads = 256, kWarps = kThreads / 32, kVecs = 4, kBatch = kThreads * kVecs * 4;   // logits a CTA has in hand
-constexpr uint32_t kList = 1024, kMaxLists = 1024;
+constexpr uint32_t kList = 1024, kOwn = 6, kMaxLists = kOwn * kThreads;       // kOwn: a thread's entries of a request's
+constexpr uint32_t kCtas = 4;             // to an SM
 constexpr uint32_t kNone = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -33,13 +36,15 @@ struct BeamParams {
 };
 // A CTA's shared memory: while it works on its part, and on a request's parts.
 struct PartMemory {
-    float v[kList], lane_top[kThreads], warp_m[kWarps], warp_s[kWarps], kept_v[kList];
-    uint32_t i[kList], kept_i[kList], count, kept;
-    int least;                           // the threshold, as a whole number in the order of floats
+    uint64_t listed[kList], kept[kList]; // keys
+    float top[2][32], warp_m[kWarps], warp_s[kWarps];
+    uint32_t n_listed, n_kept;
 };
 struct FinalMemory {
-    double offset[WR_CUDA_BATCH_MAX], head[kMaxLists], t[kList], warp_t[kWarps];
-    uint32_t b[kList], i[kList], count;
+    double offset[WR_CUDA_BATCH_MAX];
+    float top[32];
+    uint64_t t[kList], at[kList];        // totals in the order of whole numbers; beam and token
+    uint32_t n;
 };
 union Memory {
     PartMemory part;
@@ -66,18 +71,64 @@ template <typename T> __device__ __forceinline__ T warp_sort(T v, uint32_t lane)
         }
     return v;
 }
-// the better of two candidates
-__device__ __forceinline__ bool before(float v, uint32_t i, float w, uint32_t j) { return v > w || (v == w && i < j); }
-
 __device__ __forceinline__ const float *row_of(const wr_beam_args &a, uint32_t r) { return a.logits + (size_t)(a.mapped ? a.map[r] : r) * a.ld; }
 
-// a < b in the order of results: the logit or total, then the beam, then the token
-__device__ __forceinline__ bool before(double v, uint32_t b, uint32_t i, double w, uint32_t c, uint32_t j)
-{
-    return v > w || (v == w && (b < c || (b == c && i < j)));
-}
 __device__ __forceinline__ int order(float v) { const int i = __float_as_int(v); return i ^ ((i >> 31) & 0x7fffffff); }
 __device__ __forceinline__ float value(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
+// A row's candidate as one number, the better the larger: the logit, then the lower token.  (-0 and 0 are equal.)
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t token)
+{
+    return (uint64_t)((uint32_t)order(v + 0.f) ^ 0x80000000u) << 32 | (uint32_t)~token;
+}
+__device__ __forceinline__ float logit_of(uint64_t key) { return value((int)((uint32_t)(key >> 32) ^ 0x80000000u)); }
+__device__ __forceinline__ uint64_t key_of(double t)
+{
+    const long long i = __double_as_longlong(t + 0.0);
+    return (uint64_t)(i ^ ((i >> 63) & 0x7fffffffffffffffll)) ^ 0x8000000000000000ull;
+}
+__device__ __forceinline__ double total_of(uint64_t key)
+{
+    const long long i = (long long)(key ^ 0x8000000000000000ull);
+    return __longlong_as_double(i ^ ((i >> 63) & 0x7fffffffffffffffll));
+}
+// The places of n entries in their order, by counting the better ones; eight threads to an entry.
+template <typename Better, typename Place> __device__ __forceinline__ void rank(uint32_t n, Better better, Place place)
+{
+    const uint32_t sub = threadIdx.x & 7;
+    for (uint32_t i0 = 0; i0 < n; i0 += kThreads / 8) {
+        const uint32_t i = i0 + threadIdx.x / 8;
+        uint32_t count = 0;
+        if (i < n) {
+#pragma unroll 4
+            for (uint32_t j = sub; j < n; j += 8) count += better(j, i);
+        }
+#pragma unroll
+        for (int o = 4; o >= 1; o >>= 1) count += __shfl_xor_sync(0xffffffffu, count, o);
+        if (i < n && sub == 0) place(i, count);
+    }
+}
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// A number that k of all threads' values reach: of every warp's four largest, 32 together, the k-th.  (One that k of a warp's own reach
+// lets eight times as many through.)  The CTA meets in it; `top` is not used again before it has met once more.
+static_assert(kWarps * 4 == 32, "");
+__device__ __forceinline__ float bound_of_all(float (&top)[32], float v, uint32_t k, uint32_t warp, uint32_t lane)
+{
+    const float sorted = warp_sort(v, lane);
+    if (lane < 4) top[4 * warp + lane] = sorted;
+    __syncthreads();
+    return __shfl_sync(0xffffffffu, warp_sort(top[lane], lane), k - 1);
+}
 // sums of exponentials against two maxima as one
 __device__ __forceinline__ void join(float &m, float &s, float m2, float s2)
 {
@@ -99,85 +150,75 @@ __device__ __forceinline__ void part_of_row(const BeamParams &p, PartMemory &sm,
     // Vectors are aligned in memory: the row begins `lead` elements into the first one.
     const float *const x = row_of(p.a, row);
     const uint32_t lead = (uint32_t)((uintptr_t)x >> 2) & 3u;
-    const uint64_t first = (uint64_t)part * p.batches * kBatch, end = (uint64_t)p.a.vocab + lead;
+    const float *const aligned = x - lead;
+    const uint32_t first = part * p.batches * kBatch, end = p.a.vocab + lead;      // (below 2^32: a vocabulary is below 2^31)
     auto load = [&](uint32_t b, float (&v)[4 * kVecs]) {
+        const uint32_t lo = first + b * kBatch;
+        if (lo && lo + kBatch <= end) {
+#pragma unroll
+            for (uint32_t u = 0; u < kVecs; ++u) {
+                const float4 w = __ldcs(reinterpret_cast<const float4 *>(aligned + lo) + u * kThreads + threadIdx.x);
+                v[4 * u] = w.x; v[4 * u + 1] = w.y; v[4 * u + 2] = w.z; v[4 * u + 3] = w.w;
+            }
+            return;
+        }
 #pragma unroll
         for (uint32_t u = 0; u < kVecs; ++u) {
-            const uint64_t at = first + (uint64_t)b * kBatch + (u * kThreads + threadIdx.x) * 4u;
+            const uint32_t at = lo + (u * kThreads + threadIdx.x) * 4u;
             if (at >= lead && at + 4 <= end) {
-                const float4 w = __ldcs(reinterpret_cast<const float4 *>(x + (at - lead)));
+                const float4 w = __ldcs(reinterpret_cast<const float4 *>(aligned + at));
                 v[4 * u] = w.x; v[4 * u + 1] = w.y; v[4 * u + 2] = w.z; v[4 * u + 3] = w.w;
             } else {
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) v[4 * u + e] = at + e >= lead && at + e < end ? __ldcs(x + (at + e - lead)) : -INFINITY;
+                for (uint32_t e = 0; e < 4; ++e) v[4 * u + e] = at + e >= lead && at + e < end ? __ldcs(aligned + at + e) : -INFINITY;
             }
         }
     };
-    auto token_of = [&](uint32_t b, uint32_t e) {
-        return (uint32_t)(first + (uint64_t)b * kBatch + ((e / 4) * kThreads + threadIdx.x) * 4u + (e & 3) - lead);
-    };
-    float v[4 * kVecs], next[4 * kVecs], m = -INFINITY, s = 0.f;
+    auto token_of = [&](uint32_t b, uint32_t e) { return first + b * kBatch + ((e / 4) * kThreads + threadIdx.x) * 4u + (e & 3) - lead; };
+    float v[4 * kVecs], next[4 * kVecs], m = -INFINITY, bound = -FLT_MAX;
+    uint64_t s2 = 0;                     // two sums of exponentials
     load(0, v);
     if (threadIdx.x == 0) {
-        sm.count = sm.kept = 0;
-        sm.least = order(-INFINITY);
+        sm.n_listed = sm.n_kept = 0;
     }
     __syncthreads();
-    for (uint32_t b = 0; b < p.batches; ++b) {
-        if (first + (uint64_t)b * kBatch >= end) break;
-        if (b + 1 < p.batches) load(b + 1, next);
+    const uint32_t batches = first < end ? min(p.batches, (end - first + kBatch - 1) / kBatch) : 0u;
+    for (uint32_t b = 0; b < batches; ++b) {
+        if (b + 1 < batches) load(b + 1, next);
         float top = -INFINITY;
 #pragma unroll
-        for (uint32_t e = 0; e < 4 * kVecs; ++e) top = fmaxf(top, v[e]);
+        for (uint32_t e = 0; e < 4 * kVecs; e += 2) top = max3(top, v[e], v[e + 1]);
         const float was = m;
         m = fmaxf(m, top);
-        const float base = m == -INFINITY ? 0.f : m;
-        s *= ex2((was - base) * kLog2e);
+        const float base = m == -INFINITY ? 0.f : m, shrink = ex2((was - base) * kLog2e);
+        s2 = mul2(s2, pack2(shrink, shrink));
 #pragma unroll
-        for (uint32_t e = 0; e < 4 * kVecs; ++e) s += ex2((v[e] - base) * kLog2e);
-        // A threshold from what every lane has seen.  (Of more than 16, a warp's lanes alone let too many through: the first batch
-        // asks all the CTA's.)
-        float bound;
-        if (k > 16 && b == 0) {
-            sm.lane_top[threadIdx.x] = m;
-            __syncthreads();
-            uint32_t larger_ones = 0;
-            for (uint32_t i = 0; i < kThreads; i += 4) {
-                const float4 w = *reinterpret_cast<const float4 *>(sm.lane_top + i);
-                larger_ones += (w.x > m || (w.x == m && i < threadIdx.x)) + (w.y > m || (w.y == m && i + 1 < threadIdx.x)) +
-                               (w.z > m || (w.z == m && i + 2 < threadIdx.x)) + (w.w > m || (w.w == m && i + 3 < threadIdx.x));
-            }
-            if (larger_ones == k - 1) sm.least = order(m);
-            __syncthreads();
-            bound = value(sm.least);
-        } else {
-            // (a warp's threshold moves when one of its lanes' maxima does)
-            if (__any_sync(0xffffffffu, m > was)) {
-                const float kth = __shfl_sync(0xffffffffu, warp_sort(m, lane), k - 1);
-                if (lane == 0) atomicMax(&sm.least, order(kth));
-            }
-            if (b == 0) __syncthreads();
-            bound = value(*(volatile int *)&sm.least);           // (whichever warps have answered: any of their bounds is one)
+        for (uint32_t e = 0; e < 4 * kVecs; e += 2) {
+            float d0, d1;
+            unpack2(mul2(add2(pack2(v[e], v[e + 1]), pack2(-base, -base)), pack2(kLog2e, kLog2e)), d0, d1);
+            s2 = add2(s2, pack2(ex2(d0), ex2(d1)));
         }
+        // a threshold from what every thread has seen, looked for again whenever that has doubled
+        if ((b & (b + 1)) == 0) bound = fmaxf(bound_of_all(sm.top[b & 1], m, k, warp, lane), -FLT_MAX);
         if (top >= bound) {
 #pragma unroll
             for (uint32_t e = 0; e < 4 * kVecs; ++e)
-                if (v[e] >= bound && v[e] > -INFINITY) {
-                    const uint32_t at = atomicAdd(&sm.count, 1);
-                    if (at < kList) {
-                        sm.v[at] = v[e];
-                        sm.i[at] = token_of(b, e);
-                    }
+                if (v[e] >= bound) {
+                    const uint32_t at = atomicAdd(&sm.n_listed, 1);
+                    if (at < kList) sm.listed[at] = key_of(v[e], token_of(b, e));
                 }
         }
 #pragma unroll
         for (uint32_t e = 0; e < 4 * kVecs; ++e) v[e] = next[e];
     }
     // the part's sum: lanes, then warps, in order
+    float s, half;
+    unpack2(s2, s, half);
+    s += half;
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-        join(m, s, m2, s2);
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), other = __shfl_xor_sync(0xffffffffu, s, o);
+        join(m, s, m2, other);
     }
     if (lane == 0) {
         sm.warp_m[warp] = m;
@@ -188,64 +229,42 @@ __device__ __forceinline__ void part_of_row(const BeamParams &p, PartMemory &sm,
         for (uint32_t w = 1; w < kWarps; ++w) join(m, s, sm.warp_m[w], sm.warp_s[w]);
         p.sums[(size_t)row * p.parts + part] = make_float2(m, s);
     }
-    const uint32_t listed = sm.count;
-    if (listed <= kList) {
-        const float bound = value(sm.least);                     // (it has grown since most entries were listed)
-        for (uint32_t i = threadIdx.x; i < listed; i += kThreads)
-            if (sm.v[i] >= bound) {
-                const uint32_t at = atomicAdd(&sm.kept, 1);
-                sm.kept_v[at] = sm.v[i];
-                sm.kept_i[at] = sm.i[i];
-            }
-        __syncthreads();
-        const uint32_t n = sm.kept;
-        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-            const float w = sm.kept_v[i];
-            const uint32_t at = sm.kept_i[i];
-            uint32_t place = 0;
-#pragma unroll 4
-            for (uint32_t j = 0; j < n; ++j) place += before(sm.kept_v[j], sm.kept_i[j], w, at);
-            if (place < k) best[place] = make_uint2(__float_as_uint(w), at);
+    uint32_t n = sm.n_listed;
+    if (n <= kList) {
+        const uint64_t *list = sm.listed;
+        if (batches > 1) {                                       // (as many comparisons to an entry as there are entries: fewer first)
+            const uint64_t least = key_of(bound, kNone);
+            for (uint32_t i = threadIdx.x; i < n; i += kThreads)
+                if (sm.listed[i] >= least) sm.kept[atomicAdd(&sm.n_kept, 1)] = sm.listed[i];
+            __syncthreads();
+            n = sm.n_kept;
+            list = sm.kept;
         }
+        rank(n, [&](uint32_t j, uint32_t i) { return list[j] > list[i]; },
+             [&](uint32_t i, uint32_t place) { if (place < k) best[place] = make_uint2(__float_as_uint(logit_of(list[i])), ~(uint32_t)list[i]); });
         if (threadIdx.x >= n && threadIdx.x < k) best[threadIdx.x] = make_uint2(__float_as_uint(-INFINITY), kNone);
         return;
     }
     // too many for the list: the largest, then the largest behind it, and so on
-    float last_v = INFINITY;
-    uint32_t last_i = 0;
-    bool started = false;
+    uint64_t last = ~0ull;
     for (uint32_t j = 0; j < k; ++j) {
-        float top_v = -INFINITY;
-        uint32_t top_i = kNone;
-        for (uint32_t b = 0; b < p.batches; ++b) {
+        uint64_t most = 0;
+        for (uint32_t b = 0; b < batches; ++b) {
             load(b, v);
 #pragma unroll
             for (uint32_t e = 0; e < 4 * kVecs; ++e) {
-                const uint32_t at = token_of(b, e);
-                if (v[e] > -INFINITY && (!started || before(last_v, last_i, v[e], at)) && before(v[e], at, top_v, top_i)) {
-                    top_v = v[e];
-                    top_i = at;
-                }
+                const uint64_t key = key_of(v[e], token_of(b, e));
+                if (v[e] > -INFINITY && key < last && key > most) most = key;
             }
         }
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) {
-            const float w = __shfl_xor_sync(0xffffffffu, top_v, o);
-            const uint32_t at = __shfl_xor_sync(0xffffffffu, top_i, o);
-            if (before(w, at, top_v, top_i)) top_v = w, top_i = at;
-        }
+        for (int o = 16; o >= 1; o >>= 1) most = larger(most, (uint64_t)__shfl_xor_sync(0xffffffffu, (unsigned long long)most, o));
         __syncthreads();
-        if (lane == 0) {
-            sm.v[warp] = top_v;
-            sm.i[warp] = top_i;
-        }
+        if (lane == 0) sm.listed[warp] = most;
         __syncthreads();
-        for (uint32_t w = 0; w < kWarps; ++w)
-            if (before(sm.v[w], sm.i[w], top_v, top_i)) top_v = sm.v[w], top_i = sm.i[w];
-        if (threadIdx.x == 0) best[j] = make_uint2(__float_as_uint(top_v), top_i);
-        started = true;
-        last_v = top_v;
-        last_i = top_i;
+        for (uint32_t w = 0; w < kWarps; ++w) most = larger(most, sm.listed[w]);
+        if (threadIdx.x == 0) best[j] = most ? make_uint2(__float_as_uint(logit_of(most)), ~(uint32_t)most) : make_uint2(__float_as_uint(-INFINITY), kNone);
+        last = most;
     }
 }
 
@@ -255,120 +274,110 @@ __device__ __forceinline__ void parts_of_request(const BeamParams &p, FinalMemor
     const size_t row0 = (size_t)group * beams;
     const uint32_t lists = beams * p.parts;
     const uint2 *const best = p.best + row0 * p.parts * k;
-    // every list's best, on its way while the sums are put together
-    float mine[(kMaxLists + kThreads - 1) / kThreads];
+    // Few candidates: all of them are on their way while the sums are put together.  Many: the first of every list.
+    const bool few = lists * k <= kOwn * kThreads;
+    uint2 mine[kOwn];
 #pragma unroll
-    for (uint32_t u = 0; u < kMaxLists / kThreads; ++u) {
+    for (uint32_t u = 0; u < kOwn; ++u) {
         const uint32_t i = threadIdx.x + u * kThreads;
-        if (i < lists) mine[u] = __uint_as_float(__ldcg(&best[(size_t)i * k].x));
+        mine[u] = make_uint2(__float_as_uint(-INFINITY), kNone);
+        if (i < (few ? lists * k : lists)) mine[u] = __ldcg(best + (few ? i : (size_t)i * k));
     }
-    if (threadIdx.x == 0) sm.count = 0;
+    if (threadIdx.x == 0) sm.n = 0;
     // score less the logarithm of the row's sum
     for (uint32_t b = warp; b < beams; b += kWarps) {
-        const float2 *sums = p.sums + (row0 + b) * p.parts;
-        float top = -INFINITY;
-        for (uint32_t i = lane; i < p.parts; i += 32) top = fmaxf(top, __ldcg(sums + i).x);
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        double s = 0.0;
+        float m = -INFINITY, s = 0.f;
         for (uint32_t i = lane; i < p.parts; i += 32) {
-            const float2 ms = __ldcg(sums + i);
-            if (ms.y != 0.f) s += (double)ms.y * exp((double)ms.x - (double)top);
-        }
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        const double t = (double)p.a.scores[row0 + b] - ((double)top + log(s));
-        if (lane == 0) sm.offset[b] = t > -INFINITY && t < INFINITY ? t : -INFINITY;         // (no sum, or none that is finite)
-    }
-    __syncthreads();
-    // a bound from 32 threads' best
-    double top = -INFINITY;
-#pragma unroll
-    for (uint32_t u = 0; u < kMaxLists / kThreads; ++u) {
-        const uint32_t i = threadIdx.x + u * kThreads;
-        if (i >= lists) continue;
-        sm.head[i] = sm.offset[i / p.parts] + (double)mine[u];
-        top = larger(top, sm.head[i]);
-    }
-    const double kth = __shfl_sync(0xffffffffu, warp_sort(top, lane), k - 1);
-    if (lane == 0) sm.warp_t[warp] = kth;
-    __syncthreads();
-    double bound = sm.warp_t[0];
-    for (uint32_t w = 1; w < kWarps; ++w) bound = larger(bound, sm.warp_t[w]);
-    // a warp to a list that reaches it
-    for (uint32_t i = warp; i < lists; i += kWarps) {
-        if (!(sm.head[i] >= bound && sm.head[i] > -INFINITY) || lane >= k) continue;
-        const uint2 c = __ldcg(best + (size_t)i * k + lane);
-        const double t = sm.offset[i / p.parts] + (double)__uint_as_float(c.x);
-        if (!(t >= bound && t > -INFINITY)) continue;
-        const uint32_t at = atomicAdd(&sm.count, 1);
-        if (at < kList) {
-            sm.t[at] = t;
-            sm.b[at] = i / p.parts;
-            sm.i[at] = c.y;
-        }
-    }
-    __syncthreads();
-    const uint32_t n = sm.count;
-    float *const out_s = p.a.out_scores + (size_t)group * k;
-    uint32_t *const out_b = p.a.out_beams + (size_t)group * k, *const out_t = p.a.out_tokens + (size_t)group * k;
-    if (n <= kList) {
-        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-            const double t = sm.t[i];
-            const uint32_t b = sm.b[i], at = sm.i[i];
-            uint32_t place = 0;
-#pragma unroll 4
-            for (uint32_t j = 0; j < n; ++j) place += before(sm.t[j], sm.b[j], sm.i[j], t, b, at);
-            if (place < k) {
-                out_s[place] = (float)t;
-                out_b[place] = b;
-                out_t[place] = at;
-            }
-        }
-        if (threadIdx.x >= n && threadIdx.x < k) {
-            out_s[threadIdx.x] = -INFINITY;
-            out_b[threadIdx.x] = out_t[threadIdx.x] = kNone;
-        }
-        return;
-    }
-    double last = INFINITY;
-    uint32_t last_b = 0, last_i = 0;
-    for (uint32_t place = 0; place < k; ++place) {
-        double t = -INFINITY;
-        uint32_t b = kNone, at = kNone;
-        for (uint32_t i = threadIdx.x; i < lists * k; i += kThreads) {
-            const uint2 e = __ldcg(best + i);
-            const uint32_t of = i / k / p.parts;
-            const double c = sm.offset[of] + (double)__uint_as_float(e.x);
-            if (c > -INFINITY && (!place || before(last, last_b, last_i, c, of, e.y)) && before(c, of, e.y, t, b, at)) t = c, b = of, at = e.y;
+            const float2 ms = __ldcg(p.sums + (row0 + b) * p.parts + i);
+            join(m, s, ms.x, ms.y);
         }
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) {
-            const double c = __shfl_xor_sync(0xffffffffu, t, o);
-            const uint32_t of = __shfl_xor_sync(0xffffffffu, b, o), token = __shfl_xor_sync(0xffffffffu, at, o);
-            if (before(c, of, token, t, b, at)) t = c, b = of, at = token;
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+            join(m, s, m2, s2);
+        }
+        const double t = (double)p.a.scores[row0 + b] - ((double)m + log((double)s));
+        if (lane == 0) sm.offset[b] = t > -INFINITY && t < INFINITY ? t : -INFINITY;         // (no sum, or none that is finite)
+    }
+    __syncthreads();
+    // a bound from the threads' best, rounded down
+    const uint32_t per_beam = few ? p.parts * k : p.parts;
+    double total[kOwn], top = -INFINITY;
+#pragma unroll
+    for (uint32_t u = 0; u < kOwn; ++u) {
+        const uint32_t i = threadIdx.x + u * kThreads;
+        total[u] = i < beams * per_beam ? sm.offset[i / per_beam] + (double)__uint_as_float(mine[u].x) : -INFINITY;
+        top = larger(top, total[u]);
+    }
+    const float bound = fmaxf(bound_of_all(sm.top, __double2float_rd(top), k, warp, lane), -FLT_MAX);
+    auto list = [&](double t, uint32_t b, uint32_t token) {
+        if (!(t >= bound)) return;
+        const uint32_t at = atomicAdd(&sm.n, 1);
+        if (at >= kList) return;
+        sm.t[at] = key_of(t);
+        sm.at[at] = (uint64_t)b << 32 | token;
+    };
+#pragma unroll
+    for (uint32_t u = 0; u < kOwn; ++u) {
+        const uint32_t i = threadIdx.x + u * kThreads, b = i / per_beam;
+        if (few) {
+            list(total[u], b, mine[u].y);
+        } else if (total[u] >= bound) {                          // (whose list begins above it takes all of the list)
+            const double offset = sm.offset[b];
+#pragma unroll 8
+            for (uint32_t j = 0; j < k; ++j) {
+                const uint2 c = __ldcg(best + (size_t)i * k + j);
+                list(offset + (double)__uint_as_float(c.x), b, c.y);
+            }
+        }
+    }
+    __syncthreads();
+    const uint32_t n = sm.n;
+    float *const out_s = p.a.out_scores + (size_t)group * k;
+    uint32_t *const out_b = p.a.out_beams + (size_t)group * k, *const out_t = p.a.out_tokens + (size_t)group * k;
+    auto put = [&](uint32_t place, uint64_t t, uint64_t at) {
+        out_s[place] = at == ~0ull ? -INFINITY : (float)total_of(t);
+        out_b[place] = (uint32_t)(at >> 32);
+        out_t[place] = (uint32_t)at;
+    };
+    if (n <= kList) {
+        rank(n, [&](uint32_t j, uint32_t i) { return (sm.t[j] > sm.t[i]) | ((sm.t[j] == sm.t[i]) & (sm.at[j] < sm.at[i])); },
+             [&](uint32_t i, uint32_t place) { if (place < k) put(place, sm.t[i], sm.at[i]); });
+        if (threadIdx.x >= n && threadIdx.x < k) put(threadIdx.x, 0, ~0ull);
+        return;
+    }
+    // more equal ones than a list holds: one after the other
+    uint64_t last = ~0ull, last_at = 0;
+    for (uint32_t place = 0; place < k; ++place) {
+        uint64_t most = 0, at = ~0ull;
+        auto take = [&](uint64_t t, uint64_t of) {
+            if (t > most || (t == most && of < at)) most = t, at = of;
+        };
+        for (uint32_t i = threadIdx.x; i < lists * k; i += kThreads) {
+            const uint2 c = __ldcg(best + i);
+            const double t = sm.offset[i / k / p.parts] + (double)__uint_as_float(c.x);
+            const uint64_t key = key_of(t), of = (uint64_t)(i / k / p.parts) << 32 | c.y;
+            if (t > -INFINITY && (!place || key < last || (key == last && of > last_at))) take(key, of);
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) {
+            const uint64_t t = __shfl_xor_sync(0xffffffffu, (unsigned long long)most, o), of = __shfl_xor_sync(0xffffffffu, (unsigned long long)at, o);
+            take(t, of);
         }
         __syncthreads();
         if (lane == 0) {
-            sm.t[warp] = t;
-            sm.b[warp] = b;
-            sm.i[warp] = at;
+            sm.t[warp] = most;
+            sm.at[warp] = at;
         }
         __syncthreads();
-        for (uint32_t w = 0; w < kWarps; ++w)
-            if (before(sm.t[w], sm.b[w], sm.i[w], t, b, at)) t = sm.t[w], b = sm.b[w], at = sm.i[w];
-        if (threadIdx.x == 0) {
-            out_s[place] = (float)t;
-            out_b[place] = b;
-            out_t[place] = at;
-        }
-        last = t;
-        last_b = b;
-        last_i = at;
+        for (uint32_t w = 0; w < kWarps; ++w) take(sm.t[w], sm.at[w]);
+        if (threadIdx.x == 0) put(place, most, at);
+        last = most;
+        last_at = at;
     }
 }
 
-__global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_constant__ BeamParams p)
+__global__ void __launch_bounds__(kThreads, kCtas) beam_select_kernel(const __grid_constant__ BeamParams p)
 {
     __shared__ Memory sm;
     __shared__ bool last;
@@ -379,9 +388,9 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_cons
     const uint32_t group = blockIdx.y / p.a.beams, parts = p.a.beams * p.parts;
     __syncthreads();
     if (threadIdx.x == 0) {
-        __threadfence();
-        last = atomicAdd(p.done + group, 1) == (int)parts - 1;
-        __threadfence();
+        int before;
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.done + group) : "memory");
+        last = before == (int)parts - 1;
     }
     __syncthreads();
     if (!last) return;
@@ -404,8 +413,7 @@ int wr_beam_launch(wr_cuda_ctx *ctx, const wr_beam_args &a)
     BeamParams p{};
     p.a = a;
     const uint32_t rows = a.groups * a.beams, most = (uint32_t)(((uint64_t)a.vocab + 3 + kBatch - 1) / kBatch);
-    // four CTAs to an SM are enough to keep its loads under way
-    const uint32_t want = std::min(std::max(4u * (uint32_t)ctx->sm_count / rows, 1u), std::min(most, kMaxLists / a.beams));
+    const uint32_t want = std::min(std::max(kCtas * (uint32_t)ctx->sm_count / rows, 1u), std::min(most, kMaxLists / a.beams));
     p.batches = (most + want - 1) / want;
     p.parts = (most + p.batches - 1) / p.batches;
     const size_t n = (size_t)rows * p.parts, sums = (n * sizeof(float2) + 255) & ~(size_t)255;
