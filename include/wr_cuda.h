@@ -277,12 +277,13 @@ int wr_cuda_attn_decode_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *co
                                const uint32_t *group_rows, const float *q, float *out,
                                uint32_t n_q_heads, float scale_override, int mem);
 
-/* wr_cuda_decode_step for such sessions: wr_cuda_kv_append with n_tokens = 1, then
- * wr_cuda_attn_decode_shared over positions[s] + 1 rows; group_rows[g] is at most the
- * smallest position.  Host q rows are left as given. */
+/* wr_cuda_decode_step for such sessions, in one kernel: what wr_cuda_kv_append with
+ * n_tokens = 1 stores, and wr_cuda_attn_decode_shared over positions[s] + 1 rows with the
+ * rotated queries; group_rows[g] is at most the smallest position.  The q rows are left as
+ * given, wherever they are. */
 int wr_cuda_decode_step_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer,
                                const uint32_t *positions, uint32_t n_groups, const uint32_t *group_sess,
-                               const uint32_t *group_rows, float *q, const float *k_rows,
+                               const uint32_t *group_rows, const float *q, const float *k_rows,
                                const float *v_rows, float *out, uint32_t n_q_heads, float theta_base,
                                uint32_t n_rot_pairs, uint32_t flags, float scale_override, int mem);
 

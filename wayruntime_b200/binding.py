@@ -498,7 +498,8 @@ class Context:
 
     def decode_step_shared(self, kvs, layer, positions, groups, q, k_rows, v_rows, out, n_q_heads, theta=10000.0,
                            n_rot_pairs=0, rope=True, scale=0.0):
-        """wr_cuda_decode_step_shared: decode_step for sessions that share their first rows (groups as in attn_decode_shared)."""
+        """wr_cuda_decode_step_shared: decode_step for sessions that share their first rows (groups as in attn_decode_shared);
+        the rows of q are left as given."""
         qp, qm, _q = _buf(q)
         kp, km, _k = _buf(k_rows)
         vp, vm, _v = _buf(v_rows)

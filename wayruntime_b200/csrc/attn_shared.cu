@@ -31,6 +31,7 @@
 #include <type_traits>
 
 #include "kv_share.cuh"
+#include "mathx_dev.cuh"
 #include "tcgen05_dev.cuh"
 #include "warp_reduce.cuh"
 
@@ -48,15 +49,32 @@ constexpr float kGrow = 8.0f, kLog2e = 1.4426950408889634f;
 struct Bundle {
     uint32_t group, row0, sessions;      // its group; its first session, how many
     uint32_t head0, heads;               // which of a kv head's query heads
-    uint32_t tiles, chunks, item0, part0;
+    uint32_t shared, tiles, chunks, item0, part0;        // tiles: all of them, the shared ones first
 };
+// Where share i of a bundle's tiles begins.  An own tile's work counts five quarters of a shared one's: 2.0 us against the 1.55 that
+// HBM needs for it (16 sessions behind 32768 rows: 39.8 us with even numbers).
+__host__ __device__ __forceinline__ uint32_t weight_of(uint32_t shared, uint32_t tiles) { return 4 * shared + 5 * (tiles - shared); }
+// (Shares of a weight of five at least have a tile each; or there are as many as tiles.)
+__host__ __device__ __forceinline__ uint32_t shares_of(uint32_t shared, uint32_t tiles, uint32_t share)
+{
+    const uint32_t w = weight_of(shared, tiles), n = (w + share - 1) / share;
+    return n >= tiles ? tiles : n < w / 5 ? n : w / 5;
+}
+__host__ __device__ __forceinline__ uint32_t share_at(const Bundle &b, uint32_t i)
+{
+    if (b.chunks == b.tiles) return i;
+    const uint32_t w = weight_of(b.shared, b.tiles) * i / b.chunks;        // (2.7 million at most, times 592 at most)
+    return w < 4 * b.shared ? (w + 2) / 4 : b.shared + (w - 4 * b.shared + 2) / 5;
+}
 struct SharedParams {
     Bundle bundle[kMaxBundles];
     const uint64_t *shared_pages[WR_CUDA_BATCH_MAX], *own_pages[WR_CUDA_BATCH_MAX];      // of a group; of a session, from its own rows on
     uint32_t shared_rows[WR_CUDA_BATCH_MAX], own_rows[WR_CUDA_BATCH_MAX];
     uint8_t first_bundle[WR_CUDA_BATCH_MAX];     // of a session; the next ones have its further heads
     uint32_t n_bundles, items, rows, n_q, n_kv, per;     // rows: of the result; per: query heads to a kv head
-    const float *q;
+    const float *q, *k_new, *v_new;      // k_new: null where nothing is appended
+    float theta;
+    uint32_t n_rot;                      // pairs that new keys and the queries are rotated by; 0: none
     float *out;
     float2 *ml;                          // [part]: reference (log2), sum
     float *o;                            // [part][128]
@@ -64,6 +82,7 @@ struct SharedParams {
     int *done;                           // [bundle][kv head]: parts that are there, then rows that have been added up
     uint32_t team;                       // warps that add up a row
     uint32_t widest;                     // most queries of a bundle
+    uint32_t early;                      // the shared rows have been written before the kernel in front of this one began
     float scale_log2;
     long long wait_limit;
     int *err;
@@ -118,6 +137,42 @@ constexpr uint32_t kSmem = kKSlots * kSlot + 2 * kSlot + kQBytes + 2 * p_bytes(6
 static_assert(v_slots(32) * kSlot + 2 * p_bytes(32) == v_slots(64) * kSlot + 2 * p_bytes(64), "");
 static_assert(kSmem <= 232448, "the CTA's shared memory is 227 KB at most");
 
+// Whether the tile ends with the row that its session appends.
+__device__ __forceinline__ bool appends(const SharedParams &p, const Bundle &b, const Place &at)
+{
+    return p.k_new && at.segment && (at.tile + 1) * kTile >= p.own_rows[b.row0 + at.segment - 1];
+}
+__device__ __forceinline__ uint32_t position_of(const SharedParams &p, const Bundle &b, uint32_t session)
+{
+    return p.shared_rows[b.group] + p.own_rows[session] - 1;
+}
+// A session's new row of one kv head into its page, as wr_cuda_kv_append stores it (kernels.c:1406-1407, products rounded
+// separately; quant.c:121-136): a warp, two pairs of dims to a lane.  Bulk copies that lane 0 issues afterwards see it.
+__device__ __forceinline__ void append_row(const SharedParams &p, const Bundle &b, uint32_t session, uint32_t kvh, uint32_t which, uint32_t lane)
+{
+    const uint32_t row = p.own_rows[session] - 1, d = 2 * lane;
+    const float *const x = (which ? p.v_new : p.k_new) + ((size_t)session * p.n_kv + kvh) * kHd;
+    float lo[2] = {x[d], x[d + 1]}, hi[2] = {x[d + kHd / 2], x[d + 1 + kHd / 2]};
+    if (!which && p.n_rot) {
+        const float ln_theta = wrmath::log_ref(p.theta);
+#pragma unroll
+        for (uint32_t e = 0; e < 2; ++e) {
+            if (d + e >= p.n_rot) continue;
+            float sn, cs;
+            wrmath::rope_angle(position_of(p, b, session), d + e, kHd, ln_theta, sn, cs);
+            const float u = lo[e], v = hi[e];
+            lo[e] = wrmath::sub(wrmath::mul(u, cs), wrmath::mul(v, sn));
+            hi[e] = wrmath::add(wrmath::mul(u, sn), wrmath::mul(v, cs));
+        }
+    }
+    char *const block = reinterpret_cast<char *>(p.own_pages[session][row / kPageTokens]) + wr_block_off(kvh, which, kHd);
+    *reinterpret_cast<uint32_t *>(block + wr_elem_off(row % kPageTokens, d, kHd)) =
+        wr_f32_to_f16_trunc(lo[0]) | (uint32_t)wr_f32_to_f16_trunc(lo[1]) << 16;
+    *reinterpret_cast<uint32_t *>(block + wr_elem_off(row % kPageTokens, d + kHd / 2, kHd)) =
+        wr_f32_to_f16_trunc(hi[0]) | (uint32_t)wr_f32_to_f16_trunc(hi[1]) << 16;
+    asm volatile("fence.proxy.async.global;" ::: "memory");
+    __syncwarp();
+}
 __device__ __forceinline__ Item item_of(const SharedParams &p, uint32_t i)
 {
     Item it{};
@@ -127,8 +182,8 @@ __device__ __forceinline__ Item item_of(const SharedParams &p, uint32_t i)
     i -= b.item0;
     it.kvh = i % p.n_kv;
     i /= p.n_kv;
-    it.tile0 = b.tiles * i / b.chunks;
-    it.tiles = b.tiles * (i + 1) / b.chunks - it.tile0;
+    it.tile0 = share_at(b, i);
+    it.tiles = share_at(b, i + 1) - it.tile0;
     it.nq = b.sessions * b.heads;
     it.part = b.part0 + (i * p.n_kv + it.kvh) * it.nq;
     return it;
@@ -291,6 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
     uint8_t *const ks = smem_raw, *const qs = ks + kKSlots * kSlot, *const vs = qs + kQBytes, *const ps = vs + v_ring * kSlot;
     Bars &sm = *reinterpret_cast<Bars *>(ps + 2 * p_size);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Item first = item_of(p, blockIdx.x);                   // (1 us: the arguments' way into the constant cache)
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kKSlots; ++i) {
             mbar_init(&sm.k_full[i], 1);
@@ -315,50 +371,71 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
     tc5::fence_before();
     __syncthreads();
     tc5::fence_after();
-    pdl_wait();
-    pdl_trigger();                       // (only now: what starts early behind this may rely on everything before it)
+    // What the kernel before this one may still be writing waits for it.  With p.early that is not the shared rows: the loading warps
+    // request the first tiles of these at once.
+    const bool loads = warp == 0 || warp == 2;
+    bool waited = !(p.early && loads);
+    if (waited) {
+        pdl_wait();
+        pdl_trigger();                   // (only now: what starts early behind this may rely on everything before it)
+    }
+    auto wait_before = [&](bool need) {
+        if (need && !waited) pdl_wait();
+        waited |= need;
+    };
+    // The first queries are asked for before a whole ring of keys and values is: behind that they came 1 us later.
+    auto queries_first = [&]() { asm volatile("bar.sync 7, %0;" ::"n"(64 + 128 * kGroups) : "memory"); };
+    if (loads && !p.early) queries_first();
     const uint32_t tmem = sm.tmem;
     const long long limit = p.wait_limit;
     // Item number `it` of this CTA (the first is its own number); the loading warp is at most four items ahead of the slowest reader.
-    auto item_at = [&](uint32_t it, bool &ok, bool whole_warp) -> Item {
-        if (it == 0) return item_of(p, blockIdx.x);
+    auto item_at = [&](uint32_t it, bool &ok) -> Item {
+        if (it == 0) return first;
         uint64_t *bar = &sm.item_ready[it % kItemSlots];
         const uint32_t parity = (it / kItemSlots) & 1;
-        ok = whole_warp ? mbar_wait_warp(bar, parity, limit) : mbar_wait(bar, parity, limit);
+        ok = mbar_wait_warp(bar, parity, limit);
         return ok ? sm.item[it % kItemSlots] : Item{};
     };
 
-    if (warp == 0) {
-        if (lane == 0) {                                         // work items and K
-            uint32_t n = 0;
-            bool ok = true;
-            uint32_t next = blockIdx.x;
-            for (uint32_t it = 0; ok; ++it) {
-                const Item im = item_of(p, next);
+    if (warp == 0) {                                             // work items and K
+        uint32_t n = 0;
+        bool ok = true;
+        uint32_t next = 0;
+        for (uint32_t it = 0; ok; ++it) {
+            const Item im = it ? item_of(p, next) : first;
+            if (lane == 0) {
                 sm.item[it % kItemSlots] = im;
-                mbar_arrive(&sm.item_ready[it % kItemSlots]);     // (the first one's for the phases' sake)
-                if (!im.tiles) break;
-                const Bundle &bd = p.bundle[im.bundle];
-                Place at = place_at(p, bd, im.tile0);
-                for (uint32_t t = 0; t < im.tiles; ++t, ++n, step(p, bd, at)) {
-                    const uint32_t st = n % kKSlots;
-                    bool two;
-                    const uint64_t *table = pages_of(p, bd, at, two);
-                    const uint32_t pages = two ? 2u : 1u;
-                    const char *src[2] = {reinterpret_cast<const char *>(table[0]), nullptr};
-                    if (two) src[1] = reinterpret_cast<const char *>(table[1]);
-                    if (n >= kKSlots && !mbar_wait(&sm.k_free[st], (n / kKSlots - 1) & 1, limit)) {
-                        ok = false;
-                        break;
-                    }
-                    mbar_expect_tx(&sm.k_full[st], pages * kPageBlock);
-                    for (uint32_t g = 0; g < pages; ++g)
-                        for (uint32_t h = 0; h < 2; ++h)
-                            bulk_g2s(ks + st * kSlot + h * kBox + g * 8192, src[g] + wr_block_off(im.kvh, 0, kHd) + h * 8192, 8192,
-                                     &sm.k_full[st]);
-                }
-                if (ok) next = gridDim.x + (uint32_t)atomicAdd(p.sched, 1);
+                mbar_arrive(&sm.item_ready[it % kItemSlots]);    // (the first one's for the phases' sake)
             }
+            if (!im.tiles) break;
+            const Bundle &bd = p.bundle[im.bundle];
+            Place at = place_at(p, bd, im.tile0);
+            for (uint32_t t = 0; t < im.tiles; ++t, ++n, step(p, bd, at)) {
+                if (p.early && n == 1) queries_first();
+                wait_before(at.segment != 0);
+                if (appends(p, bd, at)) append_row(p, bd, bd.row0 + at.segment - 1, im.kvh, 0, lane);
+                const uint32_t st = n % kKSlots;
+                bool two;                                        // (the pages' addresses are there when the slot is free)
+                const uint64_t *table = pages_of(p, bd, at, two), page[2] = {table[0], two ? table[1] : 0};
+                if (n >= kKSlots && !mbar_wait_warp(&sm.k_free[st], (n / kKSlots - 1) & 1, limit)) {
+                    ok = false;
+                    break;
+                }
+                if (lane) continue;
+                mbar_expect_tx(&sm.k_full[st], (two ? 2 : 1) * kPageBlock);
+                for (uint32_t g = 0; g < (two ? 2u : 1u); ++g) {
+                    const char *src = reinterpret_cast<const char *>(page[g]) + wr_block_off(im.kvh, 0, kHd);
+                    bulk_g2s(ks + st * kSlot + g * 8192, src, 8192, &sm.k_full[st]);
+                    bulk_g2s(ks + st * kSlot + kBox + g * 8192, src + 8192, 8192, &sm.k_full[st]);
+                }
+            }
+            if (p.early && it == 0 && im.tiles == 1) queries_first();
+            wait_before(true);                                   // (the counter is the earlier launch's until it has ended)
+            if (ok && lane == 0) next = gridDim.x + (uint32_t)atomicAdd(p.sched, 1);
+            next = __shfl_sync(0xffffffffu, next, 0);
+        }
+        wait_before(true);
+        if (lane == 0) {
             if (!ok) atomicCAS(p.err, 0, 81);
             // the last CTA to leave makes the counters ready for the next launch
             __threadfence();
@@ -369,31 +446,34 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             for (uint32_t i = n - min(n, kKSlots); i < n; ++i) (void)mbar_wait(&sm.k_full[i % kKSlots], (i / kKSlots) & 1, limit);
         }
         __syncwarp();
-    } else if (warp == 2) {
-        if (lane == 0) {                                         // V
-            uint32_t n = 0;
-            bool ok = true;
-            for (uint32_t it = 0; ok; ++it) {
-                const Item im = item_at(it, ok, false);
-                if (!im.tiles) break;
-                const Bundle &bd = p.bundle[im.bundle];
-                Place at = place_at(p, bd, im.tile0);
-                for (uint32_t t = 0; t < im.tiles; ++t, ++n, step(p, bd, at)) {
-                    const uint32_t st = n % v_ring;
-                    bool two;
-                    const uint64_t *table = pages_of(p, bd, at, two);
-                    const uint32_t pages = two ? 2u : 1u;
-                    const char *src[2] = {reinterpret_cast<const char *>(table[0]), nullptr};
-                    if (two) src[1] = reinterpret_cast<const char *>(table[1]);
-                    if (n >= v_ring && !mbar_wait(&sm.v_free[st], (n / v_ring - 1) & 1, limit)) {
-                        ok = false;
-                        break;
-                    }
-                    mbar_expect_tx(&sm.v_full[st], pages * kPageBlock);
-                    for (uint32_t g = 0; g < pages; ++g)
-                        bulk_g2s(vs + st * kSlot + g * kPageBlock, src[g] + wr_block_off(im.kvh, 1, kHd), kPageBlock, &sm.v_full[st]);
+    } else if (warp == 2) {                                      // V
+        uint32_t n = 0;
+        bool ok = true;
+        for (uint32_t it = 0; ok; ++it) {
+            const Item im = item_at(it, ok);
+            if (!im.tiles) break;
+            const Bundle &bd = p.bundle[im.bundle];
+            Place at = place_at(p, bd, im.tile0);
+            for (uint32_t t = 0; t < im.tiles; ++t, ++n, step(p, bd, at)) {
+                if (p.early && n == 1) queries_first();
+                wait_before(at.segment != 0);
+                if (appends(p, bd, at)) append_row(p, bd, bd.row0 + at.segment - 1, im.kvh, 1, lane);
+                const uint32_t st = n % v_ring;
+                bool two;
+                const uint64_t *table = pages_of(p, bd, at, two), page[2] = {table[0], two ? table[1] : 0};
+                if (n >= v_ring && !mbar_wait_warp(&sm.v_free[st], (n / v_ring - 1) & 1, limit)) {
+                    ok = false;
+                    break;
                 }
+                if (lane) continue;
+                mbar_expect_tx(&sm.v_full[st], (two ? 2 : 1) * kPageBlock);
+                for (uint32_t g = 0; g < (two ? 2u : 1u); ++g)
+                    bulk_g2s(vs + st * kSlot + g * kPageBlock, reinterpret_cast<const char *>(page[g]) + wr_block_off(im.kvh, 1, kHd),
+                             kPageBlock, &sm.v_full[st]);
             }
+            if (p.early && it == 0 && im.tiles == 1) queries_first();
+        }
+        if (lane == 0) {
             if (!ok) atomicCAS(p.err, 0, 82);
             for (uint32_t i = n - min(n, v_ring); i < n; ++i) (void)mbar_wait(&sm.v_full[i % v_ring], (i / v_ring) & 1, limit);
         }
@@ -420,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             return true;
         };
         for (uint32_t it = 0; ok; ++it) {
-            const Item im = item_at(it, ok, true);
+            const Item im = item_at(it, ok);
             if (!im.tiles) break;
             const uint32_t n = 2 * padded(im.nq);
             const Bundle &bd = p.bundle[im.bundle];
@@ -463,21 +543,54 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
         auto queries = [&](const Item &im, uint32_t it) {
             const uint32_t rows = padded(im.nq);
             const Bundle &bd = p.bundle[im.bundle];
-            float4 x[kMaxQ / (4 * kGroups)];
+            constexpr uint32_t kEach = kMaxQ / (4 * kGroups);
+            const uint32_t each = rows / (4 * kGroups), r0 = (warp - 3) * each;     // rows of a warp: neighbours, mostly of one session
+            float4 x[kEach];
 #pragma unroll
-            for (uint32_t u = 0; u < kMaxQ / (4 * kGroups); ++u) {
-                const uint32_t r = warp - 3 + 4 * kGroups * u;
+            for (uint32_t u = 0; u < kEach; ++u) {
+                const uint32_t r = r0 + u;
                 x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < im.nq)
+                if (u < each && r < im.nq)
                     x[u] = __ldg(reinterpret_cast<const float4 *>(
                                      p.q + ((size_t)(bd.row0 + r / bd.heads) * p.n_q + im.kvh * p.per + bd.head0 + r % bd.heads) * kHd) + lane);
+            }
+            if (it == 0) asm volatile("bar.arrive 7, %0;" ::"n"(64 + 128 * kGroups) : "memory");
+            if (p.n_rot) {                                       // (as wr_cuda_kv_append rotates them)
+                const float ln_theta = wrmath::log_ref(p.theta);
+                uint32_t of = ~0u;
+                float cs[4], sn[4];                              // of dims 4 (lane % 16) .. + 3 and those 64 on
+#pragma unroll
+                for (uint32_t u = 0; u < kEach; ++u) {
+                    const uint32_t r = r0 + u, session = r / bd.heads;
+                    if (u >= each || r >= im.nq) break;
+                    if (session != of) {
+                        float c[2], d[2];
+#pragma unroll
+                        for (uint32_t e = 0; e < 2; ++e) wrmath::rope_angle(position_of(p, bd, bd.row0 + session), 2 * lane + e, kHd, ln_theta, d[e], c[e]);
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) {
+                            const uint32_t from = 2 * (lane & 15) + e / 2;
+                            cs[e] = __shfl_sync(0xffffffffu, c[e & 1], from);
+                            sn[e] = __shfl_sync(0xffffffffu, d[e & 1], from);
+                        }
+                        of = session;
+                    }
+                    float *const y = reinterpret_cast<float *>(&x[u]);
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        const float other = __shfl_xor_sync(0xffffffffu, y[e], 16);
+                        if (4 * (lane & 15) + e >= p.n_rot) continue;
+                        y[e] = lane < 16 ? wrmath::sub(wrmath::mul(y[e], cs[e]), wrmath::mul(other, sn[e]))
+                                         : wrmath::add(wrmath::mul(other, sn[e]), wrmath::mul(y[e], cs[e]));
+                    }
+                }
             }
             if (threadIdx.x == 96) sm.large[it & 1] = 0;
             all_sync();
 #pragma unroll
-            for (uint32_t u = 0; u < kMaxQ / (4 * kGroups); ++u) {
-                const uint32_t r = warp - 3 + 4 * kGroups * u;
-                if (r >= rows) continue;
+            for (uint32_t u = 0; u < kEach; ++u) {
+                const uint32_t r = r0 + u;
+                if (u >= each) continue;
                 float y[4] = {x[u].x * p.scale_log2, x[u].y * p.scale_log2, x[u].z * p.scale_log2, x[u].w * p.scale_log2}, up = 1.f;
                 const float top = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
                 if (__any_sync(0xffffffffu, top >= 32768.f)) {
@@ -504,11 +617,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             all_sync();                                          // (sm.up, sm.large)
             if (lane == 0) mbar_arrive(&sm.q_full);
         };
-        Item im = item_at(0, ok, true);
+        Item im = item_at(0, ok);
         // (a warp whose wait ran out stays with the others: they leave together, and the groups' barriers count on all of them)
         ok = !all_or(!ok);
-        if (ok && im.tiles) queries(im, 0);
-        Item following{};
         auto work = [&](auto size, uint32_t it) {
             constexpr uint32_t NQ = decltype(size)::value, H = NQ / kGroups, V = H < 8 ? H : 8;     // V: queries to a store
             const uint32_t q0 = group * H;                       // this group's first query
@@ -525,20 +636,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             auto add_values = [&](uint32_t tile, bool own, int lo, int hi) {
                 if (!own || (hi > 0 && lo < (int)H)) {
                     const uint32_t at = tmem + kTmemO + (tile & 1) * 2 * kMaxQ + lanes + q0;
-                    float high[H], low[H];
-                    tmem_ld(at, high);
-                    tmem_ld(at + NQ, low);
-                    tc5::wait_ld();
 #pragma unroll
-                    for (uint32_t j = 0; j < H; ++j)
-                        if (fabsf(high[j]) != INFINITY) high[j] += low[j];       // (as in scores)
-                    if (!own) {
+                    for (uint32_t j0 = 0; j0 < H; j0 += V) {     // (eight at a time: more at once do not fit the registers)
+                        float high[V], low[V];
+                        tmem_ld(at + j0, high);
+                        tmem_ld(at + NQ + j0, low);
+                        tc5::wait_ld();
 #pragma unroll
-                        for (uint32_t j = 0; j < H; j += 2) add2(o[j], o[j + 1], high[j], high[j + 1]);
-                    } else {
+                        for (uint32_t j = 0; j < V; ++j)
+                            if (fabsf(high[j]) != INFINITY) high[j] += low[j];   // (as in scores)
+                        if (!own) {
 #pragma unroll
-                        for (int j = 0; j < (int)H; ++j)
-                            if (j >= lo && j < hi) o[j] += high[j];
+                            for (uint32_t j = 0; j < V; j += 2) add2(o[j0 + j], o[j0 + j + 1], high[j], high[j + 1]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < (int)V; ++j)
+                                if ((int)j0 + j >= lo && (int)j0 + j < hi) o[j0 + j] += high[j];
+                        }
                     }
                 }
                 if (moved) {
@@ -591,18 +705,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                     for (int j = 0; j < (int)H; ++j) s[j] = seen && (!OWN || (j >= lo && j < hi)) ? s[j] : -INFINITY;
                 };
                 auto scores = [&](bool infinite) {
-                    float low[H];
                     tmem_ld(at, s);
-                    tmem_ld(at + NQ, low);
-                    tc5::wait_ld();
-                    if (infinite) {
-                        // (a row with an infinity: the high part has its product, the low one may have the other sign of it or a NaN)
 #pragma unroll
-                        for (uint32_t j = 0; j < H; ++j)
-                            if (fabsf(s[j]) != INFINITY) s[j] += low[j];
-                    } else {
+                    for (uint32_t j0 = 0; j0 < H; j0 += V) {
+                        float low[V];
+                        tmem_ld(at + NQ + j0, low);
+                        tc5::wait_ld();
+                        if (infinite) {
+                            // (a row with an infinity: the high part has its product, the low one may have the other sign of it or a NaN)
 #pragma unroll
-                        for (uint32_t j = 0; j < H; j += 2) add2(s[j], s[j + 1], low[j], low[j + 1]);
+                            for (uint32_t j = 0; j < V; ++j)
+                                if (fabsf(s[j0 + j]) != INFINITY) s[j0 + j] += low[j];
+                        } else {
+#pragma unroll
+                            for (uint32_t j = 0; j < V; j += 2) add2(s[j0 + j], s[j0 + j + 1], low[j], low[j + 1]);
+                        }
                     }
                     if (large) {
 #pragma unroll
@@ -699,11 +816,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                     lo2 = lo1; hi2 = hi1;
                     lo1 = lo; hi1 = hi;
                 }
-            // the next item's queries (the last scores have been read), then this one's results
-            bool more = true;
-            following = item_at(it + 1, more, true);
-            ok = !all_or(!(ok && more));
-            if (ok && following.tiles) queries(following, it + 1);
             // (of either barrier the phase before is known to be over: the scores seen last came behind those values)
             if (ok && n > n0 + 1) ok = mbar_wait_warp(&sm.o_full[n & 1], ((n - 2) >> 1) & 1, limit);
             if (ok) ok = mbar_wait_warp(&sm.o_full[(n - 1) & 1], ((n - 1) >> 1) & 1, limit);
@@ -729,12 +841,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             }
         };
         for (uint32_t it = 0; ok && im.tiles; ++it) {
+            queries(im, it);                                     // (the last item's scores have been read)
             switch (padded(im.nq)) {
             case 16: work(std::integral_constant<uint32_t, 16>{}, it); break;
             case 32: work(std::integral_constant<uint32_t, 32>{}, it); break;
             default: work(std::integral_constant<uint32_t, 64>{}, it);
             }
-            im = following;
+            im = item_at(it + 1, ok);
+            ok = !all_or(!ok);
         }
         if (ok) ok = add_up(p, reinterpret_cast<float4 *>(ps), warp - 3, lane);
         if (!ok && lane == 0) atomicCAS(p.err, 0, 84);
@@ -772,7 +886,7 @@ int wr_shared_validate(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv,
 // Enqueue the kernel on device-resident q / out.  Caller holds ctx->lock and has validated the arguments.
 int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *seq_lens,
                      uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, const float *dq, float *dout,
-                     uint32_t n_q, float scale_override)
+                     uint32_t n_q, float scale_override, const wr_shared_append *append, bool dependent)
 {
     SharedParams p{};
     p.n_q = n_q;
@@ -780,9 +894,11 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
     p.per = n_q / p.n_kv;
     const uint32_t splits = (p.per + kMaxQ - 1) / kMaxQ, most = std::max(kMaxQ / p.per, 1u);     // bundles to a session, or sessions to a bundle
     uint32_t longest = 0;
+    bool settled = true;                 // several hold the shared rows: no step has written them
     for (uint32_t g = 0, s = 0; g < n_groups; s += group_sess[g++]) {
         p.shared_pages[g] = kv[s]->d_pages + (size_t)layer * kv[s]->n_pages;
         p.shared_rows[g] = group_rows[g];
+        settled = settled && (group_sess[g] > 1 || !group_rows[g]);
         for (uint32_t i = s; i < s + group_sess[g]; ++i) {
             p.own_pages[i] = kv[i]->d_pages + (size_t)layer * kv[i]->n_pages + group_rows[g] / kPageTokens;
             p.own_rows[i] = seq_lens[i] - group_rows[g];
@@ -790,32 +906,35 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
         for (uint32_t i = s; i < s + group_sess[g]; i += most) {
             const uint32_t n = std::min(most, s + group_sess[g] - i);
             if (p.n_bundles + splits > kMaxBundles) return WR_CUDA_ERR_LIMIT;
-            uint32_t tiles = (group_rows[g] + kTile - 1) / kTile;
+            const uint32_t shared = (group_rows[g] + kTile - 1) / kTile;
+            uint32_t tiles = shared;
             for (uint32_t t = i; t < i + n; ++t) {
                 tiles += (p.own_rows[t] + kTile - 1) / kTile;
                 p.first_bundle[t] = (uint8_t)p.n_bundles;
             }
             for (uint32_t h = 0; h < splits; ++h)
-                p.bundle[p.n_bundles++] = {g, i, n, h * kMaxQ, std::min(kMaxQ, p.per - h * kMaxQ), tiles, 0, 0, 0};
-            longest = std::max(longest, tiles);
+                p.bundle[p.n_bundles++] = {g, i, n, h * kMaxQ, std::min(kMaxQ, p.per - h * kMaxQ), shared, tiles, 0, 0, 0};
+            longest = std::max(longest, weight_of(shared, tiles));
         }
     }
-    // Items are even shares of the bundles' lists, in one round of the SMs or a few: the fewer tiles one after the other, an item's
-    // beginning and end counted as two, the sooner.
+    // Items are even shares of the bundles' lists, in one round of the SMs or a few: the less work one after the other, an item's
+    // beginning and end counted as two tiles, the sooner.  No share is less than a tile.
     auto items_of = [&](uint32_t share) {
         uint64_t n = 0;
-        for (uint32_t i = 0; i < p.n_bundles; ++i) n += (uint64_t)((p.bundle[i].tiles + share - 1) / share) * p.n_kv;
+        for (uint32_t i = 0; i < p.n_bundles; ++i) {
+            n += (uint64_t)shares_of(p.bundle[i].shared, p.bundle[i].tiles, share) * p.n_kv;
+        }
         return n;
     };
     uint32_t share = longest, best = ~0u;
     for (uint32_t rounds = 1; rounds <= 4; ++rounds) {
-        uint32_t lo = 1, hi = longest;                           // the smallest share that makes no more items than that
+        uint32_t lo = 4, hi = std::max(longest, 4u);             // the smallest share that makes no more items than that
         while (lo < hi) {
             const uint32_t mid = (lo + hi) / 2;
             if (items_of(mid) <= (uint64_t)rounds * ctx->sm_count) hi = mid;
             else lo = mid + 1;
         }
-        const uint32_t time = (uint32_t)((items_of(lo) + ctx->sm_count - 1) / ctx->sm_count) * (lo + 2);
+        const uint32_t time = (uint32_t)((items_of(lo) + ctx->sm_count - 1) / ctx->sm_count) * (lo + 8);
         if (time < best) {
             best = time;
             share = lo;
@@ -824,7 +943,7 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
     uint64_t parts = 0;
     for (uint32_t i = 0; i < p.n_bundles; ++i) {
         Bundle &b = p.bundle[i];
-        b.chunks = (b.tiles + share - 1) / share;
+        b.chunks = shares_of(b.shared, b.tiles, share);
         b.item0 = p.items;
         b.part0 = (uint32_t)parts;
         p.items += b.chunks * p.n_kv;
@@ -844,6 +963,14 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
     p.o = reinterpret_cast<float *>(ws + head + ml);
     p.q = dq;
     p.out = dout;
+    if (append) {
+        p.k_new = append->k;
+        p.v_new = append->v;
+        if (append->flags & WR_CUDA_APPEND_ROPE) {
+            p.n_rot = append->n_rot_pairs >= 1 && append->n_rot_pairs < kHd / 2 ? append->n_rot_pairs : kHd / 2;     // kernels.c:1381-1383
+            p.theta = append->theta_base < 1.0f ? 10000.0f : append->theta_base;                                    // kernels.c:1374
+        }
+    }
     p.scale_log2 = (scale_override > 0.0f ? scale_override : 1.0f / sqrtf((float)kHd)) * kLog2e;
     p.wait_limit = ctx->wait_limit;
     p.err = ctx->dev_err;
@@ -852,53 +979,47 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
         ctx->attr_flags |= 0x100u;
     }
     const uint32_t grid = std::min<uint32_t>(p.items, (uint32_t)ctx->sm_count);
+    // Behind another launch of this kernel, which writes rows that one session alone holds (a fork in between counts as another
+    // kind of launch) and lets the next begin when all before it has ended.
+    p.early = settled && dependent && ctx->pdl_index == ctx->launches && ctx->pdl_kind == WR_PDL_SHARED;
     for (uint32_t i = 0; i < p.n_bundles; ++i) p.widest = std::max(p.widest, p.bundle[i].sessions * p.bundle[i].heads);
     // a row's team: as many warps as there are for all rows at once
     for (p.team = kMergeWarps; p.team > 1 && (uint64_t)p.rows * p.team > (uint64_t)grid * kMergeWarps;) p.team /= 2;
-    WR_CUDA_TRY(wr_launch_pdl(attn_shared_kernel, dim3(grid), dim3(kThreads), (size_t)kSmem, ctx->stream, p));
+    WR_CUDA_TRY(wr_launch(dependent, attn_shared_kernel, dim3(grid), dim3(kThreads), (size_t)kSmem, ctx->stream, p));
     ctx->launches++;
+    ctx->pdl_kind = WR_PDL_SHARED;
+    ctx->pdl_index = ctx->launches;
     WR_CUDA_TRY(cudaGetLastError());
     return WR_CUDA_OK;
 }
 
-// decode_step's body (append, then attention) and attention alone share the handling of host buffers.
-static int shared_call(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *positions,
-                       const uint32_t *seq_lens, uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, float *q,
-                       const float *k_rows, const float *v_rows, float *out, uint32_t n_q, float theta_base, uint32_t n_rot_pairs,
-                       uint32_t flags, float scale_override, int mem, bool dependent)
+// attn_decode_shared and, with `append`, decode_step_shared
+static int shared_call(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *seq_lens, uint32_t n_groups,
+                       const uint32_t *group_sess, const uint32_t *group_rows, const float *q, float *out, uint32_t n_q, float scale_override,
+                       const wr_shared_append *append, int mem, bool dependent)
 {
-    const bool append = positions != nullptr;
     const uint32_t n_kv = kv[0]->n_kv_at(layer);
     const size_t kv_bytes = append ? (size_t)n_sess * n_kv * kHd * sizeof(float) : 0, q_bytes = (size_t)n_sess * n_q * kHd * sizeof(float);
-    const float *dk = k_rows, *dv = v_rows;
-    float *dq = q, *dout = out;
-    int rc;
-    if (mem == WR_CUDA_MEM_HOST) {
-        rc = wr_ctx_reserve_stage(ctx, 2 * kv_bytes + 2 * q_bytes, 0);
-        if (rc != WR_CUDA_OK) return rc;
-        char *d = (char *)ctx->stage_dev;
-        dk = (const float *)d;
-        dv = (const float *)(d + kv_bytes);
-        dq = (float *)(d + 2 * kv_bytes);
-        dout = (float *)(d + 2 * kv_bytes + q_bytes);
-        if (append) {
-            WR_CUDA_TRY(cudaMemcpyAsync((void *)dk, k_rows, kv_bytes, cudaMemcpyHostToDevice, ctx->stream));
-            WR_CUDA_TRY(cudaMemcpyAsync((void *)dv, v_rows, kv_bytes, cudaMemcpyHostToDevice, ctx->stream));
-        }
-        WR_CUDA_TRY(cudaMemcpyAsync(dq, q, q_bytes, cudaMemcpyHostToDevice, ctx->stream));
-    }
-    if (append) {
-        rc = wr_append_launch(ctx, n_sess, kv, layer, positions, 1, dk, dv, dq, n_q, theta_base, n_rot_pairs, flags, nullptr, nullptr,
-                              dependent);
-        if (rc != WR_CUDA_OK) return rc;
-    }
-    rc = wr_shared_launch(ctx, n_sess, kv, layer, seq_lens, n_groups, group_sess, group_rows, dq, dout, n_q, scale_override);
+    if (mem == WR_CUDA_MEM_DEVICE)
+        return wr_shared_launch(ctx, n_sess, kv, layer, seq_lens, n_groups, group_sess, group_rows, q, out, n_q, scale_override, append, dependent);
+    int rc = wr_ctx_reserve_stage(ctx, 2 * kv_bytes + 2 * q_bytes, 0);
     if (rc != WR_CUDA_OK) return rc;
-    if (mem == WR_CUDA_MEM_HOST) {
-        WR_CUDA_TRY(cudaMemcpyAsync(out, dout, q_bytes, cudaMemcpyDeviceToHost, ctx->stream));
-        return wr_ctx_sync_checked(ctx);
+    char *d = (char *)ctx->stage_dev;
+    float *const dq = (float *)(d + 2 * kv_bytes), *const dout = (float *)(d + 2 * kv_bytes + q_bytes);
+    wr_shared_append staged;
+    if (append) {
+        staged = *append;
+        staged.k = (const float *)d;
+        staged.v = (const float *)(d + kv_bytes);
+        WR_CUDA_TRY(cudaMemcpyAsync(d, append->k, kv_bytes, cudaMemcpyHostToDevice, ctx->stream));
+        WR_CUDA_TRY(cudaMemcpyAsync(d + kv_bytes, append->v, kv_bytes, cudaMemcpyHostToDevice, ctx->stream));
     }
-    return WR_CUDA_OK;
+    WR_CUDA_TRY(cudaMemcpyAsync(dq, q, q_bytes, cudaMemcpyHostToDevice, ctx->stream));
+    rc = wr_shared_launch(ctx, n_sess, kv, layer, seq_lens, n_groups, group_sess, group_rows, dq, dout, n_q, scale_override,
+                          append ? &staged : nullptr, dependent);
+    if (rc != WR_CUDA_OK) return rc;
+    WR_CUDA_TRY(cudaMemcpyAsync(out, dout, q_bytes, cudaMemcpyDeviceToHost, ctx->stream));
+    return wr_ctx_sync_checked(ctx);
 }
 
 extern "C" int wr_cuda_attn_decode_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer,
@@ -911,12 +1032,11 @@ extern "C" int wr_cuda_attn_decode_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_
     int rc = wr_shared_validate(ctx, n_sess, kv, layer, seq_lens, n_groups, group_sess, group_rows, q, out, n_q_heads, mem);
     if (rc != WR_CUDA_OK) return rc;
     WR_CUDA_TRY(cudaSetDevice(ctx->device));
-    return shared_call(ctx, n_sess, kv, layer, nullptr, seq_lens, n_groups, group_sess, group_rows, const_cast<float *>(q), nullptr,
-                       nullptr, out, n_q_heads, 0.f, 0, 0, scale_override, mem, true);
+    return shared_call(ctx, n_sess, kv, layer, seq_lens, n_groups, group_sess, group_rows, q, out, n_q_heads, scale_override, nullptr, mem, true);
 }
 
 int wr_decode_step_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *positions,
-                          uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, float *q, const float *k_rows,
+                          uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, const float *q, const float *k_rows,
                           const float *v_rows, float *out, uint32_t n_q_heads, float theta_base, uint32_t n_rot_pairs, uint32_t flags,
                           float scale_override, int mem, bool dependent)
 {
@@ -931,13 +1051,14 @@ int wr_decode_step_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *
         for (uint32_t i = s; i < s + group_sess[g]; ++i)
             if (group_rows[g] > positions[i]) return WR_CUDA_ERR_INVAL;
     WR_CUDA_TRY(cudaSetDevice(ctx->device));
-    return shared_call(ctx, n_sess, kv, layer, positions, seq_lens, n_groups, group_sess, group_rows, q, k_rows, v_rows, out, n_q_heads,
-                       theta_base, n_rot_pairs, flags, scale_override, mem, dependent);
+    const wr_shared_append append = {k_rows, v_rows, theta_base, n_rot_pairs, flags};
+    return shared_call(ctx, n_sess, kv, layer, seq_lens, n_groups, group_sess, group_rows, q, out, n_q_heads, scale_override, &append, mem,
+                       dependent);
 }
 
 extern "C" int wr_cuda_decode_step_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer,
                                           const uint32_t *positions, uint32_t n_groups, const uint32_t *group_sess,
-                                          const uint32_t *group_rows, float *q, const float *k_rows, const float *v_rows, float *out,
+                                          const uint32_t *group_rows, const float *q, const float *k_rows, const float *v_rows, float *out,
                                           uint32_t n_q_heads, float theta_base, uint32_t n_rot_pairs, uint32_t flags,
                                           float scale_override, int mem)
 {

@@ -207,6 +207,8 @@ extern "C" int wr_cuda_kv_fork(wr_cuda_ctx *ctx, wr_cuda_kv *kv, uint32_t n_rows
     }
     ctx->live_kv++;
     *out = f;
+    // (rows that the last launch of shared attention may still be writing may be shared ones now)
+    if (ctx->pdl_kind == WR_PDL_SHARED) ctx->pdl_kind = WR_PDL_PREFILL_PART;
     return WR_CUDA_OK;
 }
 

@@ -34,12 +34,18 @@ inline bool wr_kv_writable(const wr_cuda_kv *kv, uint32_t row0, uint32_t n)
 int wr_shared_validate(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *seq_lens,
                        uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, const void *q, const void *out,
                        uint32_t n_q, int mem);
+// the rows that decode_step_shared appends on the way (device memory)
+struct wr_shared_append {
+    const float *k, *v;
+    float theta_base;
+    uint32_t n_rot_pairs, flags;
+};
 int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *seq_lens,
                      uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, const float *dq, float *dout,
-                     uint32_t n_q, float scale_override);
+                     uint32_t n_q, float scale_override, const wr_shared_append *append, bool dependent);
 // wr_cuda_decode_step_shared; dependent: as wr_decode_step's.  Caller holds ctx->lock.
 int wr_decode_step_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *positions,
-                          uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, float *q, const float *k_rows,
+                          uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, const float *q, const float *k_rows,
                           const float *v_rows, float *out, uint32_t n_q_heads, float theta_base, uint32_t n_rot_pairs, uint32_t flags,
                           float scale_override, int mem, bool dependent = true);
 
