@@ -46,11 +46,16 @@ constexpr uint32_t kTmemCols = 512, kTmemO = 256;                               
 constexpr uint32_t kMaxBundles = 64;
 constexpr float kGrow = 8.0f, kLog2e = 1.4426950408889634f;
 
+// A bundle's columns: its queries, rounded up to a size that the groups of threads are made for.
+__host__ __device__ __forceinline__ uint32_t padded(uint32_t nq) { return nq <= 16 ? 16u : nq <= 32 ? 32u : 64u; }
 struct Bundle {
     uint32_t group, row0, sessions;      // its group; its first session, how many
     uint32_t head0, heads;               // which of a kv head's query heads
     uint32_t shared, tiles, chunks, item0, part0;        // tiles: all of them, the shared ones first
+    uint32_t nq, columns, inverse;       // sessions x heads; padded; 65536 / heads
 };
+// x / heads for a column's number, by 65536 / heads rounded up: 64 columns at most, so the remainder does not reach the next number
+__device__ __forceinline__ uint32_t over_heads(const Bundle &b, uint32_t x) { return x * b.inverse >> 16; }
 // Where share i of a bundle's tiles begins.  An own tile's work counts five quarters of a shared one's: 2.0 us against the 1.55 that
 // HBM needs for it (16 sessions behind 32768 rows: 39.8 us with even numbers).
 __host__ __device__ __forceinline__ uint32_t weight_of(uint32_t shared, uint32_t tiles) { return 4 * shared + 5 * (tiles - shared); }
@@ -89,7 +94,7 @@ struct SharedParams {
 };
 struct Item {
     uint32_t tiles, tile0;               // tiles 0: no more work
-    uint32_t bundle, kvh, nq, part;
+    uint32_t bundle, kvh, part;
 };
 // Where a role is in a bundle's list: segment 0 is the shared rows, 1 + i the i-th session's own.
 struct Place {
@@ -184,12 +189,9 @@ __device__ __forceinline__ Item item_of(const SharedParams &p, uint32_t i)
     i /= p.n_kv;
     it.tile0 = share_at(b, i);
     it.tiles = share_at(b, i + 1) - it.tile0;
-    it.nq = b.sessions * b.heads;
-    it.part = b.part0 + (i * p.n_kv + it.kvh) * it.nq;
+    it.part = b.part0 + (i * p.n_kv + it.kvh) * b.nq;
     return it;
 }
-// The queries of an item, rounded up to what a group of threads has at its fixed sizes: half of them each.
-__host__ __device__ __forceinline__ uint32_t padded(uint32_t nq) { return nq <= 16 ? 16u : nq <= 32 ? 32u : 64u; }
 __device__ __forceinline__ void group_sync(uint32_t id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ bool group_or(uint32_t id, uint32_t threads, bool x)
 {
@@ -263,8 +265,8 @@ __device__ __forceinline__ bool add_up(const SharedParams &p, float4 *sums, uint
         const uint32_t s = mine ? row / p.n_q : 0, head = mine ? row % p.n_q : 0, kvh = head / p.per;
         const uint32_t which = p.first_bundle[s] + head % p.per / kMaxQ;
         const Bundle &b = p.bundle[which];
-        const uint32_t nq = b.sessions * b.heads, stride = p.n_kv * nq;
-        const uint32_t first = b.part0 + kvh * nq + (s - b.row0) * b.heads + head % p.per - b.head0;
+        const uint32_t stride = p.n_kv * b.nq;
+        const uint32_t first = b.part0 + kvh * b.nq + (s - b.row0) * b.heads + head % p.per - b.head0;
         int *const done = p.done + which * p.n_kv + kvh;
         uint32_t n = mine && ok ? b.chunks : 0;
         if (n && sub == 0) {                                     // (few ask: thousands of warps at these words held up what they wait for)
@@ -332,7 +334,7 @@ __device__ __forceinline__ bool add_up(const SharedParams &p, float4 *sums, uint
             else acc = make_float4(acc.x / l, acc.y / l, acc.z / l, acc.w / l);
             *(reinterpret_cast<float4 *>(p.out + (size_t)row * kHd) + lane) = acc;
             // the last row leaves the counter as it was
-            if (lane == 0 && atomicAdd(done, 1) == (int)(n + nq) - 1) *done = 0;
+            if (lane == 0 && atomicAdd(done, 1) == (int)(n + b.nq) - 1) *done = 0;
         }
         if (team > 1) all_sync();
     }
@@ -373,12 +375,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
     tc5::fence_after();
     // What the kernel before this one may still be writing waits for it.  With p.early that is not the shared rows: the loading warps
     // request the first tiles of these at once.
+    // The others work out the addresses of their first queries before they wait.
     const bool loads = warp == 0 || warp == 2;
-    bool waited = !(p.early && loads);
-    if (waited) {
-        pdl_wait();
-        pdl_trigger();                   // (only now: what starts early behind this may rely on everything before it)
+    bool waited = loads && !p.early;
+    if (loads) {
+        const Place at = place_at(p, p.bundle[first.bundle], first.tile0);
+        bool two;
+        const uint64_t *const table = pages_of(p, p.bundle[first.bundle], at, two);
+        asm volatile("" ::"l"(table));                           // (worked out here: the arguments' way into the constant cache)
     }
+    if (waited) pdl_wait();
+    if (waited) pdl_trigger();           // (only now: what starts early behind this may rely on everything before it)
     auto wait_before = [&](bool need) {
         if (need && !waited) pdl_wait();
         waited |= need;
@@ -502,8 +509,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
         for (uint32_t it = 0; ok; ++it) {
             const Item im = item_at(it, ok);
             if (!im.tiles) break;
-            const uint32_t n = 2 * padded(im.nq);
             const Bundle &bd = p.bundle[im.bundle];
+            const uint32_t n = 2 * bd.columns;
             Place at = place_at(p, bd, im.tile0);
             ok = mbar_wait_warp(&sm.q_full, it & 1, limit) && score(n);
             for (uint32_t t = 0; t < im.tiles && ok; ++t, step(p, bd, at)) {
@@ -541,18 +548,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
         // The item's queries as operands: scaled so that scores are powers of two's exponents, in a high and a low F16 part.  Up to
         // 2^15 that leaves 2^-22 of an element or 2^-25, whichever is more; rows with larger ones are brought below it by a power of two.
         auto queries = [&](const Item &im, uint32_t it) {
-            const uint32_t rows = padded(im.nq);
             const Bundle &bd = p.bundle[im.bundle];
+            const uint32_t rows = bd.columns;
             constexpr uint32_t kEach = kMaxQ / (4 * kGroups);
             const uint32_t each = rows / (4 * kGroups), r0 = (warp - 3) * each;     // rows of a warp: neighbours, mostly of one session
             float4 x[kEach];
+            uint32_t from[kEach];                                // (row of q; ~0: none)
 #pragma unroll
             for (uint32_t u = 0; u < kEach; ++u) {
-                const uint32_t r = r0 + u;
+                const uint32_t r = r0 + u, session = over_heads(bd, r);
+                from[u] = u < each && r < bd.nq ? (bd.row0 + session) * p.n_q + im.kvh * p.per + bd.head0 + r - session * bd.heads : ~0u;
+                asm volatile("" ::"r"(from[u]));
+            }
+            if (it == 0) {
+                pdl_wait();
+                pdl_trigger();
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < kEach; ++u) {
                 x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (u < each && r < im.nq)
-                    x[u] = __ldg(reinterpret_cast<const float4 *>(
-                                     p.q + ((size_t)(bd.row0 + r / bd.heads) * p.n_q + im.kvh * p.per + bd.head0 + r % bd.heads) * kHd) + lane);
+                if (~from[u]) x[u] = __ldg(reinterpret_cast<const float4 *>(p.q + (size_t)from[u] * kHd) + lane);
             }
             if (it == 0) asm volatile("bar.arrive 7, %0;" ::"n"(64 + 128 * kGroups) : "memory");
             if (p.n_rot) {                                       // (as wr_cuda_kv_append rotates them)
@@ -561,8 +576,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                 float cs[4], sn[4];                              // of dims 4 (lane % 16) .. + 3 and those 64 on
 #pragma unroll
                 for (uint32_t u = 0; u < kEach; ++u) {
-                    const uint32_t r = r0 + u, session = r / bd.heads;
-                    if (u >= each || r >= im.nq) break;
+                    const uint32_t session = over_heads(bd, r0 + u);
+                    if (!~from[u]) break;
                     if (session != of) {
                         float c[2], d[2];
 #pragma unroll
@@ -824,13 +839,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             moved = false;
             add_values(n - 1, n > n_own, lo1, hi1);
             float *to = p.o + (size_t)(im.part + q0) * kHd + key;
+            const uint32_t used = bd.nq - min(bd.nq, q0);        // (of this group's columns)
 #pragma unroll
             for (uint32_t j = 0; j < H; ++j)
-                if (q0 + j < im.nq) to[(size_t)j * kHd] = o[j];
+                if (j < used) to[(size_t)j * kHd] = o[j];
             const int idx = warp_reduce_many<(int)H>(l, (int)lane);
             sm.red[q0 + idx][quarter] = l[0];
             group_sync(bar);
-            if (tid < H && q0 + tid < im.nq) {
+            if (tid < min(used, H)) {
                 const float4 w = *reinterpret_cast<const float4 *>(sm.red[q0 + tid]);
                 p.ml[im.part + q0 + tid] = make_float2(fresh ? WR_NEG_SENTINEL : -sm.nm[q0 + tid], (w.x + w.y) + (w.z + w.w));
             }
@@ -842,7 +858,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
         };
         for (uint32_t it = 0; ok && im.tiles; ++it) {
             queries(im, it);                                     // (the last item's scores have been read)
-            switch (padded(im.nq)) {
+            switch (p.bundle[im.bundle].columns) {
             case 16: work(std::integral_constant<uint32_t, 16>{}, it); break;
             case 32: work(std::integral_constant<uint32_t, 32>{}, it); break;
             default: work(std::integral_constant<uint32_t, 64>{}, it);
@@ -912,8 +928,10 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
                 tiles += (p.own_rows[t] + kTile - 1) / kTile;
                 p.first_bundle[t] = (uint8_t)p.n_bundles;
             }
-            for (uint32_t h = 0; h < splits; ++h)
-                p.bundle[p.n_bundles++] = {g, i, n, h * kMaxQ, std::min(kMaxQ, p.per - h * kMaxQ), shared, tiles, 0, 0, 0};
+            for (uint32_t h = 0; h < splits; ++h) {
+                const uint32_t heads = std::min(kMaxQ, p.per - h * kMaxQ);
+                p.bundle[p.n_bundles++] = {g, i, n, h * kMaxQ, heads, shared, tiles, 0, 0, 0, n * heads, padded(n * heads), 65535 / heads + 1};
+            }
             longest = std::max(longest, weight_of(shared, tiles));
         }
     }
@@ -947,7 +965,7 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
         b.item0 = p.items;
         b.part0 = (uint32_t)parts;
         p.items += b.chunks * p.n_kv;
-        parts += (uint64_t)b.chunks * p.n_kv * b.sessions * b.heads;
+        parts += (uint64_t)b.chunks * p.n_kv * b.nq;
     }
     if (parts > 0x7fffffffu) return WR_CUDA_ERR_LIMIT;
     // counters first: they are zeros between launches
@@ -982,7 +1000,7 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
     // Behind another launch of this kernel, which writes rows that one session alone holds (a fork in between counts as another
     // kind of launch) and lets the next begin when all before it has ended.
     p.early = settled && dependent && ctx->pdl_index == ctx->launches && ctx->pdl_kind == WR_PDL_SHARED;
-    for (uint32_t i = 0; i < p.n_bundles; ++i) p.widest = std::max(p.widest, p.bundle[i].sessions * p.bundle[i].heads);
+    for (uint32_t i = 0; i < p.n_bundles; ++i) p.widest = std::max(p.widest, p.bundle[i].columns);
     // a row's team: as many warps as there are for all rows at once
     for (p.team = kMergeWarps; p.team > 1 && (uint64_t)p.rows * p.team > (uint64_t)grid * kMergeWarps;) p.team /= 2;
     WR_CUDA_TRY(wr_launch(dependent, attn_shared_kernel, dim3(grid), dim3(kThreads), (size_t)kSmem, ctx->stream, p));
