@@ -81,6 +81,7 @@ struct SharedParams {
     float theta;
     uint32_t n_rot;                      // pairs that new keys and the queries are rotated by; 0: none
     float *out;
+    uint32_t parts;                      // of the bundles that have more than one; the others' rows are written at once
     float2 *ml;                          // [part]: reference (log2), sum
     float *o;                            // [part][128]
     int *sched;                          // next item, CTAs that have left
@@ -117,6 +118,12 @@ __device__ __forceinline__ void step(const SharedParams &p, const Bundle &b, Pla
         at.tile = 0;
         ++at.segment;
     }
+}
+// a column's row of q and of the result
+__device__ __forceinline__ uint32_t row_of(const SharedParams &p, const Bundle &b, uint32_t kvh, uint32_t column)
+{
+    const uint32_t session = over_heads(b, column);
+    return (b.row0 + session) * p.n_q + kvh * p.per + b.head0 + column - session * b.heads;
 }
 // the tile's pages of one layer: the first one's address in the table, and whether there is a second
 __device__ __forceinline__ const uint64_t *pages_of(const SharedParams &p, const Bundle &b, const Place &at, bool &two)
@@ -268,7 +275,7 @@ __device__ __forceinline__ bool add_up(const SharedParams &p, float4 *sums, uint
         const uint32_t stride = p.n_kv * b.nq;
         const uint32_t first = b.part0 + kvh * b.nq + (s - b.row0) * b.heads + head % p.per - b.head0;
         int *const done = p.done + which * p.n_kv + kvh;
-        uint32_t n = mine && ok ? b.chunks : 0;
+        uint32_t n = mine && ok && b.chunks > 1 ? b.chunks : 0;
         if (n && sub == 0) {                                     // (few ask: thousands of warps at these words held up what they wait for)
             long long t0 = 0;
             for (bool again = false;; again = true) {
@@ -556,8 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             uint32_t from[kEach];                                // (row of q; ~0: none)
 #pragma unroll
             for (uint32_t u = 0; u < kEach; ++u) {
-                const uint32_t r = r0 + u, session = over_heads(bd, r);
-                from[u] = u < each && r < bd.nq ? (bd.row0 + session) * p.n_q + im.kvh * p.per + bd.head0 + r - session * bd.heads : ~0u;
+                from[u] = u < each && r0 + u < bd.nq ? row_of(p, bd, im.kvh, r0 + u) : ~0u;
                 asm volatile("" ::"r"(from[u]));
             }
             if (it == 0) {
@@ -838,20 +844,31 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             if (n > n0 + 1) add_values(n - 2, n >= n_own + 2, lo2, hi2);
             moved = false;
             add_values(n - 1, n > n_own, lo1, hi1);
-            float *to = p.o + (size_t)(im.part + q0) * kHd + key;
-            const uint32_t used = bd.nq - min(bd.nq, q0);        // (of this group's columns)
+            const uint32_t used = min(bd.nq - min(bd.nq, q0), H);        // this group's columns that are queries'
+            const bool whole = bd.chunks == 1;
+            if (!whole) {
+                float *to = p.o + (size_t)(im.part + q0) * kHd + key;
 #pragma unroll
-            for (uint32_t j = 0; j < H; ++j)
-                if (j < used) to[(size_t)j * kHd] = o[j];
+                for (uint32_t j = 0; j < H; ++j)
+                    if (j < used) to[(size_t)j * kHd] = o[j];
+            }
             const int idx = warp_reduce_many<(int)H>(l, (int)lane);
             sm.red[q0 + idx][quarter] = l[0];
             group_sync(bar);
-            if (tid < min(used, H)) {
+            if (whole) {                                         // (the values that add_up gives one part)
+#pragma unroll
+                for (uint32_t j = 0; j < H; ++j) {
+                    if (j >= used || !ok) break;
+                    const float4 w = *reinterpret_cast<const float4 *>(sm.red[q0 + j]);
+                    const float sum = (w.x + w.y) + (w.z + w.w);
+                    p.out[(size_t)row_of(p, bd, im.kvh, q0 + j) * kHd + key] = sum == 0.f ? 0.f : o[j] / sum;
+                }
+            } else if (tid < used) {
                 const float4 w = *reinterpret_cast<const float4 *>(sm.red[q0 + tid]);
                 p.ml[im.part + q0 + tid] = make_float2(fresh ? WR_NEG_SENTINEL : -sm.nm[q0 + tid], (w.x + w.y) + (w.z + w.w));
             }
             ok = !all_or(!ok);
-            if (ok && threadIdx.x == 96) {                       // a part of these rows is there
+            if (!whole && ok && threadIdx.x == 96) {             // a part of these rows is there
                 __threadfence();
                 atomicAdd(p.done + im.bundle * p.n_kv + im.kvh, 1);
             }
@@ -866,7 +883,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             im = item_at(it + 1, ok);
             ok = !all_or(!ok);
         }
-        if (ok) ok = add_up(p, reinterpret_cast<float4 *>(ps), warp - 3, lane);
+        if (ok && p.parts) ok = add_up(p, reinterpret_cast<float4 *>(ps), warp - 3, lane);
         if (!ok && lane == 0) atomicCAS(p.err, 0, 84);
     }
     tc5::fence_before();
@@ -899,6 +916,9 @@ int wr_shared_validate(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv,
     return s == n_sess ? WR_CUDA_OK : WR_CUDA_ERR_INVAL;
 }
 
+// What adding the parts up costs, in quarters of a tile.  One session's 1 / 2 / 3 / 5 tiles for eight kv heads: 6.0 / 6.9 / 6.9 / 8.9 us
+// whole, - / 8.4 / 8.4 / 8.4 us in shares of a tile.
+constexpr uint32_t kMergeCost = 13;
 // Enqueue the kernel on device-resident q / out.  Caller holds ctx->lock and has validated the arguments.
 int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *seq_lens,
                      uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, const float *dq, float *dout,
@@ -935,8 +955,8 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
             longest = std::max(longest, weight_of(shared, tiles));
         }
     }
-    // Items are even shares of the bundles' lists, in one round of the SMs or a few: the less work one after the other, an item's
-    // beginning and end counted as two tiles, the sooner.  No share is less than a tile.
+    // Items are even shares of the bundles' lists, in one round of the SMs or a few, or whole lists: the less work one after the other,
+    // an item's beginning and end counted as two tiles, the sooner.  No share is less than a tile.
     auto items_of = [&](uint32_t share) {
         uint64_t n = 0;
         for (uint32_t i = 0; i < p.n_bundles; ++i) {
@@ -945,14 +965,15 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
         return n;
     };
     uint32_t share = longest, best = ~0u;
-    for (uint32_t rounds = 1; rounds <= 4; ++rounds) {
+    for (uint32_t rounds = 1; rounds <= 5; ++rounds) {
         uint32_t lo = 4, hi = std::max(longest, 4u);             // the smallest share that makes no more items than that
         while (lo < hi) {
             const uint32_t mid = (lo + hi) / 2;
             if (items_of(mid) <= (uint64_t)rounds * ctx->sm_count) hi = mid;
             else lo = mid + 1;
         }
-        const uint32_t time = (uint32_t)((items_of(lo) + ctx->sm_count - 1) / ctx->sm_count) * (lo + 8);
+        if (rounds == 5) lo = longest;
+        const uint32_t time = (uint32_t)((items_of(lo) + ctx->sm_count - 1) / ctx->sm_count) * (lo + 8) + (lo < longest ? kMergeCost : 0);
         if (time < best) {
             best = time;
             share = lo;
@@ -965,7 +986,7 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
         b.item0 = p.items;
         b.part0 = (uint32_t)parts;
         p.items += b.chunks * p.n_kv;
-        parts += (uint64_t)b.chunks * p.n_kv * b.nq;
+        if (b.chunks > 1) parts += (uint64_t)b.chunks * p.n_kv * b.nq;
     }
     if (parts > 0x7fffffffu) return WR_CUDA_ERR_LIMIT;
     // counters first: they are zeros between launches
@@ -977,6 +998,7 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
     p.sched = reinterpret_cast<int *>(ws);
     p.done = reinterpret_cast<int *>(ws + 256);
     p.rows = n_sess * n_q;
+    p.parts = (uint32_t)parts;
     p.ml = reinterpret_cast<float2 *>(ws + head);
     p.o = reinterpret_cast<float *>(ws + head + ml);
     p.q = dq;
