@@ -158,23 +158,40 @@ __device__ __forceinline__ uint32_t position_of(const SharedParams &p, const Bun
 {
     return p.shared_rows[b.group] + p.own_rows[session] - 1;
 }
+// What a new key is rotated by: a lane has dims 2 x lane and the next.  (Kept from row to row: the beams of a search are at one position,
+// and the angles took 2 us where a work item appends two rows.)
+struct Angles {
+    uint32_t position;
+    float sn[2], cs[2];
+};
+__device__ __noinline__ float4 angles_at(float theta, uint32_t position, uint32_t d)
+{
+    const float ln_theta = wrmath::log_ref(theta);
+    float4 x;
+    wrmath::rope_angle(position, d, kHd, ln_theta, x.x, x.z);
+    wrmath::rope_angle(position, d + 1, kHd, ln_theta, x.y, x.w);
+    return x;
+}
+__device__ __forceinline__ void turn_to(const SharedParams &p, Angles &a, uint32_t position, uint32_t lane)
+{
+    if (!p.n_rot || a.position == position) return;
+    const float4 x = angles_at(p.theta, position, 2 * lane);
+    a = {position, {x.x, x.y}, {x.z, x.w}};
+}
 // A session's new row of one kv head into its page, as wr_cuda_kv_append stores it (kernels.c:1406-1407, products rounded
 // separately; quant.c:121-136): a warp, two pairs of dims to a lane.  Bulk copies that lane 0 issues afterwards see it.
-__device__ __forceinline__ void append_row(const SharedParams &p, const Bundle &b, uint32_t session, uint32_t kvh, uint32_t which, uint32_t lane)
+__device__ __forceinline__ void append_row(const SharedParams &p, uint32_t session, uint32_t kvh, uint32_t which, const Angles &a, uint32_t lane)
 {
     const uint32_t row = p.own_rows[session] - 1, d = 2 * lane;
     const float *const x = (which ? p.v_new : p.k_new) + ((size_t)session * p.n_kv + kvh) * kHd;
     float lo[2] = {x[d], x[d + 1]}, hi[2] = {x[d + kHd / 2], x[d + 1 + kHd / 2]};
     if (!which && p.n_rot) {
-        const float ln_theta = wrmath::log_ref(p.theta);
 #pragma unroll
         for (uint32_t e = 0; e < 2; ++e) {
             if (d + e >= p.n_rot) continue;
-            float sn, cs;
-            wrmath::rope_angle(position_of(p, b, session), d + e, kHd, ln_theta, sn, cs);
             const float u = lo[e], v = hi[e];
-            lo[e] = wrmath::sub(wrmath::mul(u, cs), wrmath::mul(v, sn));
-            hi[e] = wrmath::add(wrmath::mul(u, sn), wrmath::mul(v, cs));
+            lo[e] = wrmath::sub(wrmath::mul(u, a.cs[e]), wrmath::mul(v, a.sn[e]));
+            hi[e] = wrmath::add(wrmath::mul(u, a.sn[e]), wrmath::mul(v, a.cs[e]));
         }
     }
     char *const block = reinterpret_cast<char *>(p.own_pages[session][row / kPageTokens]) + wr_block_off(kvh, which, kHd);
@@ -380,26 +397,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
     tc5::fence_before();
     __syncthreads();
     tc5::fence_after();
-    // What the kernel before this one may still be writing waits for it.  With p.early that is not the shared rows: the loading warps
-    // request the first tiles of these at once.
-    // The others work out the addresses of their first queries before they wait.
-    const bool loads = warp == 0 || warp == 2;
-    bool waited = loads && !p.early;
-    if (loads) {
-        const Place at = place_at(p, p.bundle[first.bundle], first.tile0);
-        bool two;
-        const uint64_t *const table = pages_of(p, p.bundle[first.bundle], at, two);
-        asm volatile("" ::"l"(table));                           // (worked out here: the arguments' way into the constant cache)
-    }
-    if (waited) pdl_wait();
-    if (waited) pdl_trigger();           // (only now: what starts early behind this may rely on everything before it)
+    // What the kernel before this one may still be writing waits for it, as late as can be.  With p.early that is not the shared rows.
+    bool waited = false;
     auto wait_before = [&](bool need) {
         if (need && !waited) pdl_wait();
         waited |= need;
     };
     // The first queries are asked for before a whole ring of keys and values is: behind that they came 1 us later.
     auto queries_first = [&]() { asm volatile("bar.sync 7, %0;" ::"n"(64 + 128 * kGroups) : "memory"); };
-    if (loads && !p.early) queries_first();
     const uint32_t tmem = sm.tmem;
     const long long limit = p.wait_limit;
     // Item number `it` of this CTA (the first is its own number); the loading warp is at most four items ahead of the slowest reader.
@@ -415,6 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
         uint32_t n = 0;
         bool ok = true;
         uint32_t next = 0;
+        Angles angles = {~0u, {}, {}};
         for (uint32_t it = 0; ok; ++it) {
             const Item im = it ? item_of(p, next) : first;
             if (lane == 0) {
@@ -425,12 +431,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             const Bundle &bd = p.bundle[im.bundle];
             Place at = place_at(p, bd, im.tile0);
             for (uint32_t t = 0; t < im.tiles; ++t, ++n, step(p, bd, at)) {
-                if (p.early && n == 1) queries_first();
-                wait_before(at.segment != 0);
-                if (appends(p, bd, at)) append_row(p, bd, bd.row0 + at.segment - 1, im.kvh, 0, lane);
+                bool two;
+                const bool add = appends(p, bd, at);
+                if (add) turn_to(p, angles, position_of(p, bd, bd.row0 + at.segment - 1), lane);
+                const uint64_t *const table = pages_of(p, bd, at, two);
+                asm volatile("" ::"l"(table));                   // (worked out before the wait)
+                wait_before(at.segment != 0 || !p.early);
+                if (n == p.early) queries_first();
+                if (add) append_row(p, bd.row0 + at.segment - 1, im.kvh, 0, angles, lane);
                 const uint32_t st = n % kKSlots;
-                bool two;                                        // (the pages' addresses are there when the slot is free)
-                const uint64_t *table = pages_of(p, bd, at, two), page[2] = {table[0], two ? table[1] : 0};
+                const uint64_t page[2] = {table[0], two ? table[1] : 0};      // (there when the slot is free)
                 if (n >= kKSlots && !mbar_wait_warp(&sm.k_free[st], (n / kKSlots - 1) & 1, limit)) {
                     ok = false;
                     break;
@@ -469,12 +479,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             const Bundle &bd = p.bundle[im.bundle];
             Place at = place_at(p, bd, im.tile0);
             for (uint32_t t = 0; t < im.tiles; ++t, ++n, step(p, bd, at)) {
-                if (p.early && n == 1) queries_first();
-                wait_before(at.segment != 0);
-                if (appends(p, bd, at)) append_row(p, bd, bd.row0 + at.segment - 1, im.kvh, 1, lane);
-                const uint32_t st = n % v_ring;
                 bool two;
-                const uint64_t *table = pages_of(p, bd, at, two), page[2] = {table[0], two ? table[1] : 0};
+                const uint64_t *const table = pages_of(p, bd, at, two);
+                asm volatile("" ::"l"(table));
+                wait_before(at.segment != 0 || !p.early);
+                if (n == p.early) queries_first();
+                if (appends(p, bd, at)) append_row(p, bd.row0 + at.segment - 1, im.kvh, 1, Angles{}, lane);
+                const uint32_t st = n % v_ring;
+                const uint64_t page[2] = {table[0], two ? table[1] : 0};
                 if (n >= v_ring && !mbar_wait_warp(&sm.v_free[st], (n / v_ring - 1) & 1, limit)) {
                     ok = false;
                     break;
@@ -577,7 +589,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             }
             if (it == 0) asm volatile("bar.arrive 7, %0;" ::"n"(64 + 128 * kGroups) : "memory");
             if (p.n_rot) {                                       // (as wr_cuda_kv_append rotates them)
-                const float ln_theta = wrmath::log_ref(p.theta);
                 uint32_t of = ~0u;
                 float cs[4], sn[4];                              // of dims 4 (lane % 16) .. + 3 and those 64 on
 #pragma unroll
@@ -585,9 +596,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                     const uint32_t session = over_heads(bd, r0 + u);
                     if (!~from[u]) break;
                     if (session != of) {
-                        float c[2], d[2];
-#pragma unroll
-                        for (uint32_t e = 0; e < 2; ++e) wrmath::rope_angle(position_of(p, bd, bd.row0 + session), 2 * lane + e, kHd, ln_theta, d[e], c[e]);
+                        const float4 w = angles_at(p.theta, position_of(p, bd, bd.row0 + session), 2 * lane);
+                        const float c[2] = {w.z, w.w}, d[2] = {w.x, w.y};
 #pragma unroll
                         for (uint32_t e = 0; e < 4; ++e) {
                             const uint32_t from = 2 * (lane & 15) + e / 2;
@@ -654,8 +664,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             for (uint32_t j = 0; j < H; ++j) o[j] = l[j] = 0.f;
             // O^T of a finished tile, which columns [lo, hi) attended to (another session's values stay out of the others' sums even
             // where they are not numbers); then the change of reference that the tile behind it made.
-            auto add_values = [&](uint32_t tile, bool own, int lo, int hi) {
-                if (!own || (hi > 0 && lo < (int)H)) {
+            auto add_values = [&](uint32_t tile, int lo, int hi) {
+                if (hi > 0 && lo < (int)H) {
+                    const bool all = lo <= 0 && hi >= (int)H;
                     const uint32_t at = tmem + kTmemO + (tile & 1) * 2 * kMaxQ + lanes + q0;
 #pragma unroll
                     for (uint32_t j0 = 0; j0 < H; j0 += V) {     // (eight at a time: more at once do not fit the registers)
@@ -666,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
 #pragma unroll
                         for (uint32_t j = 0; j < V; ++j)
                             if (fabsf(high[j]) != INFINITY) high[j] += low[j];   // (as in scores)
-                        if (!own) {
+                        if (all) {
 #pragma unroll
                             for (uint32_t j = 0; j < V; j += 2) add2(o[j0 + j], o[j0 + j + 1], high[j], high[j + 1]);
                         } else {
@@ -714,16 +725,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                 if (ok) ok = mbar_wait_warp(&sm.s_full[n & 1], (n >> 1) & 1, limit);
                 tc5::fence_after();
             };
-            // One tile of `here` keys or more: shared rows, or one session's own, which columns [lo, hi) of this group attend to.
-            auto tile = [&](auto which, uint32_t here, int lo, int hi) {
-                constexpr bool OWN = decltype(which)::value;
+            // One tile of `here` keys or more, which columns [lo, hi) of this group attend to.
+            auto tile = [&](uint32_t here, int lo, int hi) {
                 const uint32_t at = tmem + (n & 1) * 2 * kMaxQ + lanes + q0;
                 float s[H];
                 auto mask = [&]() {
-                    if (!OWN && here >= kTile) return;
+                    if (here >= kTile && lo <= 0 && hi >= (int)H) return;
                     const bool seen = key < here;
 #pragma unroll
-                    for (int j = 0; j < (int)H; ++j) s[j] = seen && (!OWN || (j >= lo && j < hi)) ? s[j] : -INFINITY;
+                    for (int j = 0; j < (int)H; ++j) s[j] = seen && j >= lo && j < hi ? s[j] : -INFINITY;
                 };
                 auto scores = [&](bool infinite) {
                     tmem_ld(at, s);
@@ -802,48 +812,39 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                 }
                 zeros &= ~(1u << (n & 1));
             };
-            const uint32_t rows = p.shared_rows[bd.group], n0 = n, n_end = n + im.tiles;
-            uint32_t left = (rows + kTile - 1) / kTile;          // shared tiles of this item
-            left = min(left - min(left, im.tile0), im.tiles);
-            for (uint32_t here = rows - im.tile0 * kTile, t = 0; t < left; ++t, ++n, here -= kTile) {
+            const uint32_t n0 = n, n_end = n + im.tiles;
+            int lo1 = 0, hi1 = 0, lo2 = 0, hi2 = 0;              // columns of the last tile, of the one before it
+            // (One loop for shared and own tiles, one copy of each of its steps: a kernel of twice the code took 1 to 2 us more.)
+            for (Place at = place_at(p, bd, im.tile0); n < n_end; ++n, step(p, bd, at)) {
+                const int lo = at.segment ? (int)((at.segment - 1) * bd.heads) - (int)q0 : 0, hi = at.segment ? lo + (int)bd.heads : (int)H;
+                const uint32_t here = rows_of(p, bd, at.segment) - at.tile * kTile;
                 await_scores();
-                if (t >= 2) add_values(n - 2, false, 0, 0);
-                tile(std::false_type{}, here, 0, 0);
+                if (n >= n0 + 2) add_values(n - 2, lo2, hi2);
+                moved = false;
+                if (hi > 0 && lo < (int)H) {
+                    tile(here, lo, hi);
+                } else if (!(zeros >> (n & 1) & 1)) {
+                    const uint32_t none[V / 2] = {};
+#pragma unroll
+                    for (uint32_t j = 0; j < H; j += V) {
+                        put(2 * (q0 + j), none);
+                        put(2 * (q0 + j + NQ), none);
+                    }
+                    zeros |= 1u << (n & 1);
+                }
                 if (here < kTile && group == 0) clear_rows(here);
                 hand_over();
+                lo2 = lo1; hi2 = hi1;
+                lo1 = lo; hi1 = hi;
             }
-            int lo1 = 0, hi1 = 0, lo2 = 0, hi2 = 0;              // columns of the last own tile, of the one before it
-            const uint32_t n_own = n;
-            if (n < n_end)
-                for (Place at = place_at(p, bd, im.tile0 + left); n < n_end; ++n, step(p, bd, at)) {
-                    const int lo = (int)((at.segment - 1) * bd.heads) - (int)q0, hi = lo + (int)bd.heads;
-                    const uint32_t here = p.own_rows[bd.row0 + at.segment - 1] - at.tile * kTile;
-                    await_scores();
-                    if (n >= n0 + 2) add_values(n - 2, n >= n_own + 2, lo2, hi2);
-                    moved = false;
-                    if (hi > 0 && lo < (int)H) {
-                        tile(std::true_type{}, here, lo, hi);
-                    } else if (!(zeros >> (n & 1) & 1)) {
-                        const uint32_t none[V / 2] = {};
-#pragma unroll
-                        for (uint32_t j = 0; j < H; j += V) {
-                            put(2 * (q0 + j), none);
-                            put(2 * (q0 + j + NQ), none);
-                        }
-                        zeros |= 1u << (n & 1);
-                    }
-                    if (here < kTile && group == 0) clear_rows(here);
-                    hand_over();
-                    lo2 = lo1; hi2 = hi1;
-                    lo1 = lo; hi1 = hi;
-                }
             // (of either barrier the phase before is known to be over: the scores seen last came behind those values)
-            if (ok && n > n0 + 1) ok = mbar_wait_warp(&sm.o_full[n & 1], ((n - 2) >> 1) & 1, limit);
-            if (ok) ok = mbar_wait_warp(&sm.o_full[(n - 1) & 1], ((n - 1) >> 1) & 1, limit);
-            tc5::fence_after();
-            if (n > n0 + 1) add_values(n - 2, n >= n_own + 2, lo2, hi2);
-            moved = false;
-            add_values(n - 1, n > n_own, lo1, hi1);
+#pragma unroll 1
+            for (uint32_t back = min(im.tiles, 2u); back; --back) {
+                if (ok) ok = mbar_wait_warp(&sm.o_full[(n - back) & 1], ((n - back) >> 1) & 1, limit);
+                tc5::fence_after();
+                moved = moved && back == 2;
+                add_values(n - back, back == 2 ? lo2 : lo1, back == 2 ? hi2 : hi1);
+            }
             const uint32_t used = min(bd.nq - min(bd.nq, q0), H);        // this group's columns that are queries'
             const bool whole = bd.chunks == 1;
             if (!whole) {
