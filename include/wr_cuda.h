@@ -271,7 +271,8 @@ int wr_cuda_kv_reorder(wr_cuda_ctx *ctx, uint32_t n, wr_cuda_kv *const *kv, cons
  * the sums hangs on all lengths of the call.  head_dim 128 only
  * (WR_CUDA_ERR_UNSUPPORTED), no window.  Scratch is kept by the context and grows with the
  * call: make the largest call once before capturing one.  Calls of one context share it, so
- * graphs that hold such calls are launched one after another. */
+ * graphs that hold such calls are launched one after another.  Device memory: out has
+ * nothing in common with what the call reads (WR_CUDA_ERR_INVAL). */
 int wr_cuda_attn_decode_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer,
                                const uint32_t *seq_lens, uint32_t n_groups, const uint32_t *group_sess,
                                const uint32_t *group_rows, const float *q, float *out,
@@ -296,7 +297,8 @@ int wr_cuda_decode_step_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *co
  * with a NaN or +inf; places for which there is none hold score -inf, beam and token
  * 0xffffffff.  Totals are compared in 64 bits and returned in F32.  beams <=
  * WR_CUDA_BATCH_MAX, n_out <= WR_CUDA_BEAM_MAX_OUT, n_groups * beams <= 65535
- * (WR_CUDA_ERR_LIMIT).  Scratch as wr_cuda_attn_decode_shared. */
+ * (WR_CUDA_ERR_LIMIT).  Scratch and device memory as wr_cuda_attn_decode_shared, but with n_out ==
+ * beams out_scores may be scores. */
 #define WR_CUDA_BEAM_MAX_OUT 32
 int wr_cuda_beam_select(wr_cuda_ctx *ctx, uint32_t n_groups, uint32_t beams, uint32_t vocab,
                         const float *logits, const float *scores, uint32_t n_out,

@@ -148,8 +148,74 @@ def test_captured_in_a_graph(ctx):
     check((out[0].cpu().numpy(), out[1].cpu().numpy().view(np.uint32), out[2].cpu().numpy().view(np.uint32)), other, scores, 8)
 
 
-def test_refusals(ctx):
+def test_scores_in_place(ctx):
+    import torch
+    logits, scores = rows(40, 6, 4, 9000)
+    d, s = torch.from_numpy(logits).cuda(), torch.from_numpy(scores).cuda()
+    b, t = (torch.empty((6, 4), dtype=torch.int32, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    ctx.beam_select(d, s, s, b, t)
+    ctx.sync()
+    check((s.cpu().numpy(), b.cpu().numpy().astype(np.uint32), t.cpu().numpy().astype(np.uint32)), logits, scores, 4)
+
+
+def test_many_rows_and_the_widest_choice(ctx):
+    """As many groups as there may be, and 16 beams with 32 places each."""
+    import torch
+    n = 65535
+    for groups, beams, vocab, n_out in ((n, 1, 9, 3), (n // 16, 16, 7, 32)):
+        logits, scores = rows(41 + beams, groups, beams, vocab)
+        d, s = torch.from_numpy(logits).cuda(), torch.from_numpy(scores).cuda()
+        o = torch.empty((groups, n_out), device="cuda"), *(torch.empty((groups, n_out), dtype=torch.int32, device="cuda") for _ in range(2))
+        torch.cuda.synchronize()
+        ctx.beam_select(d, s, *o)
+        ctx.sync()
+        got = [x.cpu().numpy() for x in o]
+        some = [0, 1, 777, groups - 2, groups - 1]
+        check((got[0][some], got[1][some].astype(np.uint32), got[2][some].astype(np.uint32)), logits[some], scores[some], n_out)
+
+
+def test_two_contexts_in_two_threads():
+    """Each context has its own stream and scratch; its calls may come from any thread."""
+    import threading
+    import torch
     import wayruntime_b200 as wr
+    cs = [wr.Context(0) for _ in range(2)]
+    data = [rows(50 + i, 3, 4, 20000 + i) for i in range(2)]
+    bad = []
+
+    def work(i, c):
+        try:
+            for _ in range(20):
+                check(run(c, *data[i], 8), *data[i], 8)
+        except BaseException as e:      # noqa: BLE001 (told to the thread that asserts)
+            bad.append(e)
+    ts = [threading.Thread(target=work, args=(i % 2, cs[i // 2])) for i in range(4)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    torch.cuda.synchronize()
+    assert not bad
+    for c in cs:
+        c.close()
+
+
+def test_refusals(ctx):
+    import torch
+    import wayruntime_b200 as wr
+    both = torch.zeros((2, 2, 10), device="cuda")
+    s, b, t = torch.zeros((2, 2), device="cuda"), *(torch.zeros((2, 3), dtype=torch.int32, device="cuda") for _ in range(2))
+    o = torch.zeros((2, 3), device="cuda")
+    flat = both.view(-1)
+    for bad in ((flat[:6].view(2, 3), b, t), (o, flat[34:].view(torch.int32).view(2, 3), t), (o, b, flat[10:16].view(torch.int32).view(2, 3))):
+        with pytest.raises(wr.WrCudaError) as e:                     # a result in what is read
+            ctx.beam_select(both, s, *bad)
+        assert e.value.status == -4
+    wide = torch.zeros(8, device="cuda")
+    with pytest.raises(wr.WrCudaError) as e:                         # places of other groups' scores
+        ctx.beam_select(both, wide[:4].view(2, 2), wide[:6].view(2, 3), b, t)
+    assert e.value.status == -4
     logits, scores = rows(1, 1, 2, 10)
     out = lambda n: (np.zeros((1, n), np.float32), np.zeros((1, n), np.uint32), np.zeros((1, n), np.uint32))  # noqa: E731
     for bad_logits, bad_scores, n, status in ((logits, scores, 33, -8), (np.zeros((1, 17, 10), np.float32), np.zeros((1, 17), np.float32), 4, -8),

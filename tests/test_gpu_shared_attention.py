@@ -465,6 +465,17 @@ def test_refusals(ctx):
     with pytest.raises(wr.WrCudaError) as e:                          # the row to append lies in a page that both hold
         ctx.decode_step_shared(f.kvs, 0, [100, 215], [(2, 64)], q, np.zeros((2, 2, HD), np.float32), np.zeros((2, 2, HD), np.float32), out, 4)
     assert e.value.status == -7
+    both = torch.zeros(3 * 4 * HD, device="cuda")
+    dq, k, v = both[:2 * 4 * HD].view(2, 4, HD), torch.zeros((2, 2, HD), device="cuda"), torch.zeros((2, 2, HD), device="cuda")
+    far = torch.zeros_like(dq)
+    for o in (dq, both[4 * HD:].view(2, 4, HD)):                      # a result in what is read
+        with pytest.raises(wr.WrCudaError) as e:
+            ctx.attn_decode_shared(f.kvs, 0, f.lens, [(2, 192)], dq, o, 4)
+        assert e.value.status == -4
+    for kk, vv in ((far.view(-1)[:2 * 2 * HD].view(2, 2, HD), v), (k, far.view(-1)[4 * HD:].view(2, 2, HD))):
+        with pytest.raises(wr.WrCudaError) as e:
+            ctx.decode_step_shared(f.kvs, 0, f.lens, [(2, 192)], dq, kk, vv, far, 4)
+        assert e.value.status == -4
     lib, h = ctx._lib, ctx._handles(f.kvs)
     u = ctx._u32s
     p = q.ctypes.data

@@ -905,6 +905,9 @@ int wr_shared_validate(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv,
     if (rc != WR_CUDA_OK) return rc;
     if (kv[0]->hd_at(layer) != kHd) return WR_CUDA_ERR_UNSUPPORTED;
     if (!group_sess || !group_rows || n_groups == 0 || n_groups > n_sess) return WR_CUDA_ERR_INVAL;
+    // (a row of the result may be there before another work item has read its query)
+    const size_t bytes = (size_t)n_sess * n_q * kHd * sizeof(float);
+    if (mem == WR_CUDA_MEM_DEVICE && wr_overlap(q, bytes, out, bytes)) return WR_CUDA_ERR_INVAL;
     uint32_t s = 0;
     for (uint32_t g = 0; g < n_groups; ++g) {
         if (group_sess[g] == 0 || group_sess[g] > n_sess - s || group_rows[g] % kPageTokens) return WR_CUDA_ERR_INVAL;
@@ -1087,6 +1090,8 @@ int wr_decode_step_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *
     for (uint32_t s = 0; s < n_sess; ++s) seq_lens[s] = positions[s] + 1;
     rc = wr_shared_validate(ctx, n_sess, kv, layer, seq_lens, n_groups, group_sess, group_rows, q, out, n_q_heads, mem);
     if (rc != WR_CUDA_OK) return rc;
+    const size_t bytes = (size_t)n_sess * n_q_heads * kHd * sizeof(float), kv_bytes = (size_t)n_sess * kv[0]->n_kv_at(layer) * kHd * sizeof(float);
+    if (mem == WR_CUDA_MEM_DEVICE && (wr_overlap(out, bytes, k_rows, kv_bytes) || wr_overlap(out, bytes, v_rows, kv_bytes))) return WR_CUDA_ERR_INVAL;
     // (a group's rows end before the row that is appended: what it shares is read only)
     for (uint32_t g = 0, s = 0; g < n_groups; s += group_sess[g++])
         for (uint32_t i = s; i < s + group_sess[g]; ++i)

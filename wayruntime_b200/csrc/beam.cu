@@ -444,6 +444,12 @@ extern "C" int wr_cuda_beam_select(wr_cuda_ctx *ctx, uint32_t n_groups, uint32_t
     a.n_out = n_out;
     a.ld = vocab;
     if (mem == WR_CUDA_MEM_DEVICE) {
+        // (a request's choice may be there before another's rows have been read; its own scores have been)
+        const size_t rows = (size_t)n_groups * beams, outs = (size_t)n_groups * n_out * 4;
+        for (const void *out : {(const void *)out_scores, (const void *)out_beams, (const void *)out_tokens})
+            if (wr_overlap(out, outs, logits, rows * vocab * 4) ||
+                (wr_overlap(out, outs, scores, rows * 4) && !(out == scores && out == out_scores && n_out == beams)))
+                return WR_CUDA_ERR_INVAL;
         a.logits = logits;
         a.scores = scores;
         a.out_scores = out_scores;

@@ -31,6 +31,12 @@ inline bool wr_kv_writable(const wr_cuda_kv *kv, uint32_t row0, uint32_t n)
     return true;
 }
 
+// Whether two ranges of device memory have bytes in common.
+inline bool wr_overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes)
+{
+    return (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
+}
+
 int wr_shared_validate(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer, const uint32_t *seq_lens,
                        uint32_t n_groups, const uint32_t *group_sess, const uint32_t *group_rows, const void *q, const void *out,
                        uint32_t n_q, int mem);

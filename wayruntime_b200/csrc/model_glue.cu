@@ -479,7 +479,7 @@ static uint32_t rows_together(const wr_cuda_model *m, uint32_t n_rows, wr_cuda_k
 {
     uint32_t n = 0;
     *n_groups = 0;
-    if (m->hd != 128) return 0;
+    if (m->hd != 128 || m->n_q > 64 * m->n_kv) return 0;
     bool taken[WR_CUDA_BATCH_MAX] = {};
     for (uint32_t r = 0; r < n_rows; ++r) {
         if (taken[r] || kv[r]->columns.empty()) continue;
