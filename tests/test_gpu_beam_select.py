@@ -110,6 +110,18 @@ def test_what_is_masked_ended_or_not_a_number_has_no_continuation(ctx):
     assert (got[1][0] != NONE).sum() == 21 and set(got[1][4]) == {2}
 
 
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+@pytest.mark.parametrize("vocab", [9, 300, 5000, 40000])
+@pytest.mark.parametrize("n_out", [1, 8, 32])
+def test_rows_without_a_finite_sum_beside_others(ctx, bad, vocab, n_out):
+    """One logit of some beams is not finite: their others are no continuations, and take no place from the other beams'."""
+    for beams, spoilt in ((2, [0]), (8, [1, 2, 5]), (16, list(range(0, 16, 2))), (16, list(range(1, 16)))):
+        logits, scores = rows(60 + beams + vocab, 3, beams, vocab)
+        for b in spoilt:
+            logits[:, b, (7 * b) % vocab] = bad
+        check(run(ctx, logits, scores, n_out), logits, scores, n_out)
+
+
 def test_an_ended_beams_row_is_not_read(ctx):
     """Its address may be anything the buffer covers; here NaN, which would take every candidate out if it were read."""
     logits, scores = rows(10, 1, 2, 3000)

@@ -199,7 +199,8 @@ __device__ __forceinline__ void part_of_row(const BeamParams &p, PartMemory &sm,
             s2 = add2(s2, pack2(ex2(d0), ex2(d1)));
         }
         // a threshold from what every thread has seen, looked for again whenever that has doubled
-        if ((b & (b + 1)) == 0) bound = fmaxf(bound_of_all(sm.top[b & 1], m, k, warp, lane), -FLT_MAX);
+        // (not in the words of the last time: some may still be reading those)
+        if ((b & (b + 1)) == 0) bound = fmaxf(bound_of_all(sm.top[__popc(b) & 1], m, k, warp, lane), -FLT_MAX);
         if (top >= bound) {
 #pragma unroll
             for (uint32_t e = 0; e < 4 * kVecs; ++e)
@@ -306,7 +307,8 @@ __device__ __forceinline__ void parts_of_request(const BeamParams &p, FinalMemor
 #pragma unroll
     for (uint32_t u = 0; u < kOwn; ++u) {
         const uint32_t i = threadIdx.x + u * kThreads;
-        total[u] = i < beams * per_beam ? sm.offset[i / per_beam] + (double)__uint_as_float(mine[u].x) : -INFINITY;
+        const double offset = i < beams * per_beam ? sm.offset[i / per_beam] : -INFINITY;
+        total[u] = offset > -INFINITY ? offset + (double)__uint_as_float(mine[u].x) : -INFINITY;      // (no NaN from an infinite logit)
         top = larger(top, total[u]);
     }
     const float bound = fmaxf(bound_of_all(sm.top, __double2float_rd(top), k, warp, lane), -FLT_MAX);
