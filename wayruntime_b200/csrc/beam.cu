@@ -185,9 +185,11 @@ __device__ __forceinline__ void part_of_row(const BeamParams &p, PartMemory &sm,
     const uint32_t batches = first < end ? min(p.batches, (end - first + kBatch - 1) / kBatch) : 0u;
     for (uint32_t b = 0; b < batches; ++b) {
         if (b + 1 < batches) load(b + 1, next);
-        float top = -INFINITY;
+        float tops[kVecs], top = -INFINITY;
 #pragma unroll
-        for (uint32_t e = 0; e < 4 * kVecs; e += 2) top = max3(top, v[e], v[e + 1]);
+        for (uint32_t u = 0; u < kVecs; ++u) tops[u] = max3(fmaxf(v[4 * u], v[4 * u + 1]), v[4 * u + 2], v[4 * u + 3]);
+#pragma unroll
+        for (uint32_t u = 0; u < kVecs; u += 2) top = max3(top, tops[u], tops[u + 1]);
         const float was = m;
         m = fmaxf(m, top);
         const float base = m == -INFINITY ? 0.f : m, shrink = ex2((was - base) * kLog2e);
@@ -203,11 +205,19 @@ __device__ __forceinline__ void part_of_row(const BeamParams &p, PartMemory &sm,
         if ((b & (b + 1)) == 0) bound = fmaxf(bound_of_all(sm.top[__popc(b) & 1], m, k, warp, lane), -FLT_MAX);
         if (top >= bound) {
 #pragma unroll
-            for (uint32_t e = 0; e < 4 * kVecs; ++e)
-                if (v[e] >= bound) {
-                    const uint32_t at = atomicAdd(&sm.n_listed, 1);
-                    if (at < kList) sm.listed[at] = key_of(v[e], token_of(b, e));
-                }
+            for (uint32_t u = 0; u < kVecs; ++u) {
+                if (tops[u] < bound) continue;
+                uint32_t n = 0;
+#pragma unroll
+                for (uint32_t e = 4 * u; e < 4 * u + 4; ++e) n += v[e] >= bound;
+                uint32_t at = atomicAdd(&sm.n_listed, n);
+#pragma unroll
+                for (uint32_t e = 4 * u; e < 4 * u + 4; ++e)
+                    if (v[e] >= bound) {
+                        if (at < kList) sm.listed[at] = key_of(v[e], token_of(b, e));
+                        ++at;
+                    }
+            }
         }
 #pragma unroll
         for (uint32_t e = 0; e < 4 * kVecs; ++e) v[e] = next[e];
