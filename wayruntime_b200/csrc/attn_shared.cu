@@ -10,8 +10,7 @@
 // A BUNDLE is up to 64 queries of one kv head: some sessions of a group, with the query heads that share the kv head.  Its keys
 // are a list of tiles of 128 (two pages): the group's shared rows, then each session's own.  The queries stay where they are for
 // the whole list; in a session's own tiles the other sessions' columns get weights of zero.  (Work items of their own for own
-// rows took 3 to 4 us each for a tile or two: 20.7 us for four groups of four behind 4096 rows, 36.0 for 16 sessions behind
-// 32768; with one list 16.8 and 30.6.)  A WORK ITEM is an even share of a bundle's tiles for one kv head.  Persistent CTAs, one per SM,
+// rows began and ended once more for a tile or two, 3 to 4 us each.)  A WORK ITEM is an even share of a bundle's tiles for one kv head.  Persistent CTAs, one per SM,
 // draw items from a counter, longest first; when none is left they add the shares of a row up in order (add_up), so results do
 // not hang on who worked what out.  Operands are swapped, as in attn_latent.cu: keys are the tensor core's M, queries
 // its N, so a tile costs what its queries cost.  Per tile
@@ -27,6 +26,10 @@
 // one tile stay in the tensor core's accumulator (8 steps of 16 keys behind the small ones), longer ones are F32 additions in
 // registers: the accumulator rounds towards zero, which over a long chunk would show.
 // Every wait is bounded by the context's wait limit.
+// Measured on a B200, F32 rows, 32 query and 8 kv heads, one launch behind another: 16 sessions behind 32768 rows, 145 MB, 34 us, of which
+// the tiles take 23.5 at 6.4 TB/s (the copy bandwidth is 6.54); 4 sessions behind 2011 rows 9.8 us, 2 behind 150 rows 6.6 us on the
+// device.  What the tiles do not take, 10 us of a large launch, is its ends: queries 1.7, the last values 0.9, parts written
+// and seen by the others 2, adding them up 2.5, the rest the launch itself.  Head dim 128 only: a tile's rings take the SM's shared memory.
 #include <algorithm>
 #include <type_traits>
 
@@ -46,7 +49,8 @@ constexpr uint32_t kTmemCols = 512, kTmemO = 256;                               
 constexpr uint32_t kMaxBundles = 64;
 constexpr float kGrow = 8.0f, kLog2e = 1.4426950408889634f;
 
-// A bundle's columns: its queries, rounded up to a size that the groups of threads are made for.
+// A bundle's columns: its queries, rounded up to a size that the groups of threads are made for.  (High and low parts side by side are 32,
+// 64 or 128 columns, 43, 50 or 64 cycles an instruction; fewer cost what 32 do.)
 __host__ __device__ __forceinline__ uint32_t padded(uint32_t nq) { return nq <= 16 ? 16u : nq <= 32 ? 32u : 64u; }
 struct Bundle {
     uint32_t group, row0, sessions;      // its group; its first session, how many
@@ -56,8 +60,9 @@ struct Bundle {
 };
 // x / heads for a column's number, by 65536 / heads rounded up: 64 columns at most, so the remainder does not reach the next number
 __device__ __forceinline__ uint32_t over_heads(const Bundle &b, uint32_t x) { return x * b.inverse >> 16; }
-// Where share i of a bundle's tiles begins.  An own tile's work counts five quarters of a shared one's: 2.0 us against the 1.55 that
-// HBM needs for it (16 sessions behind 32768 rows: 39.8 us with even numbers).
+// Where share i of a bundle's tiles begins.  An own tile's work counts five quarters of a shared one's: where a share begins with own
+// tiles, every session's first one sets its columns' references.  (16 sessions behind 32768 rows, 20 to 300 own ones: 36.7 us, 39.3 with even
+// numbers; behind 6000, 50 to 1500 own ones: 26.3 and 25.5.)
 __host__ __device__ __forceinline__ uint32_t weight_of(uint32_t shared, uint32_t tiles) { return 4 * shared + 5 * (tiles - shared); }
 // (Shares of a weight of five at least have a tile each; or there are as many as tiles.)
 __host__ __device__ __forceinline__ uint32_t shares_of(uint32_t shared, uint32_t tiles, uint32_t share)
@@ -277,7 +282,8 @@ __device__ __forceinline__ uint32_t idesc_values(uint32_t n) { return tc5::idesc
 
 // The parts of a row added up, in order.  The CTAs do this when there is
 // no item left to draw; a team of warps takes a row, waits for its parts (bounded), and has up to 8 x team of them under way at once.
-// (A kernel of its own behind this one: 2 to 3 us more, and the host's time for a launch.)
+// (A kernel of its own behind this one was quicker on the device where there is little to do, 7.6 against 8.7 us for two short sessions,
+// 21.0 against 22.1 for four groups behind 4096 rows, slower behind 32768, 38.4 against 37.8, and cost the host 2.2 us a call.)
 constexpr uint32_t kMergeAhead = 8, kMergeWarps = 4 * kGroups;
 __device__ __forceinline__ bool add_up(const SharedParams &p, float4 *sums, uint32_t warp, uint32_t lane)
 {

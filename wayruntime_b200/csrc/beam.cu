@@ -5,8 +5,10 @@
 // One pass over the logits: a CTA takes a part of a row and leaves the part's sum of exponentials (against the part's
 // maximum) and its n_out best logits; within a row totals are in the order of logits, so nothing else of the part can be
 // among the row's best.  The CTA that is the last of its request puts the parts together: sums and totals in 64 bits,
-// since candidates of two beams may lie closer than an F32 rounding.  HBM bounds it (4 bytes a logit) where there are many
-// rows, round trips where there are few; a second kernel for the parts took 2 us more.
+// since candidates of two beams may lie closer than an F32 rounding.  Measured on a B200: one row of 32003 logits, 8 out, 7.2 us on
+// the device, round trips one behind the other (a second kernel for the parts took 2 us more); 256 rows of 65536, 16 out, 20.4 us,
+// 3.3 TB/s, bound by instructions (comparing with the bound four logits at a time took 1.2 us off; more batches under way, two or three
+// copies to shared memory a CTA, made it 24.7 and 26.0 us).
 //
 // Candidates are found with a threshold that is sure to keep n_out of them: of 32 threads' maxima (distinct elements) the
 // n_out-th largest.  What reaches it goes to a list, what still reaches the last threshold to another, and an entry's place in
@@ -23,7 +25,7 @@ namespace {
 
 constexpr uint32_t kThreads = 256, kWarps = kThreads / 32, kVecs = 4, kBatch = kThreads * kVecs * 4;   // logits a CTA has in hand
 constexpr uint32_t kList = 1024, kOwn = 6, kMaxLists = kOwn * kThreads;       // kOwn: a thread's entries of a request's
-constexpr uint32_t kCtas = 4;             // to an SM
+constexpr uint32_t kCtas = 4;             // to an SM (5, with 48 registers a thread: 256 rows 25.8 us; 16 rows 10.3 instead of 10.9)
 constexpr uint32_t kNone = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -321,7 +323,8 @@ __device__ __forceinline__ void parts_of_request(const BeamParams &p, FinalMemor
         total[u] = offset > -INFINITY ? offset + (double)__uint_as_float(mine[u].x) : -INFINITY;      // (no NaN from an infinite logit)
         top = larger(top, total[u]);
     }
-    const float bound = fmaxf(bound_of_all(sm.top, __double2float_rd(top), k, warp, lane), -FLT_MAX);
+    // (a few are ranked as quickly as a bound is found: 32 / 64 / 128 candidates 6.4 / 7.0 / 8.2 us without, 7.0 / 7.2 / 7.3 with it)
+    const float bound = lists * k <= 64 ? -FLT_MAX : fmaxf(bound_of_all(sm.top, __double2float_rd(top), k, warp, lane), -FLT_MAX);
     auto list = [&](double t, uint32_t b, uint32_t token) {
         if (!(t >= bound)) return;
         const uint32_t at = atomicAdd(&sm.n, 1);
@@ -425,6 +428,7 @@ int wr_beam_launch(wr_cuda_ctx *ctx, const wr_beam_args &a)
     BeamParams p{};
     p.a = a;
     const uint32_t rows = a.groups * a.beams, most = (uint32_t)(((uint64_t)a.vocab + 3 + kBatch - 1) / kBatch);
+    // As many CTAs as the SMs hold at once.  (Twice as many: 26.7 instead of 22.1 us for 256 rows, 11.7 instead of 11.3 for 16.)
     const uint32_t want = std::min(std::max(kCtas * (uint32_t)ctx->sm_count / rows, 1u), std::min(most, kMaxLists / a.beams));
     p.batches = (most + want - 1) / want;
     p.parts = (most + p.batches - 1) / p.batches;
