@@ -26,9 +26,9 @@
 // one tile stay in the tensor core's accumulator (8 steps of 16 keys behind the small ones), longer ones are F32 additions in
 // registers: the accumulator rounds towards zero, which over a long chunk would show.
 // Every wait is bounded by the context's wait limit.
-// Measured on a B200, F32 rows, 32 query and 8 kv heads, one launch behind another: 16 sessions behind 32768 rows, 145 MB, 34 us, of which
-// the tiles take 23.5 at 6.4 TB/s (the copy bandwidth is 6.54); 4 sessions behind 2011 rows 9.8 us, 2 behind 150 rows 6.6 us on the
-// device.  What the tiles do not take, 10 us of a large launch, is its ends: queries 1.7, the last values 0.9, parts written
+// Measured on a B200, F32 rows, 32 query and 8 kv heads, one launch behind another: 16 sessions behind 32768 rows, 145 MB, 33.2 us, of which
+// the tiles take 23.3 at 6.4 TB/s (the copy bandwidth is 6.54; after 50 ms of nothing else the GPU is at its 1000 W, the SMs at 1690
+// instead of 1965 MHz, and it is 39 us); 4 sessions behind 2011 rows 9.5 us, 2 behind 150 rows 6.5 us on the device.  What the tiles do not take, 10 us of a large launch, is its ends: queries 1.7, the last values 0.9, parts written
 // and seen by the others 2, adding them up 2.5, the rest the launch itself.  Head dim 128 only: a tile's rings take the SM's shared memory.
 #include <algorithm>
 #include <type_traits>
@@ -61,8 +61,8 @@ struct Bundle {
 // x / heads for a column's number, by 65536 / heads rounded up: 64 columns at most, so the remainder does not reach the next number
 __device__ __forceinline__ uint32_t over_heads(const Bundle &b, uint32_t x) { return x * b.inverse >> 16; }
 // Where share i of a bundle's tiles begins.  An own tile's work counts five quarters of a shared one's: where a share begins with own
-// tiles, every session's first one sets its columns' references.  (16 sessions behind 32768 rows, 20 to 300 own ones: 36.7 us, 39.3 with even
-// numbers; behind 6000, 50 to 1500 own ones: 26.3 and 25.5.)
+// tiles, every session's first one sets its columns' references.  (16 sessions behind 32768 rows, 20 to 300 own ones: 35.4 us, 36.4 with even
+// numbers; behind 6000, 50 to 1500 own ones: 25.5 and 25.1.)
 __host__ __device__ __forceinline__ uint32_t weight_of(uint32_t shared, uint32_t tiles) { return 4 * shared + 5 * (tiles - shared); }
 // (Shares of a weight of five at least have a tile each; or there are as many as tiles.)
 __host__ __device__ __forceinline__ uint32_t shares_of(uint32_t shared, uint32_t tiles, uint32_t share)
@@ -821,27 +821,30 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
             const uint32_t n0 = n, n_end = n + im.tiles;
             int lo1 = 0, hi1 = 0, lo2 = 0, hi2 = 0;              // columns of the last tile, of the one before it
             // (One loop for shared and own tiles, one copy of each of its steps: a kernel of twice the code took 1 to 2 us more.)
-            for (Place at = place_at(p, bd, im.tile0); n < n_end; ++n, step(p, bd, at)) {
+            // Segment after segment: what does not change within one is not looked up again for every tile.
+            for (Place at = place_at(p, bd, im.tile0); n < n_end; at = {at.segment + 1, 0}) {
                 const int lo = at.segment ? (int)((at.segment - 1) * bd.heads) - (int)q0 : 0, hi = at.segment ? lo + (int)bd.heads : (int)H;
-                const uint32_t here = rows_of(p, bd, at.segment) - at.tile * kTile;
-                await_scores();
-                if (n >= n0 + 2) add_values(n - 2, lo2, hi2);
-                moved = false;
-                if (hi > 0 && lo < (int)H) {
-                    tile(here, lo, hi);
-                } else if (!(zeros >> (n & 1) & 1)) {
-                    const uint32_t none[V / 2] = {};
+                const bool mine = hi > 0 && lo < (int)H;
+                for (int here = (int)(rows_of(p, bd, at.segment) - at.tile * kTile); here > 0 && n < n_end; here -= (int)kTile, ++n) {
+                    await_scores();
+                    if (n >= n0 + 2) add_values(n - 2, lo2, hi2);
+                    moved = false;
+                    if (mine) {
+                        tile((uint32_t)here, lo, hi);
+                    } else if (!(zeros >> (n & 1) & 1)) {
+                        const uint32_t none[V / 2] = {};
 #pragma unroll
-                    for (uint32_t j = 0; j < H; j += V) {
-                        put(2 * (q0 + j), none);
-                        put(2 * (q0 + j + NQ), none);
+                        for (uint32_t j = 0; j < H; j += V) {
+                            put(2 * (q0 + j), none);
+                            put(2 * (q0 + j + NQ), none);
+                        }
+                        zeros |= 1u << (n & 1);
                     }
-                    zeros |= 1u << (n & 1);
+                    if (here < (int)kTile && group == 0) clear_rows((uint32_t)here);
+                    hand_over();
+                    lo2 = lo1; hi2 = hi1;
+                    lo1 = lo; hi1 = hi;
                 }
-                if (here < kTile && group == 0) clear_rows(here);
-                hand_over();
-                lo2 = lo1; hi2 = hi1;
-                lo1 = lo; hi1 = hi;
             }
             const int idx = warp_reduce_many<(int)H>(l, (int)lane);      // (while the last product runs)
             sm.red[q0 + idx][quarter] = l[0];
