@@ -212,14 +212,15 @@ def _buf(x):
     """(address, mem kind, keep-alive) of a numpy array / torch tensor."""
     if x is None:
         return None, None, None
+    address = getattr(x, "data_ptr", None)
+    if address is not None:
+        if not x.is_contiguous():
+            raise ValueError("buffers must be contiguous")
+        return address(), (MEM_DEVICE if x.is_cuda else MEM_HOST), x
     if isinstance(x, np.ndarray):
         if not x.flags["C_CONTIGUOUS"]:
             raise ValueError("buffers must be C-contiguous")
         return x.ctypes.data, MEM_HOST, x
-    if hasattr(x, "data_ptr"):
-        if not x.is_contiguous():
-            raise ValueError("buffers must be contiguous")
-        return x.data_ptr(), (MEM_DEVICE if x.is_cuda else MEM_HOST), x
     raise TypeError(f"unsupported buffer {type(x)}")
 
 
@@ -491,10 +492,12 @@ class Context:
         order of kvs, (sessions, rows that they share) — a list, or a Groups built once."""
         qp, qm, _q = _buf(q)
         op, om, _o = _buf(out)
-        g = Groups.of(groups, len(kvs))
-        _check(self._lib.wr_cuda_attn_decode_shared(self._h, len(kvs), self._handles(kvs), layer, self._u32s(seq_lens), len(g),
-                                                    g.sessions, g.rows, qp, op, n_q_heads, scale, _same_mem(qm, om)),
-               "wr_cuda_attn_decode_shared")
+        n = len(kvs)
+        g = groups if type(groups) is Groups and groups.total == n else Groups.of(groups, n)
+        rc = self._lib.wr_cuda_attn_decode_shared(self._h, n, self._handles(kvs), layer, self._u32s(seq_lens), g.count, g.sessions, g.rows,
+                                                  qp, op, n_q_heads, scale, qm if qm == om else _same_mem(qm, om))
+        if rc:
+            _check(rc, "wr_cuda_attn_decode_shared")
 
     def decode_step_shared(self, kvs, layer, positions, groups, q, k_rows, v_rows, out, n_q_heads, theta=10000.0,
                            n_rot_pairs=0, rope=True, scale=0.0):
@@ -504,11 +507,13 @@ class Context:
         kp, km, _k = _buf(k_rows)
         vp, vm, _v = _buf(v_rows)
         op, om, _o = _buf(out)
-        g = Groups.of(groups, len(kvs))
-        _check(self._lib.wr_cuda_decode_step_shared(self._h, len(kvs), self._handles(kvs), layer, self._u32s(positions), len(g),
-                                                    g.sessions, g.rows, qp, kp, vp, op, n_q_heads, theta, n_rot_pairs,
-                                                    APPEND_ROPE if rope else 0, scale, _same_mem(qm, km, vm, om)),
-               "wr_cuda_decode_step_shared")
+        n = len(kvs)
+        g = groups if type(groups) is Groups and groups.total == n else Groups.of(groups, n)
+        rc = self._lib.wr_cuda_decode_step_shared(self._h, n, self._handles(kvs), layer, self._u32s(positions), g.count, g.sessions, g.rows,
+                                                  qp, kp, vp, op, n_q_heads, theta, n_rot_pairs, APPEND_ROPE if rope else 0, scale,
+                                                  qm if qm == km == vm == om else _same_mem(qm, km, vm, om))
+        if rc:
+            _check(rc, "wr_cuda_decode_step_shared")
 
     def kv_reorder(self, kvs, parents, rows):
         """wr_cuda_kv_reorder: kvs[i] goes on from what kvs[parents[i]] holds; rows[i]: rows that kvs[i] holds before."""
@@ -807,10 +812,10 @@ class Groups:
     def __init__(self, groups):
         self.sessions = Batch.u32([n for n, _ in groups])
         self.rows = Batch.u32([rows for _, rows in groups])
-        self.total = sum(self.sessions)
+        self.count, self.total = len(self.sessions), sum(self.sessions)
 
     def __len__(self):
-        return len(self.sessions)
+        return self.count
 
     @classmethod
     def of(cls, groups, n_sessions):

@@ -816,12 +816,10 @@ int wr_beam_step_launch(wr_cuda_ctx *ctx, wr_cuda_model *m, const wr_beam_step &
                         const uint32_t *row_at)
 {
     const size_t rows = (size_t)b.groups * b.beams, outs = (size_t)b.groups * b.n_out;
-    if (!m->beam_dev) {
-        // (scores in; scores, beams, tokens out: a group has a beam at least and gives 32 continuations at most)
-        constexpr size_t bytes = (WR_CUDA_BATCH_MAX + 3 * WR_CUDA_BATCH_MAX * WR_CUDA_BEAM_MAX_OUT) * 4;
-        WR_CUDA_TRY(cudaHostAlloc((void **)&m->beam_host, bytes, cudaHostAllocDefault));
-        WR_CUDA_TRY(cudaMalloc((void **)&m->beam_dev, bytes));
-    }
+    // (scores in; scores, beams, tokens out: a group has a beam at least and gives 32 continuations at most)
+    constexpr size_t bytes = (WR_CUDA_BATCH_MAX + 3 * WR_CUDA_BATCH_MAX * WR_CUDA_BEAM_MAX_OUT) * 4;
+    if (!m->beam_host) WR_CUDA_TRY(cudaHostAlloc((void **)&m->beam_host, bytes, cudaHostAllocDefault));
+    if (!m->beam_dev) WR_CUDA_TRY(cudaMalloc((void **)&m->beam_dev, bytes));
     wr_beam_args a{};
     a.logits = logits;
     a.ld = ld;
