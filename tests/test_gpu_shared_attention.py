@@ -381,6 +381,24 @@ def test_many_query_heads_to_a_kv_head(ctx):
         fam.close()
 
 
+@pytest.mark.parametrize("own, rows", [([1] * 16, 64), ([1] * 16, 0), ([40, 1, 200, 64] * 4, 64)])
+def test_more_short_lists_than_multiprocessors(ctx, own, rows):
+    """16 sessions with 128 query heads to each of 8 kv heads are 256 lists of a tile or two; launch behind launch."""
+    import torch
+    hq, hkv = 1024, 8
+    fam = Family(ctx, 1500, 64, own, hkv)
+    q = _gen.normal(1510, (16, hq, HD))
+    dq = torch.from_numpy(q).cuda()
+    out = torch.full((6, 16, hq, HD), float("nan"), device="cuda")
+    torch.cuda.synchronize()
+    for o in out:
+        ctx.attn_decode_shared(fam.kvs, 0, fam.lens, [(16, rows)], dq, o, hq)
+    ctx.sync()
+    check(out[0].cpu().numpy(), [fam], q)
+    assert all(torch.equal(o, out[0]) for o in out)
+    fam.close()
+
+
 def test_a_wait_that_ran_out_elsewhere_does_not_stay(ctx):
     """An exchange whose peer never answers ends with an error (its wait is short); the calls behind it give the right answer."""
     import torch

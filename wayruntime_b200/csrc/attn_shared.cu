@@ -409,8 +409,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
         if (need && !waited) pdl_wait();
         waited |= need;
     };
-    // The first queries are asked for before a whole ring of keys and values is: behind that they came 1 us later.
-    auto queries_first = [&]() { asm volatile("bar.sync 7, %0;" ::"n"(64 + 128 * kGroups) : "memory"); };
+    // The first queries are asked for before a whole ring of keys and values is: behind that they came 1 us later.  (The CTA's warps meet
+    // once, in the first item, before any wait for a slot.)
+    bool met = false;
+    auto queries_first = [&](bool now) {
+        if (now && !met) {
+            __syncwarp();
+            asm volatile("bar.sync 7, %0;" ::"n"(64 + 128 * kGroups) : "memory");
+        }
+        met |= now;
+    };
     const uint32_t tmem = sm.tmem;
     const long long limit = p.wait_limit;
     // Item number `it` of this CTA (the first is its own number); the loading warp is at most four items ahead of the slowest reader.
@@ -443,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                 const uint64_t *const table = pages_of(p, bd, at, two);
                 asm volatile("" ::"l"(table));                   // (worked out before the wait)
                 wait_before(at.segment != 0 || !p.early);
-                if (n == p.early) queries_first();
+                queries_first(n == p.early);
                 if (add) append_row(p, bd.row0 + at.segment - 1, im.kvh, 0, angles, lane);
                 const uint32_t st = n % kKSlots;
                 const uint64_t page[2] = {table[0], two ? table[1] : 0};      // (there when the slot is free)
@@ -459,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                     bulk_g2s(ks + st * kSlot + kBox + g * 8192, src + 8192, 8192, &sm.k_full[st]);
                 }
             }
-            if (p.early && it == 0 && im.tiles == 1) queries_first();
+            queries_first(true);
             wait_before(true);                                   // (the counter is the earlier launch's until it has ended)
             if (ok && lane == 0) next = gridDim.x + (uint32_t)atomicAdd(p.sched, 1);
             next = __shfl_sync(0xffffffffu, next, 0);
@@ -489,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                 const uint64_t *const table = pages_of(p, bd, at, two);
                 asm volatile("" ::"l"(table));
                 wait_before(at.segment != 0 || !p.early);
-                if (n == p.early) queries_first();
+                queries_first(n == p.early);
                 if (appends(p, bd, at)) append_row(p, bd.row0 + at.segment - 1, im.kvh, 1, Angles{}, lane);
                 const uint32_t st = n % v_ring;
                 const uint64_t page[2] = {table[0], two ? table[1] : 0};
@@ -503,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                     bulk_g2s(vs + st * kSlot + g * kPageBlock, reinterpret_cast<const char *>(page[g]) + wr_block_off(im.kvh, 1, kHd),
                              kPageBlock, &sm.v_full[st]);
             }
-            if (p.early && it == 0 && im.tiles == 1) queries_first();
+            queries_first(true);
         }
         if (lane == 0) {
             if (!ok) atomicCAS(p.err, 0, 82);
