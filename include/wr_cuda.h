@@ -254,8 +254,8 @@ uint32_t wr_cuda_kv_shared_rows(const wr_cuda_kv *a, const wr_cuda_kv *b);
  * before; a recurrent state has to stand there).  All at once, so parents may name each other.
  * A parent's first child takes its memory over, the others copy the rows that
  * are not shared into what sessions without children held: n sessions of one
- * family (forks, equal max_ctx and layers; WR_CUDA_ERR_INVAL), whose own rows
- * nobody outside the call holds (WR_CUDA_ERR_STATE).  Enqueues on the context's
+ * family (forks, equal max_ctx and layers; WR_CUDA_ERR_INVAL).  Of the memory that such a
+ * child goes on in, nobody else holds what lies behind the shared rows (WR_CUDA_ERR_STATE).  Enqueues on the context's
  * stream and allocates nothing.  A refused call changes nothing.  Launches that a
  * graph has captured name the memory, not the session: they are captured again after
  * this call, and while the context's stream is being captured it is WR_CUDA_ERR_STATE. */

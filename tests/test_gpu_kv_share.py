@@ -187,6 +187,28 @@ def test_rows_behind_those_that_go_on_are_left_alone(ctx):
     b.close()
 
 
+def test_memory_whose_further_pages_somebody_holds_is_not_taken(ctx):
+    """The child of a session with fewer rows could not go on in it: the page behind them is held by another session too."""
+    import wayruntime_b200 as wr
+    a = ctx.kv_create(2, 2, 128, 300)
+    rows = some(300, 200, 2, 2, 128)
+    write(a, 0, rows)
+    short, other = a.fork(64), a.fork(200)
+    with pytest.raises(wr.WrCudaError) as e:
+        ctx.kv_reorder([short, a, other], [0, 0, 2], [64, 200, 200])
+    assert e.value.status == -7
+    for kv, n in ((short, 64), (a, 200), (other, 200)):
+        assert holds(kv, cut(rows, n))
+    other.close()
+    ctx.kv_reorder([short, a], [0, 0], [64, 200])
+    more = some(310, 70, 2, 2, 128)
+    for kv in (short, a):
+        assert holds(kv, cut(rows, 64))
+        write(kv, 64, more)
+        assert holds(kv, joined(cut(rows, 64), more))
+        kv.close()
+
+
 def test_refusals_change_nothing(ctx):
     import torch
     import wayruntime_b200 as wr

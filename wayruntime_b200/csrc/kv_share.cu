@@ -250,8 +250,9 @@ extern "C" int wr_cuda_kv_reorder(wr_cuda_ctx *ctx, uint32_t n, wr_cuda_kv *cons
         taken[to] = true;
         holds[i] = to;
         const uint32_t common = wr_kv_common_pages(kv[from], kv[to]);
-        if (rows[from] > common * kPageTokens && !wr_kv_writable(kv[to], common * kPageTokens, rows[from] - common * kPageTokens))
-            return WR_CUDA_ERR_STATE;
+        // (not only the rows to copy: the session goes on behind them)
+        const uint32_t own = std::min(common * kPageTokens, rows[from]);
+        if (!wr_kv_writable(kv[to], own, kv[to]->max_ctx - own)) return WR_CUDA_ERR_STATE;
         pairs[copies] = {kv[from]->d_pages, kv[to]->d_pages, common, rows[from]};
         if (slots[i] >= 0) {
             states.from[copies] = (const char *)kv[from]->state[slots[i]];
