@@ -160,6 +160,15 @@ def test_captured_in_a_graph(ctx):
     check((out[0].cpu().numpy(), out[1].cpu().numpy().view(np.uint32), out[2].cpu().numpy().view(np.uint32)), other, scores, 8)
 
 
+@pytest.mark.parametrize("vocab", [1000, 5000, 16000, 32003])
+@pytest.mark.parametrize("apart", [0.0, 3.0, 200.0])
+def test_the_widest_choice_of_beams_far_apart(ctx, vocab, apart):
+    """16 beams, 32 out: the weakest beam's best is far below what is chosen, and the last part of a row has a few logits only."""
+    logits, scores = rows(70, 2, 16, vocab)
+    scores -= apart * np.arange(16, dtype=np.float32)
+    check(run(ctx, logits, scores, 32), logits, scores, 32)
+
+
 def test_scores_in_place(ctx):
     import torch
     logits, scores = rows(40, 6, 4, 9000)

@@ -11,9 +11,9 @@
 // copies to shared memory a CTA, made it 24.7 and 26.0 us).
 //
 // Candidates are found with a threshold that is sure to keep n_out of them: of 32 threads' maxima (distinct elements) the
-// n_out-th largest.  What reaches it goes to a list, what still reaches the last threshold to another, and an entry's place in
-// the result is the number of better ones there.  Where a list runs over (rows of few values) the best are taken one after the
-// other instead.
+// n_out-th largest.  What reaches it goes to a list; where that are many, a higher threshold is looked for by halving; and an entry's
+// place in the result is the number of better ones in the list.  Where a list runs over (rows of few values) the best are taken one
+// after the other instead.
 // Ties go to the lower beam, then the lower token.  Logits of -inf are no candidates, nor is anything of a beam whose score is
 // -inf or NaN (its row is not read) or whose sum is not finite (a NaN or +inf among its logits).
 #include <cfloat>
@@ -27,6 +27,7 @@ constexpr uint32_t kThreads = 256, kWarps = kThreads / 32, kVecs = 4, kBatch = k
 constexpr uint32_t kList = 1024, kOwn = 6, kMaxLists = kOwn * kThreads;       // kOwn: a thread's entries of a request's
 constexpr uint32_t kCtas = 4;             // to an SM (5, with 48 registers a thread: 256 rows 25.8 us; 16 rows 10.3 instead of 10.9)
 constexpr uint32_t kNone = 0xffffffffu;
+static_assert(kList / WR_CUDA_BEAM_MAX_OUT >= WR_CUDA_BEAM_MAX_OUT, "");
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct BeamParams {
@@ -40,11 +41,13 @@ struct BeamParams {
 struct PartMemory {
     uint64_t listed[kList], kept[kList]; // keys
     float top[2][32], warp_m[kWarps], warp_s[kWarps];
+    uint32_t count[2][kWarps];
     uint32_t n_listed, n_kept;
 };
 struct FinalMemory {
     double offset[WR_CUDA_BATCH_MAX];
     float top[32];
+    uint32_t count[2][kWarps], most[kWarps];
     uint64_t t[kList], at[kList];        // totals in the order of whole numbers; beam and token
     uint32_t n;
 };
@@ -137,6 +140,26 @@ __device__ __forceinline__ void join(float &m, float &s, float m2, float s2)
     const float t = fmaxf(m, m2), base = t == -INFINITY ? 0.f : t;
     s = s * ex2((m - base) * kLog2e) + s2 * ex2((m2 - base) * kLog2e);
     m = t;
+}
+
+// A bound, as the whole number in whose order it is, that k entries reach as well as the given one, but no more than `enough` where such a one
+// is found: halving what lies between that and the largest.  reach(x): how many of the thread's own reach x.  The CTA meets in it.
+template <typename Reach> __device__ __forceinline__ uint32_t higher_bound(uint32_t (&counts)[2][kWarps], Reach reach, uint32_t lo, uint32_t hi, uint32_t k,
+                                                                           uint32_t enough, uint32_t warp, uint32_t lane)
+{
+    uint32_t mid = lo;
+    for (uint32_t turn = 0;; ++turn) {
+        uint32_t n = __reduce_add_sync(0xffffffffu, reach(mid));
+        if (lane == 0) counts[turn & 1][warp] = n;
+        __syncthreads();
+        n = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w) n += counts[turn & 1][w];
+        if (turn && n < k) hi = mid;
+        else lo = mid;
+        if ((n <= enough && (n >= k || !turn)) || hi - lo <= 1 || hi < lo) return lo;
+        mid = lo + (hi - lo) / 2;
+    }
 }
 
 __device__ __forceinline__ void part_of_row(const BeamParams &p, PartMemory &sm, uint32_t part, uint32_t row)
@@ -244,11 +267,25 @@ __device__ __forceinline__ void part_of_row(const BeamParams &p, PartMemory &sm,
     }
     uint32_t n = sm.n_listed;
     if (n <= kList) {
+        // As many comparisons to an entry as there are entries: fewer first, those that reach the last bound or, where these are many (a part
+        // of which some warps have little; 16 beams of 5000 logits, 32 out: 53 us), a higher one.
         const uint64_t *list = sm.listed;
-        if (batches > 1) {                                       // (as many comparisons to an entry as there are entries: fewer first)
-            const uint64_t least = key_of(bound, kNone);
+        const uint32_t enough = 5 * k;
+        uint32_t least = (uint32_t)(key_of(bound, 0) >> 32);
+        if (n > enough) {
+            auto reach = [&](uint32_t x) {
+                uint32_t c = 0;
+                for (uint32_t i = threadIdx.x; i < n; i += kThreads) c += (uint32_t)(sm.listed[i] >> 32) >= x;
+                return c;
+            };
+            float most = sm.warp_m[0];
+#pragma unroll
+            for (uint32_t w = 1; w < kWarps; ++w) most = fmaxf(most, sm.warp_m[w]);
+            least = higher_bound(sm.count, reach, least, (uint32_t)(key_of(most, 0) >> 32), k, enough, warp, lane);
+        }
+        if (batches > 1 || n > enough) {
             for (uint32_t i = threadIdx.x; i < n; i += kThreads)
-                if (sm.listed[i] >= least) sm.kept[atomicAdd(&sm.n_kept, 1)] = sm.listed[i];
+                if ((uint32_t)(sm.listed[i] >> 32) >= least) sm.kept[atomicAdd(&sm.n_kept, 1)] = sm.listed[i];
             __syncthreads();
             n = sm.n_kept;
             list = sm.kept;
@@ -324,7 +361,28 @@ __device__ __forceinline__ void parts_of_request(const BeamParams &p, FinalMemor
         top = larger(top, total[u]);
     }
     // (a few are ranked as quickly as a bound is found: 32 / 64 / 128 candidates 6.4 / 7.0 / 8.2 us without, 7.0 / 7.2 / 7.3 with it)
-    const float bound = lists * k <= 64 ? -FLT_MAX : fmaxf(bound_of_all(sm.top, __double2float_rd(top), k, warp, lane), -FLT_MAX);
+    float bound = -FLT_MAX;
+    if (lists * k > 64) {
+        // (No more lists than fill the list.  A warp's totals are one beam's or two: of a beam that is far behind, the four largest are a low bound.  16 beams of 32003 logits, 32
+        // out: 1536 candidates reached it, more than the list holds, 115 instead of 15.6 us.)
+        const float most = __double2float_rd(top);
+        bound = fmaxf(bound_of_all(sm.top, most, k, warp, lane), -FLT_MAX);
+        auto reach = [&](uint32_t x) {
+            const float least = value((int)(x ^ 0x80000000u));
+            uint32_t n = 0;
+#pragma unroll
+            for (uint32_t u = 0; u < kOwn; ++u) n += total[u] >= least;
+            return n;
+        };
+        const uint32_t largest = __reduce_max_sync(0xffffffffu, (uint32_t)order(most) ^ 0x80000000u);
+        if (lane == 0) sm.most[warp] = largest;
+        __syncthreads();
+        uint32_t hi = sm.most[0];
+#pragma unroll
+        for (uint32_t w = 1; w < kWarps; ++w) hi = max(hi, sm.most[w]);
+        const uint32_t from = (uint32_t)order(bound) ^ 0x80000000u;
+        bound = value((int)(higher_bound(sm.count, reach, from, hi, k, few ? 5 * k : kList / k, warp, lane) ^ 0x80000000u));
+    }
     auto list = [&](double t, uint32_t b, uint32_t token) {
         if (!(t >= bound)) return;
         const uint32_t at = atomicAdd(&sm.n, 1);
