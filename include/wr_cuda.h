@@ -436,8 +436,8 @@ uint64_t wr_cuda_model_last_enqueue_ns(const wr_cuda_model *m);
  * sessions, one new token each; prefill: n_rows <= max_rows tokens of one
  * session), KV appended at `positions` as wr_cuda_decode_step /
  * wr_cuda_kv_append do — the caller commits the new length only when the call
- * returns 0.  A token id >= vocab is WR_CUDA_ERR_INVAL before anything runs
- * (session.c:413).  Results are written for rows [out_from, n_rows), all to
+ * returns 0.  A token id >= vocab (session.c:413) or a session given twice is
+ * WR_CUDA_ERR_INVAL before anything runs.  Results are written for rows [out_from, n_rows), all to
  * host memory, each pointer optional: hidden_out [n][hidden] (the residual
  * stream before the final norm), normed_out [n][hidden], logits_out[i] ->
  * [vocab] for row out_from+i (an entry may be NULL), argmax_out[i] = the first

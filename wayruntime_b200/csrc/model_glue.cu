@@ -486,7 +486,7 @@ static uint32_t rows_together(const wr_cuda_model *m, uint32_t n_rows, wr_cuda_k
         if (taken[r] || kv[r]->columns.empty()) continue;
         uint32_t pages = ~0u, first = n;
         for (uint32_t t = r + 1; t < n_rows; ++t) {
-            if (taken[t] || kv[t] == kv[r]) continue;
+            if (taken[t]) continue;
             const uint32_t common = wr_kv_common_pages(kv[r], kv[t]);
             if (common * kPageTokens < kTogether) continue;
             if (n == first) rows[n++] = r;
@@ -522,6 +522,9 @@ static int forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_rows
     const uint32_t n_sess = (mode == WR_CUDA_FWD_DECODE) ? n_rows : 1;
     for (uint32_t s = 0; s < n_sess; ++s) {
         if (!kv[s] || kv[s]->n_layers != m->n_layers) return WR_CUDA_ERR_INVAL;
+        // (distinct sessions, here and not only in the launches: a pass divides its rows among several kinds of them)
+        for (uint32_t t = 0; t < s; ++t)
+            if (kv[t] == kv[s]) return WR_CUDA_ERR_INVAL;
         for (uint32_t L = 0; L < m->n_layers; ++L)
             if (kv[s]->n_kv_at(L) != m->n_kv || kv[s]->hd_at(L) != m->hd) return WR_CUDA_ERR_INVAL;
         if (!wr_kv_writable(kv[s], positions[s], mode == WR_CUDA_FWD_DECODE ? 1 : n_rows)) return WR_CUDA_ERR_STATE;
