@@ -551,6 +551,7 @@ static int kv_rows_xfer(wr_cuda_ctx *ctx, wr_cuda_kv *kv, uint32_t layer, int wh
         kv->d_pages + (size_t)layer * kv->n_pages, dbuf, row0, n, n_kv, hd, (uint32_t)which,
         to_cache);
     ctx->launches++;
+    if (to_cache) wr_pdl_rows(ctx);
     WR_CUDA_TRY(cudaGetLastError());
     if (mem == WR_CUDA_MEM_HOST) {
         if (!to_cache)

@@ -76,7 +76,7 @@ bool same_geom(const wr_kv_geom &a, const wr_kv_geom &b)
 }
 
 // Enqueues the copies of all layers, layers with equal pages together.  (Ordinary launches: the rows have been written when
-// they begin, and they are done when anything behind them begins.)
+// they begin.  Who reads the copies waits for them: wr_pdl_rows.)
 int copy_rows(wr_cuda_ctx *ctx, const wr_cuda_kv *of, const copy_pair *pairs, uint32_t n)
 {
     copy_params p;
@@ -102,6 +102,7 @@ int copy_rows(wr_cuda_ctx *ctx, const wr_cuda_kv *of, const copy_pair *pairs, ui
             }
         kv_copy_kernel<<<dim3(pages * p.per_page, m, n), kCopyThreads, 0, ctx->stream>>>(p);
         const int rc = finish_launch(ctx);
+        wr_pdl_rows(ctx);
         if (rc != WR_CUDA_OK) return rc;
     }
     return WR_CUDA_OK;
@@ -111,7 +112,9 @@ int copy_states(wr_cuda_ctx *ctx, const state_params &p, uint32_t n)
     if (!n) return WR_CUDA_OK;
     const uint32_t blocks = (uint32_t)std::min<uint64_t>((p.bytes / 16 + kCopyThreads - 1) / kCopyThreads, 4u * (uint32_t)ctx->sm_count);
     state_copy_kernel<<<dim3(blocks, n), kCopyThreads, 0, ctx->stream>>>(p);
-    return finish_launch(ctx);
+    const int rc = finish_launch(ctx);
+    wr_pdl_rows(ctx);                    // (the rows copied just before it may not be there either)
+    return rc;
 }
 
 // Sessions change hands on the host, which a graph would not do again when it is launched.
@@ -209,7 +212,7 @@ extern "C" int wr_cuda_kv_fork(wr_cuda_ctx *ctx, wr_cuda_kv *kv, uint32_t n_rows
     ctx->live_kv++;
     *out = f;
     // (rows that the last launch of shared attention may still be writing may be shared ones now)
-    if (ctx->pdl_kind == WR_PDL_SHARED) ctx->pdl_kind = WR_PDL_PREFILL_PART;
+    if (ctx->pdl_kind == WR_PDL_SHARED) ctx->pdl_kind = WR_PDL_ROWS;
     return WR_CUDA_OK;
 }
 

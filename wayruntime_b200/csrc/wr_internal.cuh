@@ -129,9 +129,16 @@ struct wr_cuda_ctx {
 };
 // NONE says that nothing before the kernel that asks can still be running; a kernel that lets the next one start early
 // and does not cover every SM (PREFILL_PART) is something else: behind it the prompt append may still be writing pages.
-// Shared attention with an append (SHARED) writes pages itself.
+// Shared attention with an append (SHARED) writes pages itself.  So do ordinary launches that fill rows (ROWS: write_rows, the copies of
+// forks and reordering): behind them a kernel can begin when their CTAs have left, but sees what they stored only behind its wait.
 enum { WR_PDL_NONE = 0, WR_PDL_APPEND = 1, WR_PDL_DECODE_FULL = 2, WR_PDL_DECODE_PART = 3, WR_PDL_PREFILL_FULL = 4,
-       WR_PDL_PREFILL_PART = 5, WR_PDL_SHARED = 6 };
+       WR_PDL_PREFILL_PART = 5, WR_PDL_SHARED = 6, WR_PDL_ROWS = 7 };
+// The launch counted last has filled rows of pages.
+inline void wr_pdl_rows(wr_cuda_ctx *ctx)
+{
+    ctx->pdl_kind = WR_PDL_ROWS;
+    ctx->pdl_index = ctx->launches;
+}
 
 // What one layer of a session keeps: K/V pages, a recurrent state, both or neither.
 struct wr_kv_layer {
