@@ -1041,8 +1041,9 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
     }
     const uint32_t grid = std::min<uint32_t>(p.items, (uint32_t)ctx->sm_count);
     // Behind another launch of this kernel, which writes rows that one session alone holds (a fork in between counts as another
-    // kind of launch) and lets the next begin when all before it has ended.
-    p.early = settled && dependent && ctx->pdl_index == ctx->launches && ctx->pdl_kind == WR_PDL_SHARED;
+    // kind of launch) and lets the next begin when all before it has ended.  Both run, or both are nodes of one graph.
+    const unsigned long long capture = wr_ctx_capture(ctx);
+    p.early = settled && dependent && ctx->pdl_index == ctx->launches && ctx->pdl_kind == WR_PDL_SHARED && ctx->pdl_capture == capture;
     for (uint32_t i = 0; i < p.n_bundles; ++i) p.widest = std::max(p.widest, p.bundle[i].columns);
     // a row's team: as many warps as there are for all rows at once
     for (p.team = kMergeWarps; p.team > 1 && (uint64_t)p.rows * p.team > (uint64_t)grid * kMergeWarps;) p.team /= 2;
@@ -1050,6 +1051,7 @@ int wr_shared_launch(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, u
     ctx->launches++;
     ctx->pdl_kind = WR_PDL_SHARED;
     ctx->pdl_index = ctx->launches;
+    ctx->pdl_capture = capture;
     WR_CUDA_TRY(cudaGetLastError());
     return WR_CUDA_OK;
 }

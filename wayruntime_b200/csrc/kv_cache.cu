@@ -260,6 +260,17 @@ int wr_ctx_try_ws(wr_cuda_ctx *ctx, size_t ws_bytes)
     return WR_CUDA_OK;
 }
 
+unsigned long long wr_ctx_capture(wr_cuda_ctx *ctx)
+{
+    cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(ctx->stream, &s, &id) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return ~0ull;                    // (a capture gone wrong)
+    }
+    return s == cudaStreamCaptureStatusNone ? 0 : id;
+}
+
 int wr_ctx_keep(wr_cuda_ctx *ctx, size_t bytes, char **out)
 {
     if (bytes > ctx->kept_bytes) {

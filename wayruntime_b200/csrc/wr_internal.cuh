@@ -126,6 +126,7 @@ struct wr_cuda_ctx {
     // while pdl_index == launches (nothing of ours was launched since).
     uint64_t pdl_index = ~0ull;
     int pdl_kind = 0;                // WR_PDL_*
+    unsigned long long pdl_capture = 0;      // (SHARED) the capture it went into, 0: none
 };
 // NONE says that nothing before the kernel that asks can still be running; a kernel that lets the next one start early
 // and does not cover every SM (PREFILL_PART) is something else: behind it the prompt append may still be writing pages.
@@ -234,6 +235,9 @@ int wr_ctx_sync_checked(wr_cuda_ctx *ctx);
 int wr_ctx_reserve_ws(wr_cuda_ctx *ctx, size_t ws_bytes, size_t tickets);
 // The workspace for callers that can do without: where memory does not suffice it stays as it is, and nothing waits.
 int wr_ctx_try_ws(wr_cuda_ctx *ctx, size_t ws_bytes);
+// Number of the capture that the context's stream is in, 0: none.  (A launch that is captured has not run: what a launch
+// outside its capture may skip on account of it hangs on what really comes before.)
+unsigned long long wr_ctx_capture(wr_cuda_ctx *ctx);
 // Scratch that stays where it is for the context's life: a larger call gets more, elsewhere.  Its first WR_KEPT_HEAD bytes are
 // counters that every launch leaves as zeros (and wr_ctx_sync_checked makes zeros again when a kernel has given up): shared
 // attention's in the first half, those of 65536 requests' beams in the second.
