@@ -270,7 +270,7 @@ int wr_cuda_kv_reorder(wr_cuda_ctx *ctx, uint32_t n, wr_cuda_kv *const *kv, cons
  * values as wr_cuda_attn_decode, to rounding: F32 queries and F32 sums, and the order of
  * the sums hangs on all lengths of the call.  head_dim 128 only
  * (WR_CUDA_ERR_UNSUPPORTED), no window.  Scratch is kept by the context and grows with the
- * call: make the largest call once before capturing one.  Calls of one context share it, so
+ * call: make the largest call once before capturing one (WR_CUDA_ERR_STATE where it would have to grow).  Calls of one context share it, so
  * graphs that hold such calls are launched one after another.  Device memory: out has
  * nothing in common with what the call reads (WR_CUDA_ERR_INVAL). */
 int wr_cuda_attn_decode_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uint32_t layer,

@@ -274,6 +274,8 @@ unsigned long long wr_ctx_capture(wr_cuda_ctx *ctx)
 int wr_ctx_keep(wr_cuda_ctx *ctx, size_t bytes, char **out)
 {
     if (bytes > ctx->kept_bytes) {
+        // (a capture would take the clearing of the counters along: calls before its graph runs would find anything there)
+        if (wr_ctx_capture(ctx)) return WR_CUDA_ERR_STATE;
         // (twice as much as before at least: all that is outgrown together is no more than what is in use)
         const size_t want = std::max({bytes, 2 * ctx->kept_bytes, (size_t)8 << 20});
         void *p = nullptr;

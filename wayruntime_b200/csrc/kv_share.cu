@@ -118,11 +118,7 @@ int copy_states(wr_cuda_ctx *ctx, const state_params &p, uint32_t n)
 }
 
 // Sessions change hands on the host, which a graph would not do again when it is launched.
-bool capturing(wr_cuda_ctx *ctx)
-{
-    cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
-    return cudaStreamIsCapturing(ctx->stream, &s) != cudaSuccess || s != cudaStreamCaptureStatusNone;
-}
+bool capturing(wr_cuda_ctx *ctx) { return wr_ctx_capture(ctx) != 0; }
 
 }  // namespace
 

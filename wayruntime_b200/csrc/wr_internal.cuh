@@ -238,7 +238,7 @@ int wr_ctx_try_ws(wr_cuda_ctx *ctx, size_t ws_bytes);
 // Number of the capture that the context's stream is in, 0: none.  (A launch that is captured has not run: what a launch
 // outside its capture may skip on account of it hangs on what really comes before.)
 unsigned long long wr_ctx_capture(wr_cuda_ctx *ctx);
-// Scratch that stays where it is for the context's life: a larger call gets more, elsewhere.  Its first WR_KEPT_HEAD bytes are
+// Scratch that stays where it is for the context's life: a larger call gets more, elsewhere (not in a capture: WR_CUDA_ERR_STATE).  Its first WR_KEPT_HEAD bytes are
 // counters that every launch leaves as zeros (and wr_ctx_sync_checked makes zeros again when a kernel has given up): shared
 // attention's in the first half, those of 65536 requests' beams in the second.
 #define WR_KEPT_HEAD (512u << 10)
