@@ -38,3 +38,39 @@ def test_a_session_given_twice_is_refused(ctx, n):  # noqa: F811
     for kv in (a, f, other):
         kv.close()
     m.close()
+
+
+def test_a_session_forked_in_other_threads_while_it_goes_on(ctx):  # noqa: F811
+    """Calls of a context come from any thread: passes of a session while others fork its beginning, compare and close the forks."""
+    import threading
+    m = dense(ctx)
+    a, toks = started(m, 11, 700), prompt_of(12, 40, 1003)
+    want = [m.forward(m.FWD_DECODE, [a], [700 + i], [t], logits=True)["logits"] for i, t in enumerate(toks)]
+    bad, over = [], threading.Event()
+
+    def forks(seed):
+        rng = np.random.default_rng(seed)
+        try:
+            while not over.is_set():
+                n = int(rng.integers(1, 700))
+                f = a.fork(n)
+                g = f.fork(n // 2)
+                assert a.shared_rows(f) == n // 64 * 64 and g.shared_rows(f) == n // 2 // 64 * 64
+                f.close()
+                g.close()
+        except BaseException as e:      # noqa: BLE001 (told to the thread that asserts)
+            bad.append(e)
+    ts = [threading.Thread(target=forks, args=(i,)) for i in range(3)]
+    for t in ts:
+        t.start()
+    try:
+        for _ in range(3):
+            for i, t in enumerate(toks):
+                assert np.array_equal(m.forward(m.FWD_DECODE, [a], [700 + i], [t], logits=True)["logits"], want[i])
+    finally:
+        over.set()
+        for t in ts:
+            t.join()
+    assert not bad
+    a.close()
+    m.close()

@@ -359,12 +359,12 @@ int wr_decode_step(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *const *kv, uin
                    uint32_t n_rot_pairs, uint32_t flags, float scale_override, uint32_t window, int mem, bool dependent)
 {
     if (!ctx) return WR_CUDA_ERR_INVAL;
+    std::lock_guard<std::mutex> g(ctx->lock);
     int rc = wr_append_validate(ctx, n_sess, kv, layer, positions, 1, k_rows, v_rows, q, n_q_heads,
                                 mem);
     if (rc != WR_CUDA_OK) return rc;
     uint32_t seq_lens[WR_CUDA_BATCH_MAX];
     for (uint32_t s = 0; s < n_sess; ++s) seq_lens[s] = positions[s] + 1;
-    std::lock_guard<std::mutex> g(ctx->lock);
     rc = wr_decode_validate(ctx, n_sess, kv, layer, seq_lens, q, out, n_q_heads, mem, 0);
     if (rc != WR_CUDA_OK) return rc;
     WR_CUDA_TRY(cudaSetDevice(ctx->device));

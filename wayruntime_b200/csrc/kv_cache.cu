@@ -543,11 +543,11 @@ static int kv_rows_xfer(wr_cuda_ctx *ctx, wr_cuda_kv *kv, uint32_t layer, int wh
     if (hd == 0) return WR_CUDA_ERR_UNSUPPORTED;
     if (n == 0) return WR_CUDA_OK;
     if ((uint64_t)row0 + n > kv->max_ctx) return WR_CUDA_ERR_CTX_FULL;
-    if (to_cache && !wr_kv_writable(kv, row0, n)) return WR_CUDA_ERR_STATE;
     if (mem != WR_CUDA_MEM_HOST && mem != WR_CUDA_MEM_DEVICE) return WR_CUDA_ERR_INVAL;
     // device rows move as 16-byte vectors when head_dim allows it
     if (mem == WR_CUDA_MEM_DEVICE && (hd & 7u) == 0 && ((uintptr_t)buf & 15u)) return WR_CUDA_ERR_INVAL;
     std::lock_guard<std::mutex> g(ctx->lock);
+    if (to_cache && !wr_kv_writable(kv, row0, n)) return WR_CUDA_ERR_STATE;
     WR_CUDA_TRY(cudaSetDevice(ctx->device));
     size_t bytes = (size_t)n * n_kv * hd * 2u;
     uint16_t *dbuf = buf;
@@ -952,11 +952,12 @@ extern "C" int wr_cuda_kv_append(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *
                                  uint32_t n_q_heads, float theta_base, uint32_t n_rot_pairs,
                                  uint32_t flags, int mem)
 {
+    if (!ctx) return WR_CUDA_ERR_INVAL;
+    std::lock_guard<std::mutex> g(ctx->lock);
     int rc = wr_append_validate(ctx, n_sess, kv, layer, positions, n_tokens, k_rows, v_rows,
                                 q_rows, n_q_heads, mem);
     if (rc != WR_CUDA_OK) return rc;
     if (n_tokens == 0) return WR_CUDA_OK;
-    std::lock_guard<std::mutex> g(ctx->lock);
     WR_CUDA_TRY(cudaSetDevice(ctx->device));
     const size_t rows = (size_t)n_sess * n_tokens;
     const size_t kv_bytes = rows * kv[0]->n_kv_at(layer) * kv[0]->hd_at(layer) * sizeof(float);

@@ -12,7 +12,7 @@ struct wr_kv_column {
     std::atomic<uint32_t> holders{1};
 };
 
-// Leading pages that both hold.
+// Leading pages that both hold.  (Caller holds ctx->lock, here and below: forking a session makes its list of columns longer.)
 inline uint32_t wr_kv_common_pages(const wr_cuda_kv *a, const wr_cuda_kv *b)
 {
     uint32_t lo = 0, hi = (uint32_t)std::min(a->columns.size(), b->columns.size());

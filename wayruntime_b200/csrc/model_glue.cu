@@ -527,11 +527,13 @@ static int forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_rows
             if (kv[t] == kv[s]) return WR_CUDA_ERR_INVAL;
         for (uint32_t L = 0; L < m->n_layers; ++L)
             if (kv[s]->n_kv_at(L) != m->n_kv || kv[s]->hd_at(L) != m->hd) return WR_CUDA_ERR_INVAL;
-        if (!wr_kv_writable(kv[s], positions[s], mode == WR_CUDA_FWD_DECODE ? 1 : n_rows)) return WR_CUDA_ERR_STATE;
     }
 
     std::lock_guard<std::mutex> fg(m->fwd);
     const auto t_begin = std::chrono::steady_clock::now();
+    std::unique_lock<std::mutex> lock(ctx->lock);        // (another thread may be forking these sessions)
+    for (uint32_t s = 0; s < n_sess; ++s)
+        if (!wr_kv_writable(kv[s], positions[s], mode == WR_CUDA_FWD_DECODE ? 1 : n_rows)) return WR_CUDA_ERR_STATE;
     cudaStream_t st = ctx->stream;
     const uint32_t hid = m->hidden, nq = m->n_q * m->hd, nkv = m->n_kv * m->hd;
 
@@ -568,17 +570,15 @@ static int forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_rows
         }
     }
     wr_settle settle{m};
-    {
-        std::lock_guard<std::mutex> g(ctx->lock);
-        WR_CUDA_TRY(cudaSetDevice(ctx->device));
-        for (uint32_t r = 0; r < n_rows; ++r)
-            m->h_tokens[r] = tokens[mode == WR_CUDA_FWD_DECODE ? perm[r] : r];
-        WR_CUDA_TRY(cudaMemcpyAsync(m->tokens, m->h_tokens, n_rows * sizeof(uint32_t),
-                                    cudaMemcpyHostToDevice, st));
-        embed_rows_kernel<<<n_rows, 128, 0, st>>>(m->tokens, m->embed, m->resid, hid);
-        ++m->launches;
-        WR_CUDA_TRY(cudaGetLastError());
-    }
+    WR_CUDA_TRY(cudaSetDevice(ctx->device));
+    for (uint32_t r = 0; r < n_rows; ++r)
+        m->h_tokens[r] = tokens[mode == WR_CUDA_FWD_DECODE ? perm[r] : r];
+    WR_CUDA_TRY(cudaMemcpyAsync(m->tokens, m->h_tokens, n_rows * sizeof(uint32_t),
+                                cudaMemcpyHostToDevice, st));
+    embed_rows_kernel<<<n_rows, 128, 0, st>>>(m->tokens, m->embed, m->resid, hid);
+    ++m->launches;
+    WR_CUDA_TRY(cudaGetLastError());
+    lock.unlock();
     // More rows than a decode batch go through the tensor cores.  At the line already (two layers, the whole call): 17 rows of width
     // 1024 445 us with the GEMV and 258, 20 of width 2048 855 and 442, 33 of width 4096 3518 and 806.
     const bool wide = mode == WR_CUDA_FWD_PREFILL && n_rows > WR_CUDA_BATCH_MAX && m->prompt;
