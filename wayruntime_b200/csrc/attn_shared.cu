@@ -19,10 +19,12 @@
 //     before this tile's values, so both buffers of S are in use;
 //   * four groups of four warps, each with a quarter of the queries, a thread per key: exponentials against a running reference,
 //     P^T to shared memory (queries contiguous: the MN-major operand); then, a thread per value dimension, the tile's O^T is added
-//     to sums in registers.  The reference moves when a score is more than 2^8 above it: the threads vote, and only then
-//     is the maximum over keys worked out (a segment's first tile always does).
-// Queries and probabilities are split in two F16 numbers (22 bits; queries against a power of two of their row), two
-// products each, the small one first: F32 rows come in and go out, and one F16 rounding of either would leave 2^-12.  Sums of
+//     to sums in registers.  The reference moves when a score is more than 2^8 above the one that it was taken from: the threads vote, and only
+//     then is the maximum over keys worked out (a segment's first tile always does).
+// Queries and weights are split in two F16 numbers, two products each, the small one first: F32 rows come in and go out, and one F16
+// rounding of either would leave 2^-12.  The two leave 2^-22 of a number, or 2^-25 where that is more: F16 ends there.  Queries are
+// taken against a power of two of their row; weights against 2^-7 of the largest one, so what is lost of a weight is 2^-32 of that at most (a
+// long flat tail behind one large score adds up what is lost of its weights).  Sums of
 // one tile stay in the tensor core's accumulator (8 steps of 16 keys behind the small ones), longer ones are F32 additions in
 // registers: the accumulator rounds towards zero, which over a long chunk would show.
 // Every wait is bounded by the context's wait limit.
@@ -47,7 +49,8 @@ constexpr uint32_t kQBytes = 4 * kMaxQ * 128;                                   
 constexpr uint32_t kKSlots = 2, kMaxVSlots = 3, kItemSlots = 8;
 constexpr uint32_t kTmemCols = 512, kTmemO = 256;                                // two buffers of 128 columns each
 constexpr uint32_t kMaxBundles = 64;
-constexpr float kGrow = 8.0f, kLog2e = 1.4426950408889634f;
+// Weights are held against a reference 2^kLift below the largest score; it moves when a score is 2^kGrow above that: 2^15 at most.
+constexpr float kGrow = 8.0f, kLift = 7.0f, kLog2e = 1.4426950408889634f;
 
 // A bundle's columns: its queries, rounded up to a size that the groups of threads are made for.  (High and low parts side by side are 32,
 // 64 or 128 columns, 43, 50 or 64 cycles an instruction; fewer cost what 32 do.)
@@ -784,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                     mask();
 #pragma unroll
                     for (uint32_t j = 0; j < H; j += 4) top = max3_nan(max3_nan(top, s[j], s[j + 1]), s[j + 2], s[j + 3]);
-                    moved = group_or(bar, 128, !(top <= kGrow));     // (or not a number)
+                    moved = group_or(bar, 128, !(top <= kGrow + kLift));     // (or not a number)
                 }
                 if (moved) {                                     // (the same in all threads of the group)
                     scores(true);
@@ -797,11 +800,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(const __grid_c
                     group_sync(bar);
                     if (tid < H) {
                         const float4 w = *reinterpret_cast<const float4 *>(sm.red[q0 + tid]);
-                        const float top = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), WR_NEG_SENTINEL);
+                        const float ref = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), WR_NEG_SENTINEL) - kLift;
                         const float old = fresh ? WR_NEG_SENTINEL : -sm.nm[q0 + tid];
-                        const bool up = fresh || top > old + kGrow;
-                        sm.a[q0 + tid] = up ? ex2(old - top) : 1.f;
-                        if (up) sm.nm[q0 + tid] = -top;
+                        const bool up = fresh || ref > old + kGrow;
+                        sm.a[q0 + tid] = up ? ex2(old - ref) : 1.f;
+                        if (up) sm.nm[q0 + tid] = -ref;
                     }
                     group_sync(bar);
 #pragma unroll
