@@ -295,7 +295,8 @@ int wr_cuda_decode_step_shared(wr_cuda_ctx *ctx, uint32_t n_sess, wr_cuda_kv *co
  * F32 [n_groups][beams] (a beam at -inf or NaN has ended and its row is not read);
  * out_*: [n_groups][n_out].  Tokens with a logit of -inf are no continuations, nor is any of a row
  * with a NaN or +inf; places for which there is none hold score -inf, beam and token
- * 0xffffffff.  Totals are compared in 64 bits and returned in F32.  beams <=
+ * 0xffffffff.  Totals are compared in 64 bits and returned in F32; a row's log of its sum, which is an F32 one, is good to some
+ * 1e-7, and the same for rows of a call that hold the same logits.  beams <=
  * WR_CUDA_BATCH_MAX, n_out <= WR_CUDA_BEAM_MAX_OUT, n_groups * beams <= 65535
  * (WR_CUDA_ERR_LIMIT).  Scratch and device memory as wr_cuda_attn_decode_shared, but with n_out ==
  * beams out_scores may be scores. */

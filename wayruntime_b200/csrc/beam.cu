@@ -4,8 +4,10 @@
 //
 // One pass over the logits: a CTA takes a part of a row and leaves the part's sum of exponentials (against the part's
 // maximum) and its n_out best logits; within a row totals are in the order of logits, so nothing else of the part can be
-// among the row's best.  The CTA that is the last of its request puts the parts together: sums and totals in 64 bits,
-// since candidates of two beams may lie closer than an F32 rounding.  Measured on a B200: one row of 32003 logits, 8 out, 7.2 us on
+// among the row's best.  The CTA that is the last of its request puts the parts together.  Totals are 64-bit, since candidates of two
+// beams may lie closer than an F32 rounding; a part's sum is F32 (a thread's terms, ex2.approx, then lanes and warps against the largest maximum),
+// the parts' are added up in 64 bits: a row's logarithm is off by up to 4.3e-7 (16 rows of 1000 to 600000 logits of spread 0 to 6, in parts of one
+// batch and of 37).  Rows of a call that are alike have sums alike, to the bit, so that their candidates tie.  Measured on a B200: one row of 32003 logits, 8 out, 7.2 us on
 // the device, round trips one behind the other (a second kernel for the parts took 2 us more); 256 rows of 65536, 16 out, 20.4 us,
 // 3.3 TB/s, bound by instructions (comparing with the bound four logits at a time took 1.2 us off; more batches under way, two or three
 // copies to shared memory a CTA, made it 24.7 and 26.0 us).
@@ -33,6 +35,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 struct BeamParams {
     wr_beam_args a;
     uint32_t parts, batches;             // parts of a row; batches of a part
+    bool vectors;                        // all rows begin on 16 bytes
     float2 *sums;                        // [row][part]: largest logit, sum of exponentials against it
     uint2 *best;                         // [row][part][n_out]: logit's bits, token; in order
     int *done;                           // [request]: parts that are there
@@ -134,14 +137,17 @@ __device__ __forceinline__ float bound_of_all(float (&top)[32], float v, uint32_
     __syncthreads();
     return __shfl_sync(0xffffffffu, warp_sort(top[lane], lane), k - 1);
 }
-// sums of exponentials against two maxima as one
-__device__ __forceinline__ void join(float &m, float &s, float m2, float s2)
+// The lanes' sums of exponentials, each against its own maximum, as one.
+__device__ __forceinline__ float warp_max(float v) { return value(__reduce_max_sync(0xffffffffu, order(v))); }
+__device__ __forceinline__ float shrunk(float from, float to) { return ex2((from - (to == -INFINITY ? 0.f : to)) * kLog2e); }
+template <typename T> __device__ __forceinline__ void warp_join(float &m, T &s)
 {
-    const float t = fmaxf(m, m2), base = t == -INFINITY ? 0.f : t;
-    s = s * ex2((m - base) * kLog2e) + s2 * ex2((m2 - base) * kLog2e);
-    m = t;
+    const float top = warp_max(m);
+    s *= (T)shrunk(m, top);
+    m = top;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
 }
-
 // A bound, as the whole number in whose order it is, that k entries reach as well as the given one, but no more than `enough` where such a one
 // is found: halving what lies between that and the largest.  reach(x): how many of the thread's own reach x.  The CTA meets in it.
 template <typename Reach> __device__ __forceinline__ uint32_t higher_bound(uint32_t (&counts)[2][kWarps], Reach reach, uint32_t lo, uint32_t hi, uint32_t k,
@@ -172,17 +178,29 @@ __device__ __forceinline__ void part_of_row(const BeamParams &p, PartMemory &sm,
         if (threadIdx.x < k) best[threadIdx.x] = make_uint2(__float_as_uint(-INFINITY), kNone);
         return;
     }
-    // Vectors are aligned in memory: the row begins `lead` elements into the first one.
+    // Which tokens a thread takes is the same in all rows of a call, so rows alike have sums alike, to the bit.  Four neighbours at a time where every
+    // row is aligned (p.vectors), else every 256th: a warp's loads are neighbours then.
     const float *const x = row_of(p.a, row);
-    const uint32_t lead = (uint32_t)((uintptr_t)x >> 2) & 3u;
-    const float *const aligned = x - lead;
-    const uint32_t first = part * p.batches * kBatch, end = p.a.vocab + lead;      // (below 2^32: a vocabulary is below 2^31)
+    const uint32_t first = part * p.batches * kBatch, end = p.a.vocab;       // (below 2^31; a batch more is below 2^32)
     auto load = [&](uint32_t b, float (&v)[4 * kVecs]) {
         const uint32_t lo = first + b * kBatch;
-        if (lo && lo + kBatch <= end) {
+        const bool whole = lo + kBatch <= end;
+        if (!p.vectors) {
+            const float *const from = x + lo + threadIdx.x;
+            if (whole) {
+#pragma unroll
+                for (uint32_t e = 0; e < 4 * kVecs; ++e) v[e] = __ldcs(from + kThreads * e);
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 4 * kVecs; ++e) v[e] = lo + threadIdx.x + kThreads * e < end ? __ldcs(from + kThreads * e) : -INFINITY;
+            }
+            return;
+        }
+        const float4 *const from = reinterpret_cast<const float4 *>(x + lo) + threadIdx.x;
+        if (whole) {
 #pragma unroll
             for (uint32_t u = 0; u < kVecs; ++u) {
-                const float4 w = __ldcs(reinterpret_cast<const float4 *>(aligned + lo) + u * kThreads + threadIdx.x);
+                const float4 w = __ldcs(from + u * kThreads);
                 v[4 * u] = w.x; v[4 * u + 1] = w.y; v[4 * u + 2] = w.z; v[4 * u + 3] = w.w;
             }
             return;
@@ -190,16 +208,18 @@ __device__ __forceinline__ void part_of_row(const BeamParams &p, PartMemory &sm,
 #pragma unroll
         for (uint32_t u = 0; u < kVecs; ++u) {
             const uint32_t at = lo + (u * kThreads + threadIdx.x) * 4u;
-            if (at >= lead && at + 4 <= end) {
-                const float4 w = __ldcs(reinterpret_cast<const float4 *>(aligned + at));
+            if (at + 4 <= end) {
+                const float4 w = __ldcs(from + u * kThreads);
                 v[4 * u] = w.x; v[4 * u + 1] = w.y; v[4 * u + 2] = w.z; v[4 * u + 3] = w.w;
             } else {
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) v[4 * u + e] = at + e >= lead && at + e < end ? __ldcs(aligned + at + e) : -INFINITY;
+                for (uint32_t e = 0; e < 4; ++e) v[4 * u + e] = at + e < end ? __ldcs(x + at + e) : -INFINITY;
             }
         }
     };
-    auto token_of = [&](uint32_t b, uint32_t e) { return first + b * kBatch + ((e / 4) * kThreads + threadIdx.x) * 4u + (e & 3) - lead; };
+    auto token_of = [&](uint32_t b, uint32_t e) {
+        return first + b * kBatch + (p.vectors ? ((e / 4) * kThreads + threadIdx.x) * 4u + (e & 3) : e * kThreads + threadIdx.x);
+    };
     float v[4 * kVecs], next[4 * kVecs], m = -INFINITY, bound = -FLT_MAX;
     uint64_t s2 = 0;                     // two sums of exponentials
     load(0, v);
@@ -251,18 +271,16 @@ __device__ __forceinline__ void part_of_row(const BeamParams &p, PartMemory &sm,
     float s, half;
     unpack2(s2, s, half);
     s += half;
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), other = __shfl_xor_sync(0xffffffffu, s, o);
-        join(m, s, m2, other);
-    }
+    warp_join(m, s);
     if (lane == 0) {
         sm.warp_m[warp] = m;
         sm.warp_s[warp] = s;
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (uint32_t w = 1; w < kWarps; ++w) join(m, s, sm.warp_m[w], sm.warp_s[w]);
+        s = 0.f;
+        for (uint32_t w = 1; w < kWarps; ++w) m = fmaxf(m, sm.warp_m[w]);
+        for (uint32_t w = 0; w < kWarps; ++w) s = fmaf(sm.warp_s[w], shrunk(sm.warp_m[w], m), s);
         p.sums[(size_t)row * p.parts + part] = make_float2(m, s);
     }
     uint32_t n = sm.n_listed;
@@ -336,17 +354,16 @@ __device__ __forceinline__ void parts_of_request(const BeamParams &p, FinalMemor
     if (threadIdx.x == 0) sm.n = 0;
     // score less the logarithm of the row's sum
     for (uint32_t b = warp; b < beams; b += kWarps) {
-        float m = -INFINITY, s = 0.f;
+        float m = -INFINITY;
+        double s = 0.0;
         for (uint32_t i = lane; i < p.parts; i += 32) {
             const float2 ms = __ldcg(p.sums + (row0 + b) * p.parts + i);
-            join(m, s, ms.x, ms.y);
+            const float top = fmaxf(m, ms.x);
+            s = s * (double)shrunk(m, top) + (double)ms.y * (double)shrunk(ms.x, top);
+            m = top;
         }
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) {
-            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-            join(m, s, m2, s2);
-        }
-        const double t = (double)p.a.scores[row0 + b] - ((double)m + log((double)s));
+        warp_join(m, s);
+        const double t = (double)p.a.scores[row0 + b] - ((double)m + log(s));
         if (lane == 0) sm.offset[b] = t > -INFINITY && t < INFINITY ? t : -INFINITY;         // (no sum, or none that is finite)
     }
     __syncthreads();
@@ -485,9 +502,10 @@ int wr_beam_launch(wr_cuda_ctx *ctx, const wr_beam_args &a)
 {
     BeamParams p{};
     p.a = a;
-    const uint32_t rows = a.groups * a.beams, most = (uint32_t)(((uint64_t)a.vocab + 3 + kBatch - 1) / kBatch);
+    const uint32_t rows = a.groups * a.beams, most = (uint32_t)(((uint64_t)a.vocab + kBatch - 1) / kBatch);
     // As many CTAs as the SMs hold at once.  (Twice as many: 26.7 instead of 22.1 us for 256 rows, 11.7 instead of 11.3 for 16.)
     const uint32_t want = std::min(std::max(kCtas * (uint32_t)ctx->sm_count / rows, 1u), std::min(most, kMaxLists / a.beams));
+    p.vectors = ((uintptr_t)a.logits & 15u) == 0 && a.ld % 4 == 0;
     p.batches = (most + want - 1) / want;
     p.parts = (most + p.batches - 1) / p.batches;
     const size_t n = (size_t)rows * p.parts, sums = (n * sizeof(float2) + 255) & ~(size_t)255;
