@@ -156,13 +156,14 @@ class Engine:
         """The best continuations of a prompt, at most `beams`, as Hypothesis, by score / length ** length_penalty.  One ends
         with a stop id or after max_new tokens; the search ends when `beams` have ended and none that goes on ranks above
         the last of them as it stands.  The beams' sessions are forks of the prompt's: its pages are kept once, and a step
-        attends to them once for all beams where the model's stack does that (wr_cuda_model_beam_step)."""
+        attends to them once for all beams where the model's stack does that (wr_cuda_model_beam_step).  Any number of stop ids: a step that
+        may have to pass over more of them than one choice on the device has places for chooses per beam (beams + stop ids at most
+        32), beyond that on the host."""
         stop = frozenset(stop)
         if not prompt or max_new < 1:
             raise ValueError("a prompt token and a new one at least")
         if not 1 <= beams <= BATCH_MAX:
             raise ValueError(f"1 to {BATCH_MAX} beams")
-        m, n_out = self.model, min((1 + len(stop)) * beams, BEAM_MAX_OUT)
         sessions, histories, ended = [self.session(len(prompt) + max_new)], [[]], []
         rank = lambda h: h.rank(length_penalty)  # noqa: E731
         try:
@@ -171,12 +172,12 @@ class Engine:
             tokens, scores = [prompt[-1]], [0.0]
             while True:
                 live = sessions[:len(tokens)]
-                found = m.beam_step([s.kv for s in live], [s.pos for s in live], tokens, [scores], n_out)
+                found = self._continuations(live, tokens, scores, beams, len(stop))
                 for s in live:
                     s.pos += 1
                 going = []                               # (score, parent, token), best first
-                for place, (score, parent, token) in enumerate(zip(*(x[0].tolist() for x in found))):
-                    if parent == NO_BEAM or len(going) == beams:
+                for place, (score, parent, token) in enumerate(found):
+                    if len(going) == beams:
                         break
                     if token not in stop:
                         going.append((score, parent, token))
@@ -197,6 +198,34 @@ class Engine:
             for s in sessions:
                 s.close()
         return sorted(ended, key=rank, reverse=True)[:beams]
+
+    def _continuations(self, live, tokens, scores, beams, stops):
+        """A step of all live beams, and its continuations as (score, parent, token), best first: as far as `beams` that are not among
+        `stops` ids lie."""
+        m, kvs, at, places = self.model, [s.kv for s in live], [s.pos for s in live], (1 + stops) * beams
+        if places <= BEAM_MAX_OUT:
+            found = zip(*(x[0].tolist() for x in m.beam_step(kvs, at, tokens, [scores], places)))
+            return [c for c in found if c[1] != NO_BEAM]
+        # More places than one choice has: from every beam as many as can be among them, put together here.  (Of one beam's, `beams` are none
+        # of the stop ids behind which the others lie.)
+        each = beams + stops
+        if each <= BEAM_MAX_OUT:
+            s, b, t = (x.tolist() for x in m.beam_step(kvs, at, tokens, [[x] for x in scores], each))
+            found = [(s[p][i], p, t[p][i]) for p in range(len(live)) for i in range(each) if b[p][i] != NO_BEAM]
+        else:
+            found = []
+            for p, row in enumerate(m.forward(m.FWD_DECODE, kvs, at, tokens, logits=True)["logits"]):
+                row = row.astype(np.float64)
+                top = row.max()
+                if not np.isfinite(top):                 # (no continuation, or a logit that is not a number)
+                    continue
+                total = scores[p] + (row - (top + np.log(np.exp(row - top).sum())))
+                least = np.partition(total, -each)[-each] if each < len(total) else -np.inf
+                best = np.flatnonzero((total >= least) & (row > -np.inf))
+                best = best[np.argsort(-total[best], kind="stable")][:each]
+                found += [(float(total[t]), p, int(t)) for t in best]
+        found.sort(key=lambda c: -c[0])                  # (stable: equal ones by beam, then token)
+        return [(float(np.float32(s)), p, t) for s, p, t in found[:places]]
 
     def _follow(self, sessions, parents, beams):
         """Sessions [0, len(parents)) go on from those that parents names.  The others wait until there are more beams again."""
