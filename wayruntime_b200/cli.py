@@ -56,8 +56,10 @@ def main(argv=None) -> int:
     g.add_argument("--length-penalty", type=float, default=1.0, help="beams rank by score / length ** this")
     g.add_argument("--device", type=int, default=0)
     a = ap.parse_args(argv)
-    if a.command == "generate" and a.beams and a.temperature:
-        ap.error("--beams takes the most probable continuations: no --temperature")
+    if a.command == "generate" and a.beams:
+        for option in ("temperature", "top_k", "top_p", "seed"):
+            if getattr(a, option) != g.get_default(option):
+                ap.error(f"--beams takes the most probable continuations: no --{option.replace('_', '-')}")
     if a.command == "models":
         from . import models
         print("\n".join(models.architectures()))
