@@ -453,11 +453,17 @@ int wr_cuda_model_forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t
                           float *normed_out, float *const *logits_out, uint32_t *argmax_out,
                           float *attn_tap_out);
 
+/* Whether decode passes of wr_cuda_model_forward attend together to long beginnings that sessions hold together (wr_cuda_kv_fork; the
+ * dense stack).  Not unless asked: a session's result does not depend on which others share the call.  Together,
+ * shared pages are fetched once for all, and the order of a session's sums hangs on the lengths of all of them. */
+int wr_cuda_model_set_together(wr_cuda_model *m, int on);
+
 /* One step of beam searches: a decode pass (as wr_cuda_model_forward, WR_CUDA_FWD_DECODE) of
  * n_groups * beams <= WR_CUDA_BATCH_MAX rows, then wr_cuda_beam_select on its logits, which
  * stay on the device.  Either kind of model.  scores and out_* are host memory; kv,
  * positions and tokens are as for the pass.  Sessions of the dense stack that hold pages together
- * attend to them together where those are long enough to pay. */
+ * attend to them together where those are long enough to pay, whatever wr_cuda_model_set_together says: a beam's
+ * result is that of the pass to rounding. */
 int wr_cuda_model_beam_step(wr_cuda_ctx *ctx, wr_cuda_model *m, uint32_t n_groups, uint32_t beams,
                             wr_cuda_kv *const *kv, const uint32_t *positions, const uint32_t *tokens,
                             const float *scores, uint32_t n_out, float *out_scores,

@@ -48,8 +48,9 @@ def test_search_with_many_stop_ids(ctx, build, n, beams, stops):  # noqa: F811
     want, largest = plain_search(engine, prompt, beams, max_new, stop)
     assert [h.tokens for h in got] == [t for t, _ in want]
     for h, (_, s) in zip(got, want):
-        # each step's total: rounded, its sum within choose_error, and both the logit and the sum off by 1e-4 of the largest
-        # logit where attention goes another way (the dense stack's, together)
+        # Each step's total: rounded, its sum within choose_error, and, where attention goes another way (the dense stack's, together), the
+        # logit and the sum off by 1e-4 of the largest logit each: 1e-5 of a row's norm in each of two layers' attention (both ways within
+        # 5e-6 of 64 bits), which the two factors of a feed-forward and the norms before it and the head double at most each.
         bound = len(h.tokens) * (choose_error(np.array([s]), m.vocab)[0] + (2e-4 * largest if build is dense else 0.0))
         assert abs(h.score - s) <= bound
     m.close()

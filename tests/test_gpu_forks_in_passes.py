@@ -74,3 +74,73 @@ def test_a_session_forked_in_other_threads_while_it_goes_on(ctx):  # noqa: F811
     assert not bad
     a.close()
     m.close()
+
+
+def family_pass(m):
+    """A pass over two families, one of them with a short beginning, and sessions by themselves, in an order that mixes them."""
+    a, b, c, d, e = started(m, 1, 400), started(m, 2, 1200), started(m, 3, 90), started(m, 4, 1100), started(m, 5, 30)
+    fa, fb, fc = [a.fork(400) for _ in range(2)], b.fork(1200), c.fork(90)
+    return [e, fa[0], b, c, fa[1], d, fc, a, fb], [30, 400, 1200, 90, 400, 1100, 90, 400, 1200], prompt_of(9, 9, m.vocab)
+
+
+@pytest.mark.parametrize("qk_norm", [True, False])
+def test_a_forks_result_does_not_hang_on_who_shares_the_call(ctx, qk_norm):  # noqa: F811
+    """To the bit, as for sessions that share nothing."""
+    m = dense(ctx, qk_norm=qk_norm)
+    kvs, pos, toks = family_pass(m)
+
+    def run(rows):
+        got = m.forward(m.FWD_DECODE, [kvs[i] for i in rows], [pos[i] for i in rows], [toks[i] for i in rows], logits=True, attn_tap=True)
+        return {i: (got["logits"][j], got["attn"][:, j]) for j, i in enumerate(rows)}
+    alone = {}
+    for i in range(9):
+        alone.update(run([i]))
+    for rows in (list(range(9)), [8, 2, 5], [1, 4, 7], [7, 1], [6, 0, 3, 8, 1]):
+        for i, (logits, attn) in run(rows).items():
+            assert np.array_equal(logits, alone[i][0]) and np.array_equal(attn, alone[i][1]), (rows, i)
+    for kv in kvs:
+        kv.close()
+    m.close()
+
+
+def test_together_when_asked(ctx):  # noqa: F811
+    """Attention to rounding; asked no longer, the bits are those of before."""
+    m = dense(ctx)
+    kvs, pos, toks = family_pass(m)
+
+    def run():
+        return m.forward(m.FWD_DECODE, kvs, pos, toks, hidden=True, logits=True, argmax=True, attn_tap=True)
+    apart = run()
+    m.set_together()
+    got = run()
+    m.set_together(False)
+    again = run()
+    assert np.array_equal(apart["logits"], again["logits"]) and np.array_equal(apart["attn"], again["attn"])
+    # (the first layer's attention has the same queries and keys: F32 sums in two orders, each near 64 bits to 5e-6 of its norm)
+    for i in range(9):
+        x, y = got["attn"][0, i], apart["attn"][0, i]
+        assert np.linalg.norm(x - y) <= 1e-5 * np.linalg.norm(y), i
+        assert got["argmax"][i] == np.argmax(got["logits"][i])
+    alone = {0, 3, 5, 6}                                 # those that hold nothing long together go the way they went
+    assert all(np.array_equal(got["logits"][i], apart["logits"][i]) == (i in alone) for i in range(9))
+    for kv in kvs:
+        kv.close()
+    m.close()
+
+
+def test_a_beam_step_attends_together(ctx):  # noqa: F811
+    """Without being asked: its choice is that from the logits of a pass that was asked to."""
+    from _plain_beams import choose, choose_error
+    m = dense(ctx)
+    a = started(m, 21, 700)
+    kvs, pos, toks = [a] + [a.fork(700) for _ in range(3)], [700] * 4, prompt_of(22, 4, m.vocab)
+    scores = np.array([[-1.0, -1.5, -1.25, -2.0]], np.float32)
+    got = m.beam_step(kvs, pos, toks, scores, 8)
+    m.set_together()
+    rows = m.forward(m.FWD_DECODE, kvs, pos, toks, logits=True)["logits"]
+    want = choose(rows[None], scores, 8)
+    assert np.array_equal(got[1], want[1]) and np.array_equal(got[2], want[2])
+    assert (np.abs(got[0] - want[0]) <= choose_error(want[0], m.vocab)).all()
+    for kv in kvs:
+        kv.close()
+    m.close()

@@ -49,7 +49,7 @@ EXPORTS = [
     "wr_cuda_model_forward", "wr_cuda_kv_create_layout", "wr_cuda_model_create_mixed", "wr_cuda_model_kv_create",
     "wr_cuda_model_set_hidden_tap",
     "wr_cuda_kv_fork", "wr_cuda_kv_shared_rows", "wr_cuda_kv_reorder", "wr_cuda_attn_decode_shared", "wr_cuda_decode_step_shared",
-    "wr_cuda_beam_select", "wr_cuda_model_beam_step",
+    "wr_cuda_beam_select", "wr_cuda_model_beam_step", "wr_cuda_model_set_together",
 ]
 
 
@@ -192,6 +192,7 @@ def load_library():
                                              vp, vp, vp, vp, u32, f32, u32, u32, f32, i32]),
         "wr_cuda_beam_select": (i32, [vp, u32, u32, u32, vp, vp, u32, vp, vp, vp, i32]),
         "wr_cuda_model_beam_step": (i32, [vp, vp, u32, u32, C.POINTER(vp), C.POINTER(u32), C.POINTER(u32), vp, u32, vp, vp, vp]),
+        "wr_cuda_model_set_together": (i32, [vp, i32]),
         "wr_cuda_model_forward": (i32, [vp, vp, i32, u32, C.POINTER(vp), C.POINTER(u32), C.POINTER(u32), u32,
                                         vp, vp, C.POINTER(vp), C.POINTER(u32), vp]),
     }
@@ -723,6 +724,11 @@ class DeviceModel:
         if attn_tap: res["attn"] = tap
         return res
 
+
+    def set_together(self, on=True):
+        """wr_cuda_model_set_together: decode passes read long beginnings that sessions hold together once for all of them; a session's
+        result then hangs, to rounding, on the others of the call."""
+        _check(self._lib.wr_cuda_model_set_together(self._h, bool(on)), "wr_cuda_model_set_together")
 
     def kv_reorder(self, kvs, parents, rows):
         """Context.kv_reorder for sessions of this model."""

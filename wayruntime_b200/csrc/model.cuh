@@ -37,6 +37,7 @@ struct wr_cuda_model {
     uint32_t *h_tokens = nullptr;        // pinned: token ids in, arg-max ids out
     float *beam_host = nullptr, *beam_dev = nullptr;     // a beam step's scores in, its choice out (pinned, device); from the first one on
     uint32_t ffn_max = 0;
+    bool together = false;               // wr_cuda_model_set_together
     uint64_t launches = 0;
     uint64_t last_enqueue_ns = 0;        // host time the last forward pass spent before it began to wait
     // Decode steps that hold short and long sessions attend to the short ones on a stream of their own.

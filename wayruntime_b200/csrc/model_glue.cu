@@ -539,8 +539,8 @@ static int forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_rows
 
     // Decode rows are processed in an order of their own: the sessions that the one-kernel
     // short-context step covers first, the others after them, those that hold a long beginning
-    // together last, so that each kind is a contiguous block of rows.  Which of the first two kinds a session is
-    // depends on that session alone.  perm[i] = caller's row.
+    // together last where they attend together, so that each kind is a contiguous block of rows.  Which of the first two kinds a
+    // session is depends on that session alone.  perm[i] = caller's row.
     uint32_t perm[WR_CUDA_BATCH_MAX], pos_p[WR_CUDA_BATCH_MAX], n_short = 0, n_apart = 0, n_groups = 0;
     uint32_t group_sess[WR_CUDA_BATCH_MAX], group_rows[WR_CUDA_BATCH_MAX];
     wr_cuda_kv *kv_p[WR_CUDA_BATCH_MAX];
@@ -548,7 +548,8 @@ static int forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_rows
     if (mode == WR_CUDA_FWD_DECODE) {
         const bool use_small = (getenv("WR_CUDA_STEP_SMALL_OFF") == nullptr);
         uint32_t together[WR_CUDA_BATCH_MAX];            // rows
-        n_apart = n_rows - rows_together(m, n_rows, kv, together, &n_groups, group_sess, group_rows);
+        n_apart = n_rows;
+        if (m->together || beam) n_apart -= rows_together(m, n_rows, kv, together, &n_groups, group_sess, group_rows);
         bool apart[WR_CUDA_BATCH_MAX];
         std::fill(apart, apart + n_rows, true);
         for (uint32_t i = 0; i < n_rows - n_apart; ++i) {
@@ -798,6 +799,14 @@ static int forward(wr_cuda_ctx *ctx, wr_cuda_model *m, int mode, uint32_t n_rows
             if (c >= out_from) argmax_out[c - out_from] = m->h_tokens[m->max_rows + i];
         }
     if (beam) wr_beam_step_finish(m, *beam);
+    return WR_CUDA_OK;
+}
+
+extern "C" int wr_cuda_model_set_together(wr_cuda_model *m, int on)
+{
+    if (!m) return WR_CUDA_ERR_INVAL;
+    std::lock_guard<std::mutex> fg(m->fwd);
+    m->together = on != 0;
     return WR_CUDA_OK;
 }
 
