@@ -40,3 +40,23 @@ def test_totals_nearer_than_an_f32_rounding(ctx, vocab):  # noqa: F811
     assert np.array_equal(beam, want[1]) and np.array_equal(token, want[2])
     assert np.array_equal(beam, np.tile(np.argsort(-steps), (5, 2)))
     assert all(len(set(score[g, :4])) == 1 for g in range(5))
+
+
+@pytest.mark.parametrize("vocab", [1000, 4097, 32003, 151936])
+@pytest.mark.parametrize("spread", [1.0, 2.5, 6.0])
+def test_a_rows_sum(ctx, vocab, spread):  # noqa: F811
+    """Totals near zero, so that what is left of them is the error of the row's sum; rows one by one, and many of them in long parts."""
+    x, _ = rows(vocab, 1, 4, vocab, spread)
+    wide = x[0].astype(np.float64)
+    top = wide.max(-1)
+    lse = top + np.log(np.exp(wide - top[:, None]).sum(-1))
+    scores = (lse - top).astype(np.float32)
+    want = scores + (top - lse)
+    for repeat, batches in ((1, 1), (160, -(-vocab // 4096))):       # (640 rows: a part is a whole row)
+        got = run(ctx, np.tile(x[0], (repeat, 1))[:, None], np.tile(scores, repeat)[:, None], 1)[0].reshape(repeat, 4)
+        # A term: ex2.approx 2^-22, its argument rounded twice (|d| e^d <= 0.37, in powers of two 0.54 * 2^-24 each).  Sums: a lane's two
+        # accumulators, 8 terms a batch each and one rescaling; then the two, 5 steps across lanes, 8 warps, each of the two maxima's factors 2^-22 and
+        # two roundings, the part's sum rounded.  (Parts and the total are added up in 64 bits; the result's own rounding is relative to nearly zero.)
+        rel = 2.0 ** -22 + 2 * 0.54 * 2.0 ** -24 + batches * (8 * 2.0 ** -24 + 2.0 ** -22) + (1 + 5 + 8) * 2.0 ** -24 + 3 * (2.0 ** -22 + 2.0 ** -23)
+        assert np.abs(got - want).max() <= rel
+        assert (got == got[0]).all()
