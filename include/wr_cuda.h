@@ -242,7 +242,8 @@ int wr_cuda_attn_prefill(wr_cuda_ctx *ctx, wr_cuda_kv *kv, uint32_t layer,
  * are copied (enqueued), and so is the recurrent state, which has to stand at
  * n_rows (WR_CUDA_ERR_STATE).  A fork can be forked again.  While more than one
  * session holds a page nobody may write it: an append, a write_rows or a
- * forward pass that would is WR_CUDA_ERR_STATE before anything runs.  Destroying a
+ * forward pass that would is WR_CUDA_ERR_STATE before anything runs (what a graph has captured is not looked at again
+ * when it is launched: launches that write such a page are captured anew).  Destroying a
  * session gives back what no other holds.  Takes memory for the fork's own
  * pages; not while the context's stream is being captured (WR_CUDA_ERR_STATE). */
 int wr_cuda_kv_fork(wr_cuda_ctx *ctx, wr_cuda_kv *kv, uint32_t n_rows, wr_cuda_kv **out);

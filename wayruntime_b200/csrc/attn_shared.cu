@@ -28,7 +28,7 @@
 // one tile stay in the tensor core's accumulator (8 steps of 16 keys behind the small ones), longer ones are F32 additions in
 // registers: the accumulator rounds towards zero, which over a long chunk would show.
 // Every wait is bounded by the context's wait limit.
-// Measured on a B200, F32 rows, 32 query and 8 kv heads, one launch behind another: 16 sessions behind 32768 rows, 145 MB, 33.2 us, of which
+// Measured on a B200, F32 rows, 32 query and 8 kv heads, one launch behind another: 16 sessions behind 32768 rows, 145 MB, 33 us, of which
 // the tiles take 23.3 at 6.4 TB/s (the copy bandwidth is 6.54; after 50 ms of nothing else the GPU is at its 1000 W, the SMs at 1690
 // instead of 1965 MHz, and it is 39 us); 4 sessions behind 2011 rows 9.5 us, 2 behind 150 rows 6.5 us on the device.  What the tiles do not take, 10 us of a large launch, is its ends: queries 1.7, the last values 0.9, parts written
 // and seen by the others 2, adding them up 2.5, the rest the launch itself.  Head dim 128 only: a tile's rings take the SM's shared memory.

@@ -7,9 +7,9 @@
 // among the row's best.  The CTA that is the last of its request puts the parts together.  Totals are 64-bit, since candidates of two
 // beams may lie closer than an F32 rounding; a part's sum is F32 (a thread's terms, ex2.approx, then lanes and warps against the largest maximum),
 // the parts' are added up in 64 bits: a row's logarithm is off by up to 4.3e-7 (16 rows of 1000 to 600000 logits of spread 0 to 6, in parts of one
-// batch and of 37).  Rows of a call that are alike have sums alike, to the bit, so that their candidates tie.  Measured on a B200: one row of 32003 logits, 8 out, 7.2 us on
-// the device, round trips one behind the other (a second kernel for the parts took 2 us more); 256 rows of 65536, 16 out, 20.4 us,
-// 3.3 TB/s, bound by instructions (comparing with the bound four logits at a time took 1.2 us off; more batches under way, two or three
+// batch and of 37).  Rows of a call that are alike have sums alike, to the bit, so that their candidates tie.  Measured on a B200: one row of 32003 logits, 8 out, 7.0 us on
+// the device, round trips one behind the other (a second kernel for the parts took 2 us more); 256 rows of 65536, 16 out, 18.8 us,
+// 3.6 TB/s (67 MB, which stay in L2; 22.6 us from HBM), bound by instructions (comparing with the bound four logits at a time took 1.2 us off; more batches under way, two or three
 // copies to shared memory a CTA, made it 24.7 and 26.0 us).
 //
 // Candidates are found with a threshold that is sure to keep n_out of them: of 32 threads' maxima (distinct elements) the
@@ -179,7 +179,8 @@ __device__ __forceinline__ void part_of_row(const BeamParams &p, PartMemory &sm,
         return;
     }
     // Which tokens a thread takes is the same in all rows of a call, so rows alike have sums alike, to the bit.  Four neighbours at a time where every
-    // row is aligned (p.vectors), else every 256th: a warp's loads are neighbours then.
+    // row is aligned (p.vectors), else every 256th: a warp's loads are neighbours then.  (32 x 8 rows of 65537: 19.9 us; four neighbours by single
+    // loads 22.2.  Every 32nd leaves a part of few logits to one warp, whose four largest are a low bound: 4 x 151937 11.7 instead of 7.9.)
     const float *const x = row_of(p.a, row);
     const uint32_t first = part * p.batches * kBatch, end = p.a.vocab;       // (below 2^31; a batch more is below 2^32)
     auto load = [&](uint32_t b, float (&v)[4 * kVecs]) {
