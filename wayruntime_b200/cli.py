@@ -26,7 +26,7 @@ def generate(a) -> int:
         if a.beams:
             for p in prompts:
                 best = Engine(model).beam_search(p, a.beams, a.max_new, a.stop, a.length_penalty)
-                print(json.dumps({"prompt": p, "output": best[0].tokens, "score": best[0].score,
+                print(json.dumps({"prompt": p, "output": best[0].tokens if best else [], "score": best[0].score if best else None,
                                   "beams": [{"output": h.tokens, "score": h.score} for h in best]}))
             return 0
         for r in Engine(model).run(reqs):
